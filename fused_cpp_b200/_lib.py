@@ -6,6 +6,7 @@ ABI.  Workspaces come from torch's caching allocator and are cached per (device,
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -45,7 +46,7 @@ EXPORTS = (
     "fmoe_stage_timer_create", "fmoe_stage_timer_destroy", "fmoe_stage_timer_reset", "fmoe_stage_timer_calls",
     "fmoe_stage_timer_read", "fmoe_route_build_noalloc", "fmoe_ep_dispatch_workspace_bytes", "fmoe_ep_dispatch_prepare",
     "fmoe_w8a8_expert_rows_forward", "fmoe_bf16_expert_rows_forward", "fmoe_ep_combine_finish",
-    "fmoe_i8gemm_dynamic_scaled_mm_pair",
+    "fmoe_i8gemm_dynamic_scaled_mm_pair", "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward", "fmoe_dense_status",
     "fmoe_router_topk", "fmoe_append_shared_route",
     "fmoe_ep_peer_create", "fmoe_ep_peer_handle", "fmoe_ep_peer_connect", "fmoe_ep_peer_destroy", "fmoe_ep_peer_slab_bytes",
     "fmoe_ep_peer_dispatch", "fmoe_ep_peer_experts", "fmoe_ep_peer_combine", "fmoe_ep_peer_read_status",
@@ -181,6 +182,9 @@ def _open(path: str) -> ctypes.CDLL:
     lib.fmoe_route_build_noalloc.argtypes = [p, i64, i32, i32, p, p, p, p, p, p]
     lib.fmoe_i8gemm_dynamic_scaled_mm.argtypes = [p, i32, i64, i32, p, p, p, i32, p, i32, p, ctypes.c_size_t, p]
     lib.fmoe_i8gemm_dynamic_scaled_mm_pair.argtypes = [p, i64, i32, p, p, i32, p, p, p, i32, p, p, ctypes.c_size_t, p]
+    lib.fmoe_gated_mlp_forward.argtypes = [p, i64, p, p, i64, i32, i32, i32, ctypes.c_float, p, p, p, p]
+    lib.fmoe_gated_mlp_backward.argtypes = [p, i64, p, i64, p, p, p, p, i64, i32, i32, p, p, p, p, p]
+    lib.fmoe_dense_status.argtypes = [p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]
     lib.fmoe_append_shared_route.argtypes = [p, p, i64, i32, i64, ctypes.c_float, p, p, p]
     lib.fmoe_router_topk.argtypes = [p, p, i64, i32, i32, i32, i32, ctypes.c_float, p, p, p]
     lib.fmoe_ep_peer_create.argtypes = [i32, i32, i64, i32, i32, i32, i32, i32, i32, ctypes.POINTER(ctypes.c_void_p)]
@@ -343,6 +347,22 @@ def _require_cuda(name: str, tensor: torch.Tensor, dtype: torch.dtype) -> torch.
     if tensor.dtype is not dtype:
         raise TypeError(f"{name} must have dtype {dtype}, got {tensor.dtype}")
     return tensor if tensor.is_contiguous() else tensor.contiguous()
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device_of(tensor: torch.Tensor):
+    """Context in which the device of `tensor` is the current one, whose current stream `_stream` then gives."""
+    return _NO_GUARD if tensor.device.index == torch.cuda.current_device() else torch.cuda.device(tensor.device)
+
+
+def dense_status() -> tuple[int, int]:
+    """(error, site) of the first bounded wait that gave up in a call without a workspace (the gated block) on the current device
+    since the last time this was asked; (0, 0) in a sound run.  Synchronises."""
+    error, detail = ctypes.c_int32(0), ctypes.c_int32(0)
+    check(load().fmoe_dense_status(_stream(), ctypes.byref(error), ctypes.byref(detail)))
+    return error.value, detail.value
 
 
 def moe_forward(x, w13, w2, topk_weights, topk_ids, *, s13=None, s2=None, numerics: int = NUMERICS_TORCHREF,

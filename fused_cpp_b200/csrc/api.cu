@@ -975,6 +975,123 @@ int fmoe_i8gemm_dynamic_scaled_mm_pair(const void* x_bf16, int64_t rows, int32_t
   return error == cudaSuccess ? FMOE_OK : cuda_fail(error, "i8gemm pair GEMM");
 }
 
+namespace {
+int check_gated_shape(const char* what, int64_t rows, int hidden, int inter) {
+  const int status = check_device();
+  if (status != FMOE_OK) return status;
+  if (rows < 0 || rows > (1ll << 31) - 512) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: rows must lie in [0, 2^31 - 512]", what);
+  if (hidden <= 0 || inter <= 0 || hidden % 8 != 0 || inter % 8 != 0 || inter > (1 << 29)) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: H and F must be positive multiples of 8 (H=%d, F=%d)", what, hidden, inter);
+  }
+  return FMOE_OK;
+}
+bool vector_aligned(const void* pointer) { return reinterpret_cast<uintptr_t>(pointer) % 16 == 0; }
+int check_rows(const char* what, const char* name, const void* data, int64_t stride, int columns) {
+  if (data == nullptr || !vector_aligned(data) || stride % 8 != 0 || stride < columns) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: %s must be 16-byte aligned rows, their stride a multiple of 8 elements and at least a row", what, name);
+  }
+  return FMOE_OK;
+}
+}  // namespace
+
+int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, const void* w2, int64_t rows, int32_t hidden, int32_t inter,
+                           int32_t activation, float swiglu_limit, void* h, void* by_gate_up, void* y, void* stream_ptr) {
+  static const char* const what = "gated_mlp_forward";
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  int status = check_gated_shape(what, rows, hidden, inter);
+  if (status != FMOE_OK) return status;
+  if (activation != FMOE_ACTIVATION_SILU && activation != FMOE_ACTIVATION_GELU && activation != FMOE_ACTIVATION_SWIGLUOAI) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, activation);
+  }
+  if (!(swiglu_limit >= 0.0f) || (swiglu_limit > 0.0f && activation != FMOE_ACTIVATION_SILU)) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: swiglu_limit must be 0 (none) or positive, and belongs to SILU", what);
+  }
+  if (rows == 0) return FMOE_OK;
+  if ((status = check_rows(what, "x", x, x_stride, hidden)) != FMOE_OK || (status = check_rows(what, "w13", w13, hidden, hidden)) != FMOE_OK ||
+      (status = check_rows(what, "w2", w2, inter, inter)) != FMOE_OK || (status = check_rows(what, "h", h, inter, inter)) != FMOE_OK ||
+      (status = check_rows(what, "y", y, hidden, hidden)) != FMOE_OK) {
+    return status;
+  }
+  if (!vector_aligned(by_gate_up)) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: by_gate_up must be 16-byte aligned", what);
+  int* words = nullptr;
+  cudaError_t error = fmoe::dense_status_words(&words);
+  if (error == cudaSuccess) {
+    error = fmoe::launch_gated_projection(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
+                                          swiglu_limit, static_cast<uint16_t*>(h), static_cast<uint16_t*>(by_gate_up), words, stream, false);
+  }
+  if (error == cudaSuccess) {
+    const fmoe::DenseProductArgs down = {{static_cast<const uint16_t*>(h), inter}, {static_cast<const uint16_t*>(w2), inter}, static_cast<uint16_t*>(y), rows, hidden, inter};
+    error = fmoe::launch_dense_products(fmoe::DenseForm::kRowsRows, &down, 1, words, stream, true);
+  }
+  return error == cudaSuccess ? FMOE_OK : cuda_fail(error, what);
+}
+
+int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w13, const void* w2, const void* h,
+                            const void* by_gate_up, int64_t rows, int32_t hidden, int32_t inter, void* d_gate_up, void* dx, void* dw13, void* dw2,
+                            void* stream_ptr) {
+  static const char* const what = "gated_mlp_backward";
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  int status = check_gated_shape(what, rows, hidden, inter);
+  if (status != FMOE_OK) return status;
+  if (rows == 0) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: no rows, no gradients to compute", what);
+  const bool needs_gate_up = dx != nullptr || dw13 != nullptr;
+  if ((status = check_rows(what, "dy", dy, dy_stride, hidden)) != FMOE_OK) return status;
+  if (dw13 != nullptr && (status = check_rows(what, "x", x, x_stride, hidden)) != FMOE_OK) return status;
+  if (dx != nullptr && (status = check_rows(what, "w13", w13, hidden, hidden)) != FMOE_OK) return status;
+  if (dw2 != nullptr && (status = check_rows(what, "h", h, inter, inter)) != FMOE_OK) return status;
+  if (needs_gate_up && ((status = check_rows(what, "w2", w2, inter, inter)) != FMOE_OK ||
+                        (status = check_rows(what, "by_gate_up", by_gate_up, 2 * static_cast<int64_t>(inter), 2 * inter)) != FMOE_OK ||
+                        (status = check_rows(what, "d_gate_up", d_gate_up, 2 * static_cast<int64_t>(inter), 2 * inter)) != FMOE_OK)) {
+    return status;
+  }
+  if (!vector_aligned(dx) || !vector_aligned(dw13) || !vector_aligned(dw2)) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: gradients must be 16-byte aligned", what);
+  }
+  int* words = nullptr;
+  cudaError_t error = fmoe::dense_status_words(&words);
+  bool chained = false;
+  if (error == cudaSuccess && needs_gate_up) {
+    error = fmoe::launch_gated_backward(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const uint16_t*>(by_gate_up),
+                                        rows, hidden, inter, static_cast<uint16_t*>(d_gate_up), words, stream, chained);
+    chained = true;
+  }
+  if (error == cudaSuccess && dx != nullptr) {
+    const fmoe::DenseProductArgs product = {{static_cast<const uint16_t*>(d_gate_up), 2 * static_cast<int64_t>(inter)},
+                                            {static_cast<const uint16_t*>(w13), hidden}, static_cast<uint16_t*>(dx), rows, hidden, 2 * static_cast<int64_t>(inter)};
+    error = fmoe::launch_dense_products(fmoe::DenseForm::kRowsByK, &product, 1, words, stream, chained);
+    chained = true;
+  }
+  // Both weight gradients in one launch: apart, each ends with a wave of tiles that does not fill the chip.
+  fmoe::DenseProductArgs products[2];
+  int count = 0;
+  if (dw13 != nullptr) {
+    products[count++] = {{static_cast<const uint16_t*>(d_gate_up), 2 * static_cast<int64_t>(inter)}, {static_cast<const uint16_t*>(x), x_stride},
+                         static_cast<uint16_t*>(dw13), 2 * static_cast<int64_t>(inter), hidden, rows};
+  }
+  if (dw2 != nullptr) {
+    products[count++] = {{static_cast<const uint16_t*>(dy), dy_stride}, {static_cast<const uint16_t*>(h), inter}, static_cast<uint16_t*>(dw2), hidden, inter, rows};
+  }
+  if (error == cudaSuccess && count > 0) error = fmoe::launch_dense_products(fmoe::DenseForm::kByKByK, products, count, words, stream, chained);
+  return error == cudaSuccess ? FMOE_OK : cuda_fail(error, what);
+}
+
+int fmoe_dense_status(void* stream_ptr, int32_t* error_out, int32_t* detail) {
+  if (error_out == nullptr || detail == nullptr) return fail(FMOE_ERR_INVALID_ARGUMENT, "dense_status: null pointer");
+  const int status = check_device();
+  if (status != FMOE_OK) return status;
+  int* words = nullptr;
+  int host[fmoe::kStatusWords];
+  cudaError_t error = fmoe::dense_status_words(&words);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (error == cudaSuccess) error = cudaMemcpyAsync(host, words, sizeof(host), cudaMemcpyDeviceToHost, stream);
+  if (error == cudaSuccess) error = cudaMemsetAsync(words, 0, sizeof(host), stream);
+  if (error == cudaSuccess) error = cudaStreamSynchronize(stream);
+  if (error != cudaSuccess) return cuda_fail(error, "dense_status");
+  *error_out = host[fmoe::kStatusError];
+  *detail = host[fmoe::kStatusWaitSite];
+  return FMOE_OK;
+}
+
 #ifdef FMOE_DIAG
 int fmoe_diag_quotient_check(uint32_t seed, int32_t numerators, void* mismatches, void* stream) {
   const int status = check_device();

@@ -1,0 +1,514 @@
+// Dense bf16 products of the gated feed-forward block over many rows (fused_cpp_b200.moe.gated_mlp), forward and backward:
+//   h = act(x Wg^T, x Wu^T)      both projections, the activation and their product in one kernel
+//   y = h W2^T
+//   dh = dy W2, times the partial derivatives of h: d_gate_up
+//   dx = d_gate_up W13,  dW13 = d_gate_up^T x,  dW2 = dy^T h
+// All are out[m, n] = sum over k of A[m, k] B[n, k] on tcgen05.mma (bf16 products, fp32 sums) with another layout of the operands in
+// memory each, and none of the operands is transposed on the way: an operand whose rows run along k ("by k": [k, m]) is staged as
+// 64 x 64 blocks that the tensor core reads as M/N-major tiles.
+//
+// Two CTAs of a cluster drive one 256 x 256 tile (cta_group::2): each stages its 128 A rows and its half of the B rows (64 KB a K block of
+// 64 for the pair), which is what an SM can take from L2 while the tensor pipe works (umma2_gemm.cu has the figures).  D rows are token or weight rows and lie in
+// the lanes of tensor memory; its columns are output channels, so that a lane holds 32 neighbouring channels of one row and stores them as
+// four 16-byte vectors.  For the gated projection CTA 0 stages 128 gate rows and CTA 1 the 128 up rows of the same channels: gate and up of
+// a channel are columns c and 128 + c of the same lane.  Two accumulators of 256 columns take turns: the epilogue of a tile runs under the products of the
+// next.
+//
+// The forward pass keeps dh/dgate and dh/dup in bf16 instead of gate and up: the backward epilogue is one product per value, its error one rounding, and
+// a value next to an activation's limit cannot be rounded across it.
+#include <cuda.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "pair_ptx.cuh"
+#include "ptx.cuh"
+
+namespace fmoe {
+
+namespace {
+
+constexpr int kRowsPerCta = 128;                  // A rows staged by one CTA
+constexpr int kBlockK = 64;                       // K elements of a pipeline stage: 128 bytes
+constexpr int kChunkBytes = 64 * kBlockK * 2;     // a 64 x 64 block
+constexpr int kUmmaK = 16;
+constexpr int kEpilogueWarps = 8;
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kTmemColumns = 512;
+constexpr int kMaxStages = 8;
+constexpr int kTileGroup = 8;  // row tiles that are walked together (see tile_at)
+
+enum class Epilogue { kPlain, kGated, kGatedBack };
+
+template <int kTileN>
+struct TileConfig {
+  static constexpr int kABytes = kRowsPerCta * kBlockK * 2;
+  static constexpr int kBRows = kTileN / 2;  // of one CTA
+  static constexpr int kBBytes = kBRows * kBlockK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 192 * 1024 / kStageBytes;
+  static_assert(kStages <= kMaxStages, "the barriers of all stages");
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + 1024;
+};
+
+struct Control {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+static_assert(sizeof(Control) <= 1024, "control block exceeds its shared-memory reservation");
+
+struct Problem {
+  uint16_t* out;
+  int64_t m;
+  int n;         // output channels
+  int k_blocks;
+  int m_tiles, n_tiles;
+};
+
+struct Args {
+  Problem problem[2];
+  int64_t tiles[2];  // tiles of the first problem, and of both
+  uint16_t* by_gate_up_out;
+  const uint16_t* by_gate_up;
+  int activation;
+  float limit;
+  int* status;
+};
+
+struct Tile {
+  int problem, m, n;
+};
+
+// Tiles in the order of their numbers: groups of kTileGroup row tiles, inside a group all row tiles of a column tile before the next one, so that the
+// tiles in flight (74 pairs) share both their A rows and their B rows in L2.
+__device__ __forceinline__ Tile tile_at(const Args& args, int64_t index) {
+  Tile t;
+  t.problem = index >= args.tiles[0] ? 1 : 0;
+  const Problem& p = args.problem[t.problem];
+  const int local = static_cast<int>(index - (t.problem ? args.tiles[0] : 0));
+  const int per_group = kTileGroup * p.n_tiles;
+  const int group = local / per_group;
+  const int rest = local - group * per_group;
+  const int group_m = min(kTileGroup, p.m_tiles - group * kTileGroup);
+  t.n = rest / group_m;
+  t.m = group * kTileGroup + rest - t.n * group_m;
+  return t;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
+  const __nv_bfloat162 pair = __floats2bfloat162_rn(low, high);
+  return *reinterpret_cast<const uint32_t*>(&pair);
+}
+
+// Up to 32 neighbouring channels of a row as bf16: `columns` of them exist, a multiple of 8.
+__device__ __forceinline__ void store_channels(uint16_t* to, const float (&v)[32], int columns) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (8 * q >= columns) break;
+    *reinterpret_cast<uint4*>(to + 8 * q) = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
+                                                       pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
+  }
+}
+
+// h and its partial derivatives (common: gate * act'(gate) forms; NaN stays NaN through the limits).
+template <typename Tag>
+__device__ __forceinline__ void gated_with_derivatives(Tag, float gate, float up, float limit, float* h, float* by_gate, float* by_up) {
+  if constexpr (Tag::value == FMOE_ACT_GELU) {
+    const float cdf = normcdff(gate);  // 0.5 (1 + erf) would lose the values of the left tail
+    const float density = 0.39894228040143267794f * __expf(-0.5f * gate * gate);
+    *h = gate * cdf * up;
+    *by_gate = up * (cdf + gate * density);
+    *by_up = gate * cdf;
+  } else {
+    constexpr bool kOai = Tag::value == FMOE_ACT_SWIGLUOAI;
+    const float bound = kOai ? 7.0f : (limit > 0.0f ? limit : __int_as_float(0x7f800000));
+    constexpr float kAlpha = kOai ? 1.702f : 1.0f;
+    const bool gate_cut = gate > bound;
+    const bool up_cut = fabsf(up) > bound;
+    const float g = gate_cut ? bound : gate;
+    const float u = (up_cut ? copysignf(bound, up) : up) + (kOai ? 1.0f : 0.0f);
+    const float s = __fdividef(1.0f, 1.0f + __expf(-kAlpha * g));  // e^-g = inf divides to 0
+    const float gs = g * s;
+    *h = gs * u;
+    *by_gate = gate_cut ? 0.0f : u * s * (1.0f + kAlpha * g * (1.0f - s));
+    *by_up = up_cut ? 0.0f : gs;
+  }
+}
+
+template <Epilogue kEpilogue, bool kAByK, bool kBByK, int kTileN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_constant__ CUtensorMap b_map0,
+                       const __grid_constant__ CUtensorMap a_map1, const __grid_constant__ CUtensorMap b_map1,
+                       const __grid_constant__ Args args) {
+  using Cfg = TileConfig<kTileN>;
+  constexpr int kStages = Cfg::kStages;
+  constexpr int kColumns = kEpilogue == Epilogue::kGated ? kTileN / 2 : kTileN;  // output channels of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Control* ctl = reinterpret_cast<Control*>(smem + static_cast<size_t>(kStages) * Cfg::kStageBytes);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_cta_rank();
+  const bool leader = cta == 0;
+  int* status = args.status;
+  const int64_t tiles = args.tiles[1];
+  const int64_t first_tile = blockIdx.x >> 1;
+  const int64_t tile_stride = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&ctl->full[s], 1);
+      ptx::mbar_init(&ctl->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(&ctl->acc_full[b], 1);
+      ptx::mbar_init(&ctl->acc_empty[b], 2 * kEpilogueWarps);  // the epilogue warps of both CTAs
+    }
+    ctl->abort_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&ctl->tmem_base, kTmemColumns);
+    tmem_relinquish_pair();
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers are initialised before anything signals them
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  volatile int* abort_flag = &ctl->abort_flag;
+  const uint32_t smem_base = ptx::smem_u32(smem);
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs; the whole warp walks the loop, one elected lane issues) ----------------
+    const bool issuer = ptx::elect_one();
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    const uint32_t full_leader0 = map_to_cta(ptx::smem_u32(&ctl->full[0]), 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    for (int64_t index = first_tile; index < tiles; index += tile_stride) {
+      const Tile tile = tile_at(args, index);
+      const CUtensorMap* const a_map = tile.problem ? &a_map1 : &a_map0;
+      const CUtensorMap* const b_map = tile.problem ? &b_map1 : &b_map0;
+      const int k_blocks = args.problem[tile.problem].k_blocks;
+      const int a_row = tile.m * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta);
+      const int b_row = kEpilogue == Epilogue::kGated ? tile.n * kColumns + static_cast<int>(cta) * args.problem[0].n
+                                                      : tile.n * kTileN + Cfg::kBRows * static_cast<int>(cta);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        ptx::mbar_wait(&ctl->empty[stage], phase ^ 1u, abort_flag, status, 41);
+        if (issuer) {
+          const uint32_t dst = smem_base + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+          const uint32_t bar = full_leader0 + 8u * static_cast<uint32_t>(stage);
+          if (leader) ptx::mbar_arrive_expect_tx(&ctl->full[stage], 2 * Cfg::kStageBytes);
+          const int k0 = kb * kBlockK;
+          if constexpr (kAByK) {
+            tma_load_2d_pair(dst, a_map, bar, a_row, k0);
+            tma_load_2d_pair(dst + kChunkBytes, a_map, bar, a_row + 64, k0);
+          } else {
+            tma_load_2d_pair(dst, a_map, bar, k0, a_row);
+          }
+          if constexpr (kBByK) {
+#pragma unroll
+            for (int i = 0; i < Cfg::kBRows / 64; ++i) tma_load_2d_pair(dst + Cfg::kABytes + i * kChunkBytes, b_map, bar, b_row + 64 * i, k0);
+          } else {
+            tma_load_2d_pair(dst + Cfg::kABytes, b_map, bar, k0, b_row);
+          }
+        }
+        ++issued;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (leader) {
+      // Drain: the leader's full barriers count both CTAs' bytes, so this also covers the follower's loads.
+      const int pending = issued < kStages ? issued : kStages;
+      for (int back = 0; back < pending; ++back) {
+        int s = stage - 1 - back;
+        uint32_t p = phase;
+        if (s < 0) {
+          s += kStages;
+          p ^= 1u;
+        }
+        const unsigned long long start = ptx::global_timer_ns();
+        while (!ptx::mbar_try_wait(&ctl->full[s], p)) {
+          if (ptx::global_timer_ns() - start > ptx::kWaitLimitNs) break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader CTA only) ----------------
+    if (leader) {
+      const bool issuer = ptx::elect_one();
+      // Descriptor words: see ptx::make_smem_desc_sw128.  K-major: the next 16 K elements are 32 bytes on.  M/N-major: blocks of 64 rows of the
+      // operand lie kChunkBytes apart (leading offset), groups of eight K rows 1024 bytes (stride offset), and the next 16
+      // K elements are two such groups on.
+      constexpr uint32_t kByKLead = static_cast<uint32_t>(kChunkBytes >> 4) << 16;
+      constexpr uint32_t kALead = kAByK ? kByKLead : (1u << 16);
+      constexpr uint32_t kBLead = kBByK ? kByKLead : (1u << 16);
+      constexpr uint32_t kAStep = kAByK ? 2048 >> 4 : 32 >> 4;
+      constexpr uint32_t kBStep = kBByK ? 2048 >> 4 : 32 >> 4;
+      constexpr uint32_t kIdesc = ptx::make_instr_desc(false, 2 * kRowsPerCta, kTileN) | (kAByK ? 1u << 15 : 0u) | (kBByK ? 1u << 16 : 0u);
+      const uint32_t desc_hi = static_cast<uint32_t>(1024 >> 4) | (1u << 14) | (2u << 29);
+      const uint32_t stage0 = (smem_base & 0x3ffffu) >> 4;
+      const uint32_t empty_c0 = map_to_cta(ptx::smem_u32(&ctl->empty[0]), 0);
+      const uint32_t empty_c1 = map_to_cta(ptx::smem_u32(&ctl->empty[0]), 1);
+      const uint32_t accfull_c0 = map_to_cta(ptx::smem_u32(&ctl->acc_full[0]), 0);
+      const uint32_t accfull_c1 = map_to_cta(ptx::smem_u32(&ctl->acc_full[0]), 1);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t stage_lo = stage0;
+      int local = 0;
+      for (int64_t index = first_tile; index < tiles; index += tile_stride, ++local) {
+        const int k_blocks = args.problem[index >= args.tiles[0] ? 1 : 0].k_blocks;
+        const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
+        const uint32_t use = static_cast<uint32_t>(local) >> 1;
+        const uint32_t acc = tmem_base + kTileN * buffer;
+        ptx::mbar_wait(&ctl->acc_empty[buffer], (use & 1u) ^ 1u, abort_flag, status, 42);
+        ptx::tcgen05_fence_after();
+        uint32_t accumulate = 0;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 43);
+          ptx::tcgen05_fence_after();
+          if (issuer) {
+            const uint32_t a_lo = stage_lo | kALead;
+            const uint32_t b_lo = (stage_lo + (Cfg::kABytes >> 4)) | kBLead;
+#pragma unroll
+            for (uint32_t ks = 0; ks < kBlockK / kUmmaK; ++ks) {
+              umma_pair<false>(acc, a_lo + kAStep * ks, b_lo + kBStep * ks, desc_hi, kIdesc, ks == 0 ? accumulate : 1u);
+            }
+            tcgen05_commit_pair(empty_c0 + 8u * static_cast<uint32_t>(stage));
+            tcgen05_commit_pair(empty_c1 + 8u * static_cast<uint32_t>(stage));
+          }
+          accumulate = 1;
+          stage_lo += Cfg::kStageBytes >> 4;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+            stage_lo = stage0;
+          }
+        }
+        if (issuer) {
+          tcgen05_commit_pair(accfull_c0 + 8u * buffer);
+          tcgen05_commit_pair(accfull_c1 + 8u * buffer);
+        }
+      }
+    }
+  } else {
+    // ---------------- epilogue (warps 2.. of both CTAs) ----------------
+    ptx::grid_dependency_wait();
+    const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id % 4
+    const int chunk_first = (warp - 2) >> 2;
+    constexpr int kChunkStep = kEpilogueWarps / 4;
+    constexpr int kChunks = kColumns / 32;
+    const uint32_t acc_lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t acc_empty_leader = map_to_cta(ptx::smem_u32(&ctl->acc_empty[0]), 0);
+    int local = 0;
+    for (int64_t index = first_tile; index < tiles; index += tile_stride, ++local) {
+      const Tile tile = tile_at(args, index);
+      const Problem& p = args.problem[tile.problem];
+      const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
+      const uint32_t use = static_cast<uint32_t>(local) >> 1;
+      const int64_t row = static_cast<int64_t>(tile.m) * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + quarter * 32 + lane;
+      const bool row_ok = row < p.m;
+      const int n0 = tile.n * kColumns;
+      const uint32_t acc = acc_lane_base + kTileN * buffer;
+      ptx::mbar_wait(&ctl->acc_full[buffer], use & 1u, abort_flag, status, 44);
+      ptx::tcgen05_fence_after();
+      for (int chunk = chunk_first; chunk < kChunks; chunk += kChunkStep) {
+        const int col = n0 + 32 * chunk;
+        const int columns = row_ok ? p.n - col : 0;  // of this lane's chunk that exist, if below 32
+        uint32_t bits[32];
+        tmem_ld_x32(acc + 32u * static_cast<uint32_t>(chunk), bits);
+        if constexpr (kEpilogue == Epilogue::kGated) {
+          uint32_t up_bits[32];
+          tmem_ld_x32(acc + static_cast<uint32_t>(kTileN / 2) + 32u * static_cast<uint32_t>(chunk), up_bits);
+          ptx::tmem_ld_wait();
+          float h[32], by_gate[32], by_up[32];
+          with_activation<false>(args.activation, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              gated_with_derivatives(act, __uint_as_float(bits[j]), __uint_as_float(up_bits[j]), args.limit, &h[j], &by_gate[j], &by_up[j]);
+            }
+          });
+          store_channels(p.out + row * p.n + col, h, columns);
+          if (args.by_gate_up_out != nullptr) {
+            uint16_t* const by = args.by_gate_up_out + row * 2 * p.n + col;
+            store_channels(by, by_gate, columns);
+            store_channels(by + p.n, by_up, columns);
+          }
+        } else if constexpr (kEpilogue == Epilogue::kGatedBack) {
+          uint4 by_gate[4], by_up[4];
+          const uint16_t* const by = args.by_gate_up + row * 2 * p.n + col;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            by_gate[q] = by_up[q] = make_uint4(0, 0, 0, 0);
+            if (8 * q < columns) {
+              by_gate[q] = *reinterpret_cast<const uint4*>(by + 8 * q);
+              by_up[q] = *reinterpret_cast<const uint4*>(by + p.n + 8 * q);
+            }
+          }
+          ptx::tmem_ld_wait();
+          uint16_t* const to = p.out + row * 2 * p.n + col;
+          float v[32];
+          const uint32_t* const gate_words = reinterpret_cast<const uint32_t*>(by_gate);
+          const uint32_t* const up_words = reinterpret_cast<const uint32_t*>(by_up);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            v[j] = __uint_as_float(bits[j]) * __uint_as_float((j & 1) ? gate_words[j >> 1] & 0xffff0000u : gate_words[j >> 1] << 16);
+          }
+          store_channels(to, v, columns);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            v[j] = __uint_as_float(bits[j]) * __uint_as_float((j & 1) ? up_words[j >> 1] & 0xffff0000u : up_words[j >> 1] << 16);
+          }
+          store_channels(to + p.n, v, columns);
+        } else {
+          ptx::tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(bits[j]);
+          store_channels(p.out + row * p.n + col, v, columns);
+        }
+        __syncwarp();  // the next tensor-memory load wants the whole warp
+      }
+      ptx::tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * buffer);
+    }
+  }
+
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while its peer may still signal its barriers or read its operands
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tcgen05_fence_after();
+    tmem_dealloc_pair(tmem_base, kTmemColumns);
+  }
+}
+
+struct Operands {
+  DenseOperand a, b;
+  int64_t b_rows;  // rows of B along its n axis in memory (2 * inter for the gated projection)
+};
+
+template <Epilogue kEpilogue, bool kAByK, bool kBByK, int kTileN>
+cudaError_t launch_tiles(Args args, const Operands* operands, int count, const int64_t* depth, cudaStream_t stream, bool chained) {
+  using Cfg = TileConfig<kTileN>;
+  auto kernel = gated_pair_gemm_kernel<kEpilogue, kAByK, kBByK, kTileN>;
+  static PerDeviceOnce configured;
+  const int device = current_device_ordinal();
+  if (configured.needed(device)) {
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kSmemBytes));
+    if (error != cudaSuccess) return error;
+    configured.mark(device);
+  }
+  constexpr int kColumns = kEpilogue == Epilogue::kGated ? kTileN / 2 : kTileN;
+  CUtensorMap maps[4];
+  int64_t total = 0;
+  for (int i = 0; i < 2; ++i) {
+    const int from = i < count ? i : 0;
+    Problem& p = args.problem[i];
+    if (i >= count) p = args.problem[0];
+    const Operands& o = operands[from];
+    const uint64_t m = static_cast<uint64_t>(p.m), n = static_cast<uint64_t>(o.b_rows), k = static_cast<uint64_t>(depth[from]);
+    const bool ok = make_sw128_map(&maps[2 * i], o.a.data, false, kAByK ? k : m, kAByK ? m : k, kAByK ? kBlockK : kRowsPerCta, o.a.stride) &&
+                    make_sw128_map(&maps[2 * i + 1], o.b.data, false, kBByK ? k : n, kBByK ? n : k, kBByK ? kBlockK : Cfg::kBRows, o.b.stride);
+    if (!ok) return cudaErrorInvalidValue;
+    p.k_blocks = static_cast<int>((k + kBlockK - 1) / kBlockK);
+    p.m_tiles = static_cast<int>((p.m + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta));
+    p.n_tiles = (p.n + kColumns - 1) / kColumns;
+    if (i < count) total += static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+    if (i == 0) args.tiles[0] = total;
+  }
+  args.tiles[1] = total;
+  if (total > (1ll << 30)) return cudaErrorInvalidValue;
+  int64_t pairs = sm_count_of_current_device() / 2;
+  if (pairs > total) pairs = total;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(2 * pairs)), kThreads, Cfg::kSmemBytes, stream, chained, maps[0], maps[1], maps[2], maps[3], args);
+}
+
+template <Epilogue kEpilogue, bool kAByK, bool kBByK>
+cudaError_t launch_form(const Args& args, const Operands* operands, int count, const int64_t* depth, cudaStream_t stream, bool chained) {
+  return launch_tiles<kEpilogue, kAByK, kBByK, 256>(args, operands, count, depth, stream, chained);
+}
+
+// Where the kernels of the operators without a workspace of their own report a wait that gave up.
+__device__ int status_words[kStatusWords];
+
+}  // namespace
+
+cudaError_t dense_status_words(int** words) {
+  static int* known[kMaxDevices] = {};
+  const int device = current_device_ordinal();
+  if (device >= 0 && device < kMaxDevices && known[device] != nullptr) {
+    *words = known[device];
+    return cudaSuccess;
+  }
+  void* address = nullptr;
+  const cudaError_t error = cudaGetSymbolAddress(&address, status_words);
+  if (error != cudaSuccess) return error;
+  *words = static_cast<int*>(address);
+  if (device >= 0 && device < kMaxDevices) known[device] = *words;
+  return cudaSuccess;
+}
+
+cudaError_t launch_gated_projection(const uint16_t* x, int64_t x_stride, const uint16_t* w13, int64_t rows, int hidden, int inter, int activation,
+                                    float limit, uint16_t* h, uint16_t* by_gate_up, int* status, cudaStream_t stream, bool chained) {
+  Args args = {};
+  args.problem[0].out = h;
+  args.problem[0].m = rows;
+  args.problem[0].n = inter;
+  args.by_gate_up_out = by_gate_up;
+  args.activation = activation;
+  args.limit = limit;
+  args.status = status;
+  const Operands operands = {{x, x_stride}, {w13, hidden}, 2 * static_cast<int64_t>(inter)};
+  const int64_t depth = hidden;
+  return launch_form<Epilogue::kGated, false, false>(args, &operands, 1, &depth, stream, chained);
+}
+
+cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const uint16_t* by_gate_up, int64_t rows, int hidden,
+                                  int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained) {
+  Args args = {};
+  args.problem[0].out = d_gate_up;
+  args.problem[0].m = rows;
+  args.problem[0].n = inter;
+  args.by_gate_up = by_gate_up;
+  args.status = status;
+  const Operands operands = {{dy, dy_stride}, {w2, inter}, inter};
+  const int64_t depth = hidden;
+  return launch_form<Epilogue::kGatedBack, false, true>(args, &operands, 1, &depth, stream, chained);
+}
+
+cudaError_t launch_dense_products(DenseForm form, const DenseProductArgs* products, int count, int* status, cudaStream_t stream, bool chained) {
+  if (count < 1 || count > 2) return cudaErrorInvalidValue;
+  Args args = {};
+  Operands operands[2];
+  int64_t depth[2];
+  for (int i = 0; i < count; ++i) {
+    const DenseProductArgs& p = products[i];
+    args.problem[i].out = p.out;
+    args.problem[i].m = p.m;
+    args.problem[i].n = p.n;
+    operands[i] = {p.a, p.b, p.n};
+    depth[i] = p.k;
+  }
+  args.status = status;
+  switch (form) {
+    case DenseForm::kRowsRows: return launch_form<Epilogue::kPlain, false, false>(args, operands, count, depth, stream, chained);
+    case DenseForm::kRowsByK: return launch_form<Epilogue::kPlain, false, true>(args, operands, count, depth, stream, chained);
+    case DenseForm::kByKByK: return launch_form<Epilogue::kPlain, true, true>(args, operands, count, depth, stream, chained);
+  }
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace fmoe

@@ -738,12 +738,12 @@ EncodeTiledFn encode_tiled_fn() {
 
 }  // namespace
 
-bool make_sw128_map(CUtensorMap* map, const void* base, bool int8, uint64_t rows, uint64_t k, uint32_t box_rows) {
+bool make_sw128_map(CUtensorMap* map, const void* base, bool int8, uint64_t rows, uint64_t k, uint32_t box_rows, uint64_t row_stride) {
   EncodeTiledFn encode = encode_tiled_fn();
   if (encode == nullptr) return false;
   const uint32_t elem_bytes = int8 ? 1 : 2;
   const cuuint64_t dims[2] = {k, rows};
-  const cuuint64_t strides[1] = {k * elem_bytes};
+  const cuuint64_t strides[1] = {(row_stride > 0 ? row_stride : k) * elem_bytes};
   const cuuint32_t box[2] = {kBlockKBytes / elem_bytes, box_rows};
   const cuuint32_t elem_strides[2] = {1, 1};
   const CUresult result = encode(map, int8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,

@@ -322,6 +322,24 @@ FMOE_API int fmoe_i8gemm_dynamic_scaled_mm_pair(const void* x_bf16, int64_t rows
                                                 const int8_t* second_w, const float* second_scale, int32_t second_n,
                                                 void* second_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- gated feed-forward block, forward and backward (bf16, row-major) -------------------------
+ * x [rows, H] with x_stride elements from a row to the next, w13 [2F, H] (gate rows, then up rows), w2 [H, F]:
+ *   h = act(x Wg^T, x Wu^T) (bf16),  y = h W2^T.
+ * activation: FMOE_ACTIVATION_SILU (swiglu_limit > 0: gate clamped from above and up to +-limit first), _GELU, _SWIGLUOAI.
+ * h [rows, F] and y [rows, H] are written; by_gate_up [rows, 2F] (nullable) takes the partial derivatives of h by gate and by up for a
+ * backward pass.  H and F are multiples of 8, every row starts on a 16-byte boundary.  Enqueues two launches. */
+FMOE_API int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, const void* w2, int64_t rows, int32_t hidden,
+                                    int32_t inter, int32_t activation, float swiglu_limit, void* h, void* by_gate_up, void* y,
+                                    void* stream);
+/* Gradients from dy [rows, H] and what the forward call kept: dx [rows, H], dw13 [2F, H], dw2 [H, F], each left out where null.
+ * d_gate_up [rows, 2F] is scratch (needed for dx and dw13).  rows >= 1.  Enqueues up to three launches. */
+FMOE_API int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w13,
+                                     const void* w2, const void* h, const void* by_gate_up, int64_t rows, int32_t hidden,
+                                     int32_t inter, void* d_gate_up, void* dx, void* dw13, void* dw2, void* stream);
+/* First device-side error (FMOE_ERR_DEVICE_WAIT: a bounded wait gave up, detail = its site) of the calls on the current device that
+ * have no workspace of their own, since the last time it was asked.  Synchronises the stream and clears the record. */
+FMOE_API int fmoe_dense_status(void* stream, int32_t* error, int32_t* detail);
+
 /* ---- router front-end ------------------------------------------------------------------------- */
 
 #define FMOE_SCORING_SOFTMAX 0

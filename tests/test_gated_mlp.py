@@ -1,0 +1,47 @@
+"""Arguments of the gated feed-forward block that are refused before anything reaches the GPU."""
+import pytest
+import torch
+
+from fused_cpp_b200 import moe
+
+
+def _call(**changes):
+    arguments = {"input": torch.zeros(3, 16, dtype=torch.bfloat16), "w13": torch.zeros(48, 16, dtype=torch.bfloat16),
+                 "w2": torch.zeros(16, 24, dtype=torch.bfloat16)}
+    options = {name: changes.pop(name) for name in list(changes) if name not in arguments}
+    arguments.update(changes)
+    return moe.gated_mlp(arguments["input"], arguments["w13"], arguments["w2"], **options)
+
+
+@pytest.mark.parametrize("changes, error, text", [
+    ({"input": torch.zeros(3, 16)}, TypeError, "input must be torch.bfloat16"),
+    ({"w13": torch.zeros(48, 16)}, TypeError, "w13 must be torch.bfloat16"),
+    ({"w2": torch.zeros(16, 24)}, TypeError, "w2 must be torch.bfloat16"),
+    ({"input": [1.0]}, TypeError, "must be a torch.Tensor"),
+    ({"input": torch.zeros(3, 24, dtype=torch.bfloat16)}, ValueError, "H=16"),
+    ({"w13": torch.zeros(40, 16, dtype=torch.bfloat16)}, ValueError, "w13 must be"),
+    ({"w2": torch.zeros(1, 16, 24, dtype=torch.bfloat16)}, ValueError, "weights must be"),
+    ({"w13": torch.zeros(24, 16, dtype=torch.bfloat16), "w2": torch.zeros(16, 12, dtype=torch.bfloat16)}, ValueError, "multiples of 8"),
+    ({"activation": "relu"}, ValueError, "activation must be"),
+    ({"swiglu_limit": 7.0}, ValueError, "swiglu_limit=10.0"),
+    ({"swiglu_limit": 10.0, "activation": "gelu"}, ValueError, "only valid with activation='silu'"),
+    ({}, ValueError, "CUDA"),
+])
+def test_refusals(changes, error, text):
+    with pytest.raises(error, match=text):
+        _call(**changes)
+
+
+def test_backward_refusals():
+    x, w13, w2 = (torch.zeros(*shape, dtype=torch.bfloat16) for shape in ((3, 16), (48, 16), (16, 24)))
+    h, derivatives = torch.zeros(3, 24, dtype=torch.bfloat16), torch.zeros(3, 48, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="input's shape"):
+        moe.gated_mlp_backward(x[:2], x, w13, w2, h, derivatives)
+    with pytest.raises(ValueError, match="what gated_mlp_forward returned"):
+        moe.gated_mlp_backward(x, x, w13, w2, h[:, :16], derivatives)
+    with pytest.raises(TypeError, match="dy must be torch.bfloat16"):
+        moe.gated_mlp_backward(x.float(), x, w13, w2, h, derivatives)
+    with pytest.raises(ValueError, match="needs"):
+        moe.gated_mlp_backward(x, x, w13, w2, h, derivatives, needs=(True,))
+    with pytest.raises(ValueError, match="CUDA"):
+        moe.gated_mlp_backward(x, x, w13, w2, h, derivatives)
