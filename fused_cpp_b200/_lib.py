@@ -46,7 +46,8 @@ EXPORTS = (
     "fmoe_stage_timer_create", "fmoe_stage_timer_destroy", "fmoe_stage_timer_reset", "fmoe_stage_timer_calls",
     "fmoe_stage_timer_read", "fmoe_route_build_noalloc", "fmoe_ep_dispatch_workspace_bytes", "fmoe_ep_dispatch_prepare",
     "fmoe_w8a8_expert_rows_forward", "fmoe_bf16_expert_rows_forward", "fmoe_ep_combine_finish",
-    "fmoe_i8gemm_dynamic_scaled_mm_pair", "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward", "fmoe_dense_status",
+    "fmoe_i8gemm_dynamic_scaled_mm_pair", "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward",
+    "fmoe_i8gemm_lora_workspace_bytes", "fmoe_i8gemm_dynamic_scaled_mm_lora", "fmoe_dense_status",
     "fmoe_router_topk", "fmoe_append_shared_route",
     "fmoe_ep_peer_create", "fmoe_ep_peer_handle", "fmoe_ep_peer_connect", "fmoe_ep_peer_destroy", "fmoe_ep_peer_slab_bytes",
     "fmoe_ep_peer_dispatch", "fmoe_ep_peer_experts", "fmoe_ep_peer_combine", "fmoe_ep_peer_read_status",
@@ -108,6 +109,11 @@ class Config(ctypes.Structure):
         ("w13_bias", ctypes.c_void_p), ("w2_bias", ctypes.c_void_p), ("route_rows_bf16", ctypes.c_int32),
         ("w8a16_form", ctypes.c_int32),
     ]
+
+
+class LoraAdapters(ctypes.Structure):
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scaling", ctypes.c_void_p), ("count", ctypes.c_int32), ("rank", ctypes.c_int32),
+                ("a_stride", ctypes.c_int32), ("b_stride", ctypes.c_int32)]
 
 
 class WorkspaceLayout(ctypes.Structure):
@@ -182,6 +188,9 @@ def _open(path: str) -> ctypes.CDLL:
     lib.fmoe_route_build_noalloc.argtypes = [p, i64, i32, i32, p, p, p, p, p, p]
     lib.fmoe_i8gemm_dynamic_scaled_mm.argtypes = [p, i32, i64, i32, p, p, p, i32, p, i32, p, ctypes.c_size_t, p]
     lib.fmoe_i8gemm_dynamic_scaled_mm_pair.argtypes = [p, i64, i32, p, p, i32, p, p, p, i32, p, p, ctypes.c_size_t, p]
+    lib.fmoe_i8gemm_lora_workspace_bytes.restype = ctypes.c_size_t
+    lib.fmoe_i8gemm_lora_workspace_bytes.argtypes = [i64, i32, i32, i32]
+    lib.fmoe_i8gemm_dynamic_scaled_mm_lora.argtypes = [p, i64, i32, p, p, p, i32, ctypes.POINTER(LoraAdapters), p, i32, p, i32, p, ctypes.c_size_t, p]
     lib.fmoe_gated_mlp_forward.argtypes = [p, i64, p, p, i64, i32, i32, i32, ctypes.c_float, p, p, p, p]
     lib.fmoe_gated_mlp_backward.argtypes = [p, i64, p, i64, p, p, p, p, i64, i32, i32, p, p, p, p, p]
     lib.fmoe_dense_status.argtypes = [p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]

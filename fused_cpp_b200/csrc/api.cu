@@ -8,6 +8,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "lora.h"
 #ifdef FMOE_DIAG
 #include "diag.h"
 #endif
@@ -975,6 +976,65 @@ int fmoe_i8gemm_dynamic_scaled_mm_pair(const void* x_bf16, int64_t rows, int32_t
   return error == cudaSuccess ? FMOE_OK : cuda_fail(error, "i8gemm pair GEMM");
 }
 
+size_t fmoe_i8gemm_lora_workspace_bytes(int64_t rows, int32_t k, int32_t rank, int32_t out_is_bf16) {
+  if (rows < 0 || k <= 0 || rank <= 0 || rank > fmoe::kLoraMaxRank) return 0;
+  const size_t planes = out_is_bf16 ? 1 : fmoe::kLoraPlanes;
+  return align_up(dense_layout(rows, k).total, 256) + planes * static_cast<size_t>(rows) * fmoe::lora_rank_padded(rank) * 2;
+}
+
+int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t k, const int8_t* w, const float* w_scale, const float* bias,
+                                       int32_t n, const fmoe_lora_adapters* adapters, const void* adapter_ids, int32_t ids_are_64, void* out,
+                                       int32_t out_is_bf16, void* workspace, size_t workspace_bytes, void* stream_ptr) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  int status = check_device();
+  if (status != FMOE_OK) return status;
+  if (rows < 0 || rows > (1ll << 30) || k <= 0 || n <= 0 || n > (1 << 30)) return fail(FMOE_ERR_INVALID_ARGUMENT, "i8gemm lora: rows must lie in [0, 2^30], K and N be positive");
+  if (adapters == nullptr || adapters->a == nullptr || adapters->b == nullptr || adapters->scaling == nullptr) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "i8gemm lora: null adapters");
+  }
+  if (adapters->count <= 0 || adapters->rank <= 0 || adapters->rank > fmoe::kLoraMaxRank) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "i8gemm lora: needs at least one adapter and a rank in [1, %d], got %d of rank %d", fmoe::kLoraMaxRank, adapters->count,
+                adapters->rank);
+  }
+  if (adapters->a_stride < k || adapters->a_stride % 8 != 0 || adapters->b_stride < adapters->rank || adapters->b_stride % 8 != 0 ||
+      reinterpret_cast<uintptr_t>(adapters->a) % 16 != 0 || reinterpret_cast<uintptr_t>(adapters->b) % 16 != 0) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "i8gemm lora: adapter rows must be 16-byte aligned, their strides multiples of 8 and at least a row");
+  }
+  if (rows == 0) return FMOE_OK;
+  if (w == nullptr || w_scale == nullptr || out == nullptr || adapter_ids == nullptr || x_bf16 == nullptr) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "i8gemm lora: null pointer");
+  }
+  const size_t needed = fmoe_i8gemm_lora_workspace_bytes(rows, k, adapters->rank, out_is_bf16);
+  if (workspace == nullptr || workspace_bytes < needed) return fail(FMOE_ERR_WORKSPACE, "i8gemm lora: workspace missing or too small (%zu bytes needed)", needed);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return fail(FMOE_ERR_WORKSPACE, "i8gemm lora: workspace must be 256-byte aligned");
+  const DenseLayout layout = dense_layout(rows, k);
+  char* const base = static_cast<char*>(workspace);
+  fmoe::LoraGemmArgs args = {};
+  args.adapters = {static_cast<const uint16_t*>(adapters->a), static_cast<const uint16_t*>(adapters->b), adapters->a_stride, adapters->b_stride, adapters->scaling,
+                   adapter_ids, ids_are_64, adapters->count, adapters->rank};
+  uint16_t* const t = reinterpret_cast<uint16_t*>(base + align_up(layout.total, 256));
+  args.planes = out_is_bf16 ? 1 : fmoe::kLoraPlanes;
+  cudaError_t error = fmoe::launch_lora_quantize(static_cast<const uint16_t*>(x_bf16), rows, k, layout.k_padded, reinterpret_cast<int8_t*>(base + layout.xq),
+                                                 reinterpret_cast<float*>(base + layout.scale), reinterpret_cast<int*>(base + layout.status), stream);
+  if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora activation quantisation");
+  error = fmoe::launch_lora_shrink(static_cast<const uint16_t*>(x_bf16), rows, k, args.adapters, t, args.planes, stream);
+  if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora coefficients");
+  args.xq = reinterpret_cast<const int8_t*>(base + layout.xq);
+  args.a_scale = reinterpret_cast<const float*>(base + layout.scale);
+  args.weight = w;
+  args.w_scale = w_scale;
+  args.bias = bias;
+  args.out = out;
+  args.out_bf16 = out_is_bf16;
+  args.rows = rows;
+  args.n = n;
+  args.k_padded = layout.k_padded;
+  args.t = t;
+  args.status = reinterpret_cast<int*>(base + layout.status);
+  error = fmoe::launch_lora_gemm(args, stream);
+  return error == cudaSuccess ? FMOE_OK : cuda_fail(error, "i8gemm lora GEMM");
+}
+
 namespace {
 int check_gated_shape(const char* what, int64_t rows, int hidden, int inter) {
   const int status = check_device();
@@ -1017,7 +1077,7 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
   cudaError_t error = fmoe::dense_status_words(&words);
   if (error == cudaSuccess) {
     error = fmoe::launch_gated_projection(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
-                                          swiglu_limit, static_cast<uint16_t*>(h), static_cast<uint16_t*>(by_gate_up), words, stream, false);
+                                          swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(by_gate_up), words, stream, false);
   }
   if (error == cudaSuccess) {
     const fmoe::DenseProductArgs down = {{static_cast<const uint16_t*>(h), inter}, {static_cast<const uint16_t*>(w2), inter}, static_cast<uint16_t*>(y), rows, hidden, inter};
@@ -1051,7 +1111,7 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
   cudaError_t error = fmoe::dense_status_words(&words);
   bool chained = false;
   if (error == cudaSuccess && needs_gate_up) {
-    error = fmoe::launch_gated_backward(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const uint16_t*>(by_gate_up),
+    error = fmoe::launch_gated_backward(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const float*>(by_gate_up),
                                         rows, hidden, inter, static_cast<uint16_t*>(d_gate_up), words, stream, chained);
     chained = true;
   }

@@ -292,6 +292,8 @@ inline cudaError_t launch_streaming(void (*kernel)(Params...), dim3 grid, unsign
 // 2-D tensor [rows, k] with 128-byte-swizzled boxes of {128 bytes of a row, box_rows} (umma_gemm.cu); row_stride: elements from a row
 // to the next, 0 = k.
 bool make_sw128_map(CUtensorMap* map, const void* base, bool int8, uint64_t rows, uint64_t k, uint32_t box_rows, uint64_t row_stride = 0);
+// 3-D bf16 tensor [planes, rows, columns], row_stride elements from a row to the next, boxes of {128 bytes of a row, box_rows} of one plane.
+bool make_sw128_map_3d(CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows, uint64_t planes, uint64_t row_stride, uint32_t box_rows);
 
 // ---- gated_gemm.cu: dense bf16 products of the gated feed-forward block over many rows (two-SM kernel).
 // out[m, n] = sum over k of A[m, k] B[n, k]; an operand marked `by_k` lies in memory as [k, m] or [k, n].
@@ -307,11 +309,11 @@ struct DenseProductArgs {
   int64_t k;
 };
 // h = act(x Wg^T, x Wu^T) for rows x [rows, hidden] and w13 [2 * inter, hidden]; by_gate_up (nullable): the partial derivatives of h by gate
-// and up, [rows, 2 * inter].
+// and up, fp32 [rows, 2 * inter].
 cudaError_t launch_gated_projection(const uint16_t* x, int64_t x_stride, const uint16_t* w13, int64_t rows, int hidden, int inter, int activation,
-                                    float limit, uint16_t* h, uint16_t* by_gate_up, int* status, cudaStream_t stream, bool chained);
+                                    float limit, uint16_t* h, float* by_gate_up, int* status, cudaStream_t stream, bool chained);
 // d_gate_up = (dy W2) times the partial derivatives, [rows, 2 * inter], for w2 [hidden, inter].
-cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const uint16_t* by_gate_up, int64_t rows, int hidden,
+cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* by_gate_up, int64_t rows, int hidden,
                                   int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained);
 // The status block (kStatusWords ints, zero unless a bounded wait gave up) of the current device for launches without a workspace.
 cudaError_t dense_status_words(int** words);

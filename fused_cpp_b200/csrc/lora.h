@@ -1,0 +1,63 @@
+// Low-rank adapters of many requests beside a dense W8A8 projection: arguments of the kernels in lora_shrink.cu and lora_gemm.cu.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace fmoe {
+
+constexpr int kLoraMaxRank = 512;
+constexpr int kLoraRankBlock = 64;  // ranks of a K block of the adapters' product: 128 bytes
+constexpr int kLoraPlanes = 3;      // bf16 terms of a coefficient where the result has 32 bits
+
+// Rows of the coefficients t are padded to this many ranks, with zeros: the K of one MMA.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+constexpr int lora_rank_padded(int rank) { return (rank + 15) / 16 * 16; }
+
+struct LoraAdapters {
+  const uint16_t* a;  // bf16 [count, rank, a_stride], a_stride >= k a multiple of 8, zeros behind k
+  const uint16_t* b;  // bf16 [count, n, b_stride], b_stride >= rank a multiple of 8, zeros behind rank
+  int a_stride, b_stride;
+  const float* scaling;  // [count]
+  const void* ids;       // int32 or int64 [rows]: an id outside [0, count) means no adapter
+  int ids_are_64;
+  int count, rank;
+};
+
+#ifdef __CUDACC__
+// (Through L2: the kernels read ids in front of their wait, see launch_chained.)
+__device__ __forceinline__ int load_adapter_id(const LoraAdapters& adapters, int64_t row) {
+  const int64_t id = adapters.ids_are_64 ? __ldcg(static_cast<const long long*>(adapters.ids) + row) : __ldcg(static_cast<const int*>(adapters.ids) + row);
+  return id >= 0 && id < adapters.count ? static_cast<int>(id) : -1;
+}
+#endif
+
+// Rows of x as int8 [rows, k_padded] with a scale each, zeros behind k; clears the status block of the call.
+cudaError_t launch_lora_quantize(const uint16_t* x, int64_t rows, int k, int k_padded, int8_t* q, float* scale, int* status, cudaStream_t stream);
+
+// t[plane][row][rank] = scaling[id] * (A[id] x[row]) for the rows that have an adapter (the others' are left as they are), as `planes` bf16
+// terms.  A programmatic dependent of the kernel in front, of which it needs nothing.
+cudaError_t launch_lora_shrink(const uint16_t* x, int64_t rows, int k, const LoraAdapters& adapters, uint16_t* t, int planes, cudaStream_t stream);
+
+// out[row, n] = dequantised product (+ bias) + sum over ranks of t[row, rank] B[id, n, rank].  A programmatic dependent of
+// launch_lora_shrink.
+struct LoraGemmArgs {
+  const int8_t* xq;      // [rows, k_padded]
+  const float* a_scale;  // [rows]
+  const int8_t* weight;  // [n, k_padded]
+  const float* w_scale;  // [n]
+  const float* bias;     // [n] or null
+  void* out;             // [rows, n]
+  int out_bf16;
+  int64_t rows;
+  int n, k_padded;
+  LoraAdapters adapters;
+  const uint16_t* t;
+  int planes;
+  int* status;
+};
+cudaError_t launch_lora_gemm(const LoraGemmArgs& args, cudaStream_t stream);
+
+}  // namespace fmoe

@@ -1,0 +1,496 @@
+// Dense W8A8 linear with the low-rank adapters of many requests:
+//   out[row, n] = (acc * row scale) * channel scale (+ bias[n]) + sum over r of t[row, r] B[a, n, r],   acc = Xq W^T, a = the row's adapter,
+// with the coefficients t of lora_shrink.cu.  The kernel of dense_gemm.cu (128 output channels of a cluster of `parts` CTAs that split the K
+// range; their int32 sums meet in distributed shared memory) with the adapters' product beside it, in a second accumulator of tensor memory:
+//   * Rows of a tile may have any adapters in any order.  For each adapter in use by the rows, [t of its rows, zeros for the others] x B[a]^T
+//     is a K block of bf16 MMAs: 64 ranks are one 128-byte row as the weights' K blocks are, B[a] comes by the same ring of
+//     stages, and a warp writes the masked coefficients where the token tile would lie.  A row's sum has only its own adapter's products and exact
+//     zeros in it (adapters are finite by contract), whatever its neighbours ask for.
+//   * A CTA finishes the rows [part * R, part * R + R) of its tile (R = rows / parts): it multiplies the adapters of those rows alone, so that
+//     nothing of that product is exchanged, and every adapter's channels are read by the CTAs whose rows use it.
+//   * The list of adapters comes from the ids before the wait for the kernels in front; what is behind it is the t and the tokens.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "lora.h"
+#include "ptx.cuh"
+
+namespace fmoe {
+
+namespace {
+
+constexpr int kBlockM = 128;        // output channels per CTA (TMEM lanes)
+constexpr int kBlockKBytes = 128;   // bytes of K per pipeline stage = one 128-byte swizzle row
+constexpr int kUmmaKBytes = 32;     // bytes of K per tcgen05.mma, of either kind
+constexpr int kThreads = 224;       // warp 0: TMA, warp 1: tensor memory and MMA, warps 2..5: epilogue, warp 6: masked coefficients
+constexpr int kWeightBytes = kBlockM * kBlockKBytes;
+constexpr int kMaxStages = 10;
+constexpr int kMaxParts = 8;
+constexpr int kMinPartBlocks = 2;
+constexpr int kTileRows = 128;
+
+template <int kRowTile, bool kDeep>
+struct LoraConfig {
+  static constexpr int kTokenBytes = kRowTile * kBlockKBytes;
+  static constexpr int kStageBytes = kWeightBytes + kTokenBytes;
+  static constexpr int kBudget = kDeep ? 200 * 1024 : 98 * 1024;
+  static constexpr int kStages = kBudget / kStageBytes < kMaxStages ? kBudget / kStageBytes : kMaxStages;
+  static constexpr int kTmemColumns = 2 * kRowTile;  // the int32 and the fp32 accumulator
+  static constexpr size_t kSmemBytes = 1024 /*alignment slack*/ + static_cast<size_t>(kStages) * kStageBytes + 4096 /*control block*/;
+  static_assert(kStages * kStageBytes >= kRowTile * kBlockM * 4, "the accumulator exchange reuses the stages");
+};
+
+struct LoraControl {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t vacant[kMaxStages];        // the producer found the stage empty and leaves its token tile to the coefficients
+  uint64_t coefficients[kMaxStages];  // the masked coefficients of the stage are written
+  uint64_t acc_full;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+  int slots;
+  alignas(16) float row_scale[kTileRows];
+  alignas(16) float channel_scale[kBlockM];
+  alignas(16) float channel_bias[kBlockM];
+  int id[kTileRows];
+  int slot_adapter[kTileRows];
+};
+static_assert(sizeof(LoraControl) <= 4096, "control block exceeds its shared-memory reservation");
+
+struct KernelArgs {
+  LoraGemmArgs g;
+  int row_tiles, k_blocks, parts, vector_store, rank_blocks;
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      :
+      : "r"(ptx::smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ float finish(int acc, float row_scale, float channel_scale, float bias, float delta) {
+  return __fadd_rn(__fadd_rn(dequantize(acc, row_scale, channel_scale, FMOE_NUMERICS_TORCHREF), bias), delta);
+}
+
+template <int kRowTile, bool kDeep>
+__global__ void __launch_bounds__(kThreads)
+lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap token_map, const __grid_constant__ CUtensorMap b_map,
+                 const __grid_constant__ KernelArgs args) {
+  using Cfg = LoraConfig<kRowTile, kDeep>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  LoraControl* ctl = reinterpret_cast<LoraControl*>(smem + static_cast<size_t>(Cfg::kStages) * Cfg::kStageBytes);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  int* status = args.g.status;
+  const int parts = args.parts;
+  const int part = static_cast<int>(blockIdx.x) % parts;  // = rank in the cluster
+  const int unit = static_cast<int>(blockIdx.x) / parts;  // row tiles of a channel block side by side: they share its weights
+  const int block = unit / args.row_tiles;
+  const int64_t row0 = static_cast<int64_t>(unit - block * args.row_tiles) * kRowTile;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kRowTile), args.g.rows - row0));
+  const int rows_per_part = (rows + parts - 1) / parts;
+  const int own_first = min(part * rows_per_part, rows);  // the rows of the tile that this CTA finishes
+  const int own = min(rows_per_part, rows - own_first);
+  const int n = args.g.n;
+  const int n0 = block * kBlockM;
+  const int kb_begin = part * args.k_blocks / parts;
+  const int count = (part + 1) * args.k_blocks / parts - kb_begin;  // K blocks of this CTA, at least one
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::kStages; ++s) {
+      ptx::mbar_init(&ctl->full[s], 1);
+      ptx::mbar_init(&ctl->empty[s], 1);
+      ptx::mbar_init(&ctl->vacant[s], 1);
+      ptx::mbar_init(&ctl->coefficients[s], 1);
+    }
+    ptx::mbar_init(&ctl->acc_full, 1);
+    ctl->abort_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(&ctl->tmem_base, Cfg::kTmemColumns);
+    ptx::tmem_relinquish();
+  }
+  if (warp == 6) {
+    // The adapters of the own rows, each once, in the order of their first rows.
+    int slots = 0;
+    for (int base = 0; base < own; base += 32) {
+      const int i = base + lane;
+      const int id = i < own ? load_adapter_id(args.g.adapters, row0 + own_first + i) : -1;
+      if (i < own) ctl->id[i] = id;
+      const unsigned same = __match_any_sync(0xffffffffu, id);
+      bool first = id >= 0 && (same & ((1u << lane) - 1)) == 0;
+      __syncwarp();
+      if (first) {
+        for (int j = 0; j < slots; ++j) first = first && ctl->slot_adapter[j] != id;
+      }
+      const unsigned firsts = __ballot_sync(0xffffffffu, first);
+      if (first) ctl->slot_adapter[slots + __popc(firsts & ((1u << lane) - 1))] = id;
+      slots += __popc(firsts);
+      __syncwarp();
+    }
+    if (lane == 0) ctl->slots = slots;
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  volatile int* abort_flag = &ctl->abort_flag;
+  const int slots = __shfl_sync(0xffffffffu, ctl->slots, 0);
+  // K blocks of the adapters' product: every adapter's rank blocks, the planes of each.
+  const int per_slot = args.rank_blocks * args.g.planes;
+  const int extra = slots * per_slot;
+  const int all = count + extra;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (the whole warp walks the loops, one elected lane issues) ----------------
+    const bool issuer = ptx::elect_one();
+    const int ahead = count < Cfg::kStages ? count : Cfg::kStages;
+    // Weights of the first stages: they do not depend on the kernels that may still be running.
+    for (int i = 0; i < ahead; ++i) {
+      if (issuer) {
+        ptx::mbar_arrive_expect_tx(&ctl->full[i], Cfg::kStageBytes);
+        ptx::tma_load_2d(smem + static_cast<size_t>(i) * Cfg::kStageBytes, &weight_map, &ctl->full[i], (kb_begin + i) * kBlockKBytes, n0);
+      }
+    }
+    ptx::grid_dependency_wait();
+    for (int i = 0; i < ahead; ++i) {
+      if (issuer) {
+        ptx::tma_load_2d(smem + static_cast<size_t>(i) * Cfg::kStageBytes + kWeightBytes, &token_map, &ctl->full[i], (kb_begin + i) * kBlockKBytes,
+                         static_cast<int>(row0));
+      }
+    }
+    int stage = ahead == Cfg::kStages ? 0 : ahead;
+    uint32_t phase = ahead == Cfg::kStages ? 1u : 0u;
+    for (int i = ahead; i < all; ++i) {
+      ptx::mbar_wait(&ctl->empty[stage], phase ^ 1u, abort_flag, status, 51);
+      if (issuer) {
+        uint8_t* stage_base = smem + static_cast<size_t>(stage) * Cfg::kStageBytes;
+        if (i < count) {
+          ptx::mbar_arrive_expect_tx(&ctl->full[stage], Cfg::kStageBytes);
+          ptx::tma_load_2d(stage_base, &weight_map, &ctl->full[stage], (kb_begin + i) * kBlockKBytes, n0);
+          ptx::tma_load_2d(stage_base + kWeightBytes, &token_map, &ctl->full[stage], (kb_begin + i) * kBlockKBytes, static_cast<int>(row0));
+        } else {
+          const int u = i - count;
+          const int rank_block = u % per_slot / args.g.planes;
+          ptx::mbar_arrive(&ctl->vacant[stage]);
+          ptx::mbar_arrive_expect_tx(&ctl->full[stage], kWeightBytes);
+          tma_load_3d(stage_base, &b_map, &ctl->full[stage], rank_block * kLoraRankBlock, n0, ctl->slot_adapter[u / per_slot]);
+        }
+      }
+      if (++stage == Cfg::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // Drain: every load must have landed before the CTA may exit (the MMA warp has consumed them unless it gave up).
+    const int pending = all < Cfg::kStages ? all : Cfg::kStages;
+    for (int back = 0; back < pending; ++back) {
+      int s = stage - 1 - back;
+      uint32_t p = phase;
+      if (s < 0) {
+        s += Cfg::kStages;
+        p ^= 1u;
+      }
+      const unsigned long long start = ptx::global_timer_ns();
+      while (!ptx::mbar_try_wait(&ctl->full[s], p)) {
+        if (ptx::global_timer_ns() - start > ptx::kWaitLimitNs) break;
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    const bool issuer = ptx::elect_one();
+    const uint32_t idesc = ptx::make_instr_desc(true, kBlockM, (rows + 15) & ~15);
+    const uint32_t idesc_extra = ptx::make_instr_desc(false, kBlockM, (own + 15) & ~15);
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t used = 0;  // stages, one bit each, whose coefficients barrier is in its odd phase
+    for (int i = 0; i < all; ++i) {
+      ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 52);
+      if (i >= count) {
+        ptx::mbar_wait(&ctl->coefficients[stage], (used >> stage) & 1u, abort_flag, status, 53);
+        used ^= 1u << stage;
+      }
+      ptx::tcgen05_fence_after();
+      const uint32_t stage_addr = ptx::smem_u32(smem + static_cast<size_t>(stage) * Cfg::kStageBytes);
+      if (issuer) {
+        if (i < count) {
+#pragma unroll
+          for (int ks = 0; ks < kBlockKBytes / kUmmaKBytes; ++ks) {
+            ptx::umma_ss<true>(tmem_base, ptx::make_smem_desc_sw128(stage_addr + ks * kUmmaKBytes),
+                               ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + ks * kUmmaKBytes), idesc, (i > 0 || ks > 0) ? 1u : 0u);
+          }
+        } else {
+          const int rank_block = (i - count) % per_slot / args.g.planes;
+          const int steps = (min(kLoraRankBlock, args.g.adapters.rank - rank_block * kLoraRankBlock) + 15) >> 4;
+          for (int ks = 0; ks < steps; ++ks) {
+            ptx::umma_ss<false>(tmem_base + kRowTile, ptx::make_smem_desc_sw128(stage_addr + ks * kUmmaKBytes),
+                                ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + ks * kUmmaKBytes), idesc_extra, (i > count || ks > 0) ? 1u : 0u);
+          }
+        }
+        ptx::tcgen05_commit(&ctl->empty[stage]);
+      }
+      if (++stage == Cfg::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (issuer) ptx::tcgen05_commit(&ctl->acc_full);
+  } else if (warp == 6) {
+    // ---------------- masked coefficients ----------------
+    ptx::grid_dependency_wait();
+    const int rank_padded = lora_rank_padded(args.g.adapters.rank);
+    const int own16 = (own + 15) & ~15;
+    const uint16_t* const t_rows = args.g.t + (row0 + own_first) * rank_padded;
+    int stage = count % Cfg::kStages;
+    uint32_t used = 0;  // stages, one bit each, whose vacant barrier is in its odd phase
+    for (int u = 0; u < extra; ++u) {
+      const int adapter = ctl->slot_adapter[u / per_slot];
+      const int inside = u % per_slot;
+      const int rank0 = inside / args.g.planes * kLoraRankBlock;
+      const int plane = inside % args.g.planes;
+      const int pieces = 2 * ((min(kLoraRankBlock, args.g.adapters.rank - rank0) + 15) >> 4);  // of 16 bytes in a row: a power of two but for 6
+      const uint16_t* const from = t_rows + static_cast<int64_t>(plane) * args.g.rows * rank_padded + rank0;
+      // (Not the empty barrier itself: this warp does not see its earlier phases, and would take one for another.)
+      ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 54);
+      used ^= 1u << stage;
+      uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + kWeightBytes;
+      for (int e = lane; e < own16 * pieces; e += 32) {
+        const int row = e / pieces, piece = e - row * pieces;
+        uint4 value = make_uint4(0, 0, 0, 0);
+        if (row < own && ctl->id[row] == adapter) value = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(row) * rank_padded) + piece);
+        // The 128-byte swizzle that the operand tiles have: the 16-byte piece's number is xor-ed with the row's in its group of eight.
+        *reinterpret_cast<uint4*>(to + row * kBlockKBytes + ((piece ^ (row & 7)) << 4)) = value;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&ctl->coefficients[stage]);
+      if (++stage == Cfg::kStages) stage = 0;
+    }
+  }
+
+  // ---------------- epilogue (warps 2..5): one thread per channel ----------------
+  const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id % 4
+  const int channel = quarter * 32 + lane;
+  const bool channel_ok = n0 + channel < n;
+  const bool epilogue = warp >= 2 && warp < 6;
+  float channel_scale = 1.0f, bias = 0.0f;
+  int* exchange = reinterpret_cast<int*>(smem);  // [rows][128 channels], once the stages are done with
+  const uint32_t acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+  if (epilogue) {
+    const int thread = static_cast<int>(threadIdx.x) - 64;
+    // Before the wait, hence through L2: a scale or bias that an earlier call read at this address may still lie in L1.
+    if (channel_ok) {
+      channel_scale = __ldcg(args.g.w_scale + n0 + channel);
+      if (args.g.bias != nullptr) bias = __ldcg(args.g.bias + n0 + channel);
+    }
+    ctl->channel_scale[channel] = channel_scale;
+    ctl->channel_bias[channel] = bias;
+    ptx::grid_dependency_wait();  // the row scales come from the quantiser
+    if (thread < rows) ctl->row_scale[thread] = __ldcg(args.g.a_scale + row0 + thread);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    ptx::mbar_wait(&ctl->acc_full, 0, abort_flag, status, 55);
+    ptx::tcgen05_fence_after();
+    for (int c0 = 0; c0 < rows; c0 += 16) {
+      uint32_t bits[16], delta[16];
+      ptx::tmem_ld_x8(acc + c0, bits);
+      ptx::tmem_ld_x8(acc + c0 + 8, bits + 8);
+      if (parts == 1 && extra > 0) {
+        ptx::tmem_ld_x8(acc + kRowTile + c0, delta);
+        ptx::tmem_ld_x8(acc + kRowTile + c0 + 8, delta + 8);
+      }
+      ptx::tmem_ld_wait();
+      if (parts > 1) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) exchange[(c0 + j) * kBlockM + channel] = static_cast<int>(bits[j]);
+      } else if (channel_ok) {
+        const int count16 = min(16, rows - c0);
+        const int64_t index = (row0 + c0) * n + n0 + channel;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (j >= count16) break;
+          const float value = finish(static_cast<int>(bits[j]), ctl->row_scale[c0 + j], channel_scale, bias, extra > 0 ? __uint_as_float(delta[j]) : 0.0f);
+          if (args.g.out_bf16) {
+            static_cast<uint16_t*>(args.g.out)[index + static_cast<int64_t>(j) * n] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
+          } else {
+            static_cast<float*>(args.g.out)[index + static_cast<int64_t>(j) * n] = value;
+          }
+        }
+      }
+      __syncwarp();  // the next tensor-memory load wants the whole warp
+    }
+  }
+  if (parts > 1) {
+    __syncwarp();
+    cluster_sync();  // every part's accumulators lie in its shared memory
+    if (epilogue) {
+      // A thread finishes its channel of the own rows, sixteen at a time: their adapters' sums lie in its lane of tensor memory.
+      const uint32_t mine = ptx::smem_u32(exchange) + 4u * static_cast<uint32_t>(channel);
+      for (int c0 = 0; c0 < own; c0 += 16) {
+        uint32_t delta[16];
+        if (extra > 0) {
+          ptx::tmem_ld_x8(acc + kRowTile + c0, delta);
+          ptx::tmem_ld_x8(acc + kRowTile + c0 + 8, delta + 8);
+          ptx::tmem_ld_wait();
+        }
+        const int count16 = min(16, own - c0);
+        int sums[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sums[j] = 0;
+        for (int c = 0; c < parts; ++c) {
+          uint32_t remote;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(mine), "r"(c));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (j >= count16) break;
+            int value;
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(value) : "r"(remote + static_cast<uint32_t>(own_first + c0 + j) * (kBlockM * 4)) : "memory");
+            sums[j] += value;
+          }
+        }
+        if (channel_ok) {
+          const int64_t index = (row0 + own_first + c0) * n + n0 + channel;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (j >= count16) break;
+            const float value = finish(sums[j], ctl->row_scale[own_first + c0 + j], channel_scale, bias, extra > 0 ? __uint_as_float(delta[j]) : 0.0f);
+            if (args.g.out_bf16) {
+              static_cast<uint16_t*>(args.g.out)[index + static_cast<int64_t>(j) * n] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
+            } else {
+              static_cast<float*>(args.g.out)[index + static_cast<int64_t>(j) * n] = value;
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no part leaves while another may still read its accumulators
+  }
+
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tcgen05_fence_after();
+    ptx::tmem_dealloc(tmem_base, Cfg::kTmemColumns);
+  }
+}
+
+// How many clusters of 1 .. kMaxParts CTAs can be resident at once with one CTA per SM (asked once per device).
+struct Residency {
+  int clusters[kMaxParts + 1] = {};
+};
+
+template <int kRowTile, bool kDeep>
+cudaError_t configure() {
+  auto kernel = lora_gemm_kernel<kRowTile, kDeep>;
+  const cudaError_t error =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(LoraConfig<kRowTile, kDeep>::kSmemBytes));
+  return error != cudaSuccess ? error : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
+template <int kRowTile>
+cudaError_t residency(Residency* out) {
+  static std::mutex guard;  // a thread that finds the flag set has to find the table too
+  static PerDeviceOnce configured;
+  static Residency known[kMaxDevices];
+  const std::lock_guard<std::mutex> lock(guard);
+  const int device = current_device_ordinal();
+  if (!configured.needed(device)) {
+    *out = known[device];
+    return cudaSuccess;
+  }
+  cudaError_t error = configure<kRowTile, true>();
+  if (error == cudaSuccess) error = configure<kRowTile, false>();
+  for (int parts = 1; parts <= kMaxParts && error == cudaSuccess; ++parts) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(parts));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = LoraConfig<kRowTile, true>::kSmemBytes;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = static_cast<unsigned>(parts);
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    error = cudaOccupancyMaxActiveClusters(&out->clusters[parts], lora_gemm_kernel<kRowTile, true>, &config);
+  }
+  if (error != cudaSuccess) return error;
+  if (device >= 0 && device < kMaxDevices) known[device] = *out;
+  configured.mark(device);
+  return cudaSuccess;
+}
+
+template <int kRowTile, bool kDeep>
+cudaError_t launch_kernel(const KernelArgs& args, int64_t blocks, const CUtensorMap* maps, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(blocks * args.parts));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = LoraConfig<kRowTile, kDeep>::kSmemBytes;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = static_cast<unsigned>(args.parts);
+  attributes[0].val.clusterDim.y = 1;
+  attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
+  return cudaLaunchKernelEx(&config, lora_gemm_kernel<kRowTile, kDeep>, maps[0], maps[1], maps[2], args);
+}
+
+template <int kRowTile>
+cudaError_t launch_tile(KernelArgs args, cudaStream_t stream) {
+  const LoraGemmArgs& g = args.g;
+  const uint64_t k = static_cast<uint64_t>(g.k_padded);
+  CUtensorMap maps[3];
+  if (!make_sw128_map(&maps[0], g.weight, true, g.n, k, kBlockM) || !make_sw128_map(&maps[1], g.xq, true, g.rows, k, kRowTile) ||
+      !make_sw128_map_3d(&maps[2], g.adapters.b, g.adapters.rank, g.n, g.adapters.count, g.adapters.b_stride, kBlockM)) {
+    return cudaErrorInvalidValue;
+  }
+  Residency one_per_sm;
+  const cudaError_t error = residency<kRowTile>(&one_per_sm);
+  if (error != cudaSuccess) return error;
+  args.row_tiles = static_cast<int>((g.rows + kRowTile - 1) / kRowTile);
+  const int64_t blocks = static_cast<int64_t>((g.n + kBlockM - 1) / kBlockM) * args.row_tiles;
+  if (blocks > (1ll << 27)) return cudaErrorInvalidValue;
+  // As many parts as leave all clusters resident at once, two CTAs per SM if need be, every part at least two K blocks (dense_gemm.cu).
+  args.parts = 1;
+  for (int parts = kMaxParts; parts > 1; --parts) {
+    if (blocks <= 2 * one_per_sm.clusters[parts] && parts * kMinPartBlocks <= args.k_blocks) {
+      args.parts = parts;
+      break;
+    }
+  }
+  if (blocks <= one_per_sm.clusters[args.parts]) return launch_kernel<kRowTile, true>(args, blocks, maps, stream);
+  return launch_kernel<kRowTile, false>(args, blocks, maps, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_lora_gemm(const LoraGemmArgs& g, cudaStream_t stream) {
+  KernelArgs args = {};
+  args.g = g;
+  args.k_blocks = (g.k_padded + kBlockKBytes - 1) / kBlockKBytes;
+  args.rank_blocks = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  if (g.rows <= 16) return launch_tile<16>(args, stream);
+  if (g.rows <= 32) return launch_tile<32>(args, stream);
+  if (g.rows <= 64) return launch_tile<64>(args, stream);
+  return launch_tile<128>(args, stream);
+}
+
+}  // namespace fmoe

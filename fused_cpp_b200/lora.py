@@ -1,0 +1,128 @@
+"""Low-rank adapters resident on the GPU, for the projections that serve many requests at once.
+
+    adapters = lora.prepare_adapters(a, b, scaling)          # [L, R, K], [L, N, R]; once, when adapters are loaded
+    y = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, adapter_ids)
+    y = deepseek_v4_w8a8.deepseek_v4_w8a8_linear(x, weight, adapters=adapters, adapter_ids=adapter_ids)
+
+Row m of a batch gets scaling[a] * B[a] (A[a] x[m]) added to its projection, a = adapter_ids[m]; an id outside [0, L), as -1, means none.
+`set_adapter` exchanges one of them in place while the others serve.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+from typing import Sequence
+
+import torch
+
+from . import _lib
+
+MAX_RANK = 512
+_QUANTUM = 8  # elements of a 16-byte vector
+
+
+@dataclass(frozen=True)
+class PreparedAdapters:
+    """GPU-resident adapters of one projection (opaque to callers): A [count, rank, K] and B [count, N, rank] in rows padded with zeros to
+    whole 16-byte vectors, scaling fp32 [count]."""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    scaling: torch.Tensor
+    count: int
+    rank: int
+    k: int
+    n: int
+    native: _lib.LoraAdapters = field(repr=False, compare=False, default=None)
+
+
+def _check_pair(a, b, where: str) -> None:
+    for name, tensor in (("a", a), ("b", b)):
+        if not isinstance(tensor, torch.Tensor):
+            raise TypeError(f"{where}: {name} must be a torch.Tensor")
+        if tensor.dtype != torch.bfloat16:
+            raise TypeError(f"{where}: {name} must be torch.bfloat16, got {tensor.dtype}")
+        if tensor.dim() != 2:
+            raise ValueError(f"{where}: an adapter is a [R, K] and b [N, R], got {name} of {tuple(tensor.shape)}")
+    if a.shape[0] != b.shape[1]:
+        raise ValueError(f"{where}: a [R, K] and b [N, R] must share R, got {tuple(a.shape)} and {tuple(b.shape)}")
+
+
+def _require_finite(where: str, *tensors) -> None:
+    # A product of all rows with an infinite or undefined weight would reach the rows of other requests.
+    if not all(bool(torch.isfinite(t).all()) for t in tensors):
+        raise ValueError(f"{where}: adapters and their scaling must be finite")
+
+
+def prepare_adapters(a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor | Sequence[torch.Tensor],
+                     scaling: float | Sequence[float] | torch.Tensor = 1.0) -> PreparedAdapters:
+    """Adapters of one projection [N, K], on the current CUDA device: bf16 a [L, R, K] and b [L, N, R], or sequences of [R_i, K] and
+    [N, R_i] of unequal ranks (R is the largest, the others are padded with zeros).  scaling: one number, or one per adapter."""
+    where = "prepare_adapters"
+    firsts, seconds = list(a), list(b)
+    if not firsts or len(firsts) != len(seconds):
+        raise ValueError(f"{where}: needs as many a as b, and at least one")
+    for first, second in zip(firsts, seconds):
+        _check_pair(first, second, where)
+    count, k, n = len(firsts), int(firsts[0].shape[1]), int(seconds[0].shape[0])
+    rank = max(int(first.shape[0]) for first in firsts)
+    if any(first.shape[1] != k for first in firsts) or any(second.shape[0] != n for second in seconds):
+        raise ValueError(f"{where}: all adapters must share K and N")
+    if not 1 <= rank <= MAX_RANK or k < 1 or n < 1 or any(first.shape[0] < 1 for first in firsts):
+        raise ValueError(f"{where}: ranks must lie in [1, {MAX_RANK}] and K and N be positive")
+    factors = torch.as_tensor(scaling, dtype=torch.float32).detach().reshape(-1)
+    if factors.numel() not in (1, count):
+        raise ValueError(f"{where}: scaling must be one number or one per adapter")
+    if not _lib.device_supported():
+        raise RuntimeError("lora backend unavailable: no compute-capability-10.x CUDA device (there is no CPU path)")
+    device = torch.device("cuda", torch.cuda.current_device())
+    a_rows = torch.zeros((count, rank, -(-k // _QUANTUM) * _QUANTUM), dtype=torch.bfloat16, device=device)
+    b_rows = torch.zeros((count, n, -(-rank // _QUANTUM) * _QUANTUM), dtype=torch.bfloat16, device=device)
+    if all(first.shape[0] == rank for first in firsts) and isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor):
+        a_rows[:, :, :k] = a
+        b_rows[:, :, :rank] = b
+    else:
+        for i, (first, second) in enumerate(zip(firsts, seconds)):
+            a_rows[i, : first.shape[0], :k] = first
+            b_rows[i, :, : first.shape[0]] = second
+    factors = factors.to(device).expand(count).contiguous()
+    _require_finite(where, a_rows, b_rows, factors)
+    native = _lib.LoraAdapters(a_rows.data_ptr(), b_rows.data_ptr(), factors.data_ptr(), count, rank, a_rows.shape[2], b_rows.shape[2])
+    return PreparedAdapters(a_rows, b_rows, factors, count, rank, k, n, native)
+
+
+def set_adapter(adapters: PreparedAdapters, index: int, a: torch.Tensor, b: torch.Tensor, scaling: float = 1.0) -> None:
+    """Puts [R_i, K] and [N, R_i], R_i at most the prepared rank, in the place of adapter `index`, on the current stream."""
+    where = "set_adapter"
+    if not isinstance(adapters, PreparedAdapters):
+        raise TypeError(f"{where}: adapters must come from prepare_adapters")
+    _check_pair(a, b, where)
+    if not 0 <= int(index) < adapters.count:
+        raise ValueError(f"{where}: index must lie in [0, {adapters.count})")
+    rank = int(a.shape[0])
+    if not 1 <= rank <= adapters.rank or a.shape[1] != adapters.k or b.shape[0] != adapters.n:
+        raise ValueError(f"{where}: expected a [R <= {adapters.rank}, {adapters.k}] and b [{adapters.n}, R], got {tuple(a.shape)} and {tuple(b.shape)}")
+    _require_finite(where, a, b, torch.tensor(float(scaling)))
+    with torch.no_grad():
+        adapters.a[index, :rank, : adapters.k] = a
+        adapters.a[index, rank:] = 0
+        adapters.b[index, :, :rank] = b
+        adapters.b[index, :, rank:] = 0
+        adapters.scaling[index] = float(scaling)
+
+
+def projection(x: torch.Tensor, packed, adapters: PreparedAdapters, adapter_ids: torch.Tensor, bias: torch.Tensor | None,
+               out: torch.Tensor) -> None:
+    """out [M, N] of bf16 rows x [M, K], checked by the caller; the workspace is the call's own, so that calls on several streams and
+    captured ones do not share it."""
+    rows, k = x.shape
+    lib = _lib.load()
+    out_is_bf16 = 1 if out.dtype == torch.bfloat16 else 0
+    nbytes = lib.fmoe_i8gemm_lora_workspace_bytes(rows, k, adapters.rank, out_is_bf16)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _lib.check(lib.fmoe_i8gemm_dynamic_scaled_mm_lora(
+        x.data_ptr(), rows, k, packed.packed_weight.data_ptr(), packed.weight_scale.data_ptr(), _lib._ptr(bias), packed.n, ctypes.byref(adapters.native),
+        adapter_ids.data_ptr(), 1 if adapter_ids.dtype == torch.int64 else 0, out.data_ptr(), out_is_bf16, workspace.data_ptr(), nbytes, _lib._stream()))
+
+
+__all__ = ["MAX_RANK", "PreparedAdapters", "prepare_adapters", "set_adapter"]

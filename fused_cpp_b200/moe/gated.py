@@ -8,7 +8,7 @@ activations, as plain tensors that an optimiser updates.  Both projections, the 
 second; the backward pass is three launches.  Sums are fp32; h = act(..) is rounded to bf16 for the down projection, as in the fused MoE
 operators.  `gated_mlp_forward` and `gated_mlp_backward` are the two passes for programs that keep their own tape.
 
-What a forward pass keeps for the backward pass besides its inputs: h [T, F] and the partial derivatives of h by gate and by up, bf16 [T, 2F].
+What a forward pass keeps for the backward pass besides its inputs: h [T, F] and the partial derivatives of h by gate and by up, fp32 [T, 2F].
 """
 from __future__ import annotations
 
@@ -84,7 +84,7 @@ def _forward(rows, w13, w2, code: int, limit: float, keep: bool, y):
     count, hidden = rows.shape
     inter = w2.shape[1]
     h = torch.empty((count, inter), dtype=torch.bfloat16, device=rows.device)
-    derivatives = torch.empty((count, 2 * inter), dtype=torch.bfloat16, device=rows.device) if keep else None
+    derivatives = torch.empty((count, 2 * inter), dtype=torch.float32, device=rows.device) if keep else None
     _lib.check(_lib.load().fmoe_gated_mlp_forward(rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), count, hidden, inter, code, limit,
                                                   h.data_ptr(), _lib._ptr(derivatives), y.data_ptr(), _lib._stream()))
     return h, derivatives
@@ -100,7 +100,7 @@ def _backward(dy, rows, w13, w2, h, derivatives, needs):
     dw2 = torch.empty((hidden, inter), dtype=torch.bfloat16, device=rows.device) if needs[2] else None
     d_gate_up = torch.empty((count, 2 * inter), dtype=torch.bfloat16, device=rows.device) if needs[0] or needs[1] else None
     _lib.check(_lib.load().fmoe_gated_mlp_backward(dy.data_ptr(), _stride(dy), rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), h.data_ptr(),
-                                                   derivatives.data_ptr(), count, hidden, inter, _lib._ptr(d_gate_up), _lib._ptr(dx), _lib._ptr(dw13),
+                                                   _lib._ptr(derivatives), count, hidden, inter, _lib._ptr(d_gate_up), _lib._ptr(dx), _lib._ptr(dw13),
                                                    _lib._ptr(dw2), _lib._stream()))
     return dx, dw13, dw2
 
@@ -123,7 +123,7 @@ class _GatedMLP(torch.autograd.Function):
         with _lib.on_device_of(input):
             hidden = w2.shape[0]
             dx, dw13, dw2 = _backward(_rows(dy, hidden), _rows(input, hidden), _whole(w13), _whole(w2), h,
-                                      h if derivatives is None else derivatives, ctx.needs_input_grad[:3])
+                                      derivatives, ctx.needs_input_grad[:3])
         return None if dx is None else dx.view(input.shape), dw13, dw2, None, None
 
 
@@ -168,7 +168,8 @@ def gated_mlp_backward(dy, input, w13, w2, h, derivatives, *, needs: tuple = (Tr
     hidden, inter = _check(input, w13, w2)
     _check_tensor("dy", dy, input.device)
     _check_tensor("h", h, input.device)
-    _check_tensor("derivatives", derivatives, input.device)
+    if not isinstance(derivatives, torch.Tensor) or derivatives.dtype is not torch.float32 or derivatives.device != input.device:
+        raise TypeError("derivatives must be the float32 tensor that gated_mlp_forward returned")
     if dy.shape != input.shape:
         raise ValueError(f"dy must have the input's shape {tuple(input.shape)}, got {tuple(dy.shape)}")
     rows = input.numel() // hidden

@@ -322,12 +322,32 @@ FMOE_API int fmoe_i8gemm_dynamic_scaled_mm_pair(const void* x_bf16, int64_t rows
                                                 const int8_t* second_w, const float* second_scale, int32_t second_n,
                                                 void* second_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- low-rank adapters of many requests beside the dense W8A8 linear ---------------------------
+ * out[m] = (q[m] . w) * scale[m] * w_scale (+ bias) + scaling[a] * B[a] (A[a] x[m]), a = adapter_ids[m]; an id outside [0, count) selects no
+ * adapter.  scale[m] = amax * (1/127) in fp32 (1 for a row of zeros; fmoe_i8gemm_dynamic_scaled_mm divides, and may differ in the last
+ * bit), q = clamp(rint(x / scale), -128, 127).  Ids come in any order, int32 or int64.  A [count, rank, a_stride] and B [count, n, b_stride] are bf16,
+ * strides in elements, multiples of 8, what lies behind k and behind rank is zero in A and not read in B; A, B and scaling are finite (a row's
+ * result then depends on its own adapter alone).  The coefficients scaling * (A x) are rounded to bf16 where the result is
+ * bf16, and held as three bf16 terms where it is fp32.  workspace: fmoe_i8gemm_lora_workspace_bytes, 256-byte aligned.  Three launches. */
+typedef struct fmoe_lora_adapters {
+  const void* a;
+  const void* b;
+  const float* scaling; /* [count] */
+  int32_t count, rank;  /* rank: 1 .. 512 */
+  int32_t a_stride, b_stride;
+} fmoe_lora_adapters;
+FMOE_API size_t fmoe_i8gemm_lora_workspace_bytes(int64_t rows, int32_t k, int32_t rank, int32_t out_is_bf16);
+FMOE_API int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t k, const int8_t* w, const float* w_scale,
+                                                const float* bias, int32_t n, const fmoe_lora_adapters* adapters,
+                                                const void* adapter_ids, int32_t ids_are_64, void* out, int32_t out_is_bf16,
+                                                void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- gated feed-forward block, forward and backward (bf16, row-major) -------------------------
  * x [rows, H] with x_stride elements from a row to the next, w13 [2F, H] (gate rows, then up rows), w2 [H, F]:
  *   h = act(x Wg^T, x Wu^T) (bf16),  y = h W2^T.
  * activation: FMOE_ACTIVATION_SILU (swiglu_limit > 0: gate clamped from above and up to +-limit first), _GELU, _SWIGLUOAI.
- * h [rows, F] and y [rows, H] are written; by_gate_up [rows, 2F] (nullable) takes the partial derivatives of h by gate and by up for a
- * backward pass.  H and F are multiples of 8, every row starts on a 16-byte boundary.  Enqueues two launches. */
+ * h [rows, F] and y [rows, H] are written; by_gate_up fp32 [rows, 2F] (nullable) takes the partial derivatives of h by gate and by up
+ * for a backward pass.  H and F are multiples of 8, every row starts on a 16-byte boundary.  Enqueues two launches. */
 FMOE_API int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, const void* w2, int64_t rows, int32_t hidden,
                                     int32_t inter, int32_t activation, float swiglu_limit, void* h, void* by_gate_up, void* y,
                                     void* stream);

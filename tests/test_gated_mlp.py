@@ -34,13 +34,15 @@ def test_refusals(changes, error, text):
 
 def test_backward_refusals():
     x, w13, w2 = (torch.zeros(*shape, dtype=torch.bfloat16) for shape in ((3, 16), (48, 16), (16, 24)))
-    h, derivatives = torch.zeros(3, 24, dtype=torch.bfloat16), torch.zeros(3, 48, dtype=torch.bfloat16)
+    h, derivatives = torch.zeros(3, 24, dtype=torch.bfloat16), torch.zeros(3, 48)
     with pytest.raises(ValueError, match="input's shape"):
         moe.gated_mlp_backward(x[:2], x, w13, w2, h, derivatives)
     with pytest.raises(ValueError, match="what gated_mlp_forward returned"):
         moe.gated_mlp_backward(x, x, w13, w2, h[:, :16], derivatives)
     with pytest.raises(TypeError, match="dy must be torch.bfloat16"):
         moe.gated_mlp_backward(x.float(), x, w13, w2, h, derivatives)
+    with pytest.raises(TypeError, match="derivatives must be the float32"):
+        moe.gated_mlp_backward(x, x, w13, w2, h, derivatives.bfloat16())
     with pytest.raises(ValueError, match="needs"):
         moe.gated_mlp_backward(x, x, w13, w2, h, derivatives, needs=(True,))
     with pytest.raises(ValueError, match="CUDA"):

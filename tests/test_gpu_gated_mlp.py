@@ -1,8 +1,8 @@
 """The gated feed-forward block and its gradients against the formulas in 64 bits.
 
 Tolerances, element by element.  A rounding to bf16 is off by at most u = 2^-8 of the value.  Every result is a sum of products with S the sum of
-their magnitudes; a product carries n roundings of its factors (y and dw2: that of h, n = 1; dx and dw13: those of the partial derivative and of its product
-with dh, n = 2), so n u S.  A 32-bit sum of K terms is off by at most K 2^-24 of the sum of the magnitudes, the activation's functions by less than
+their magnitudes; a product carries n roundings of its factors (y and dw2: that of h; dx and dw13: that of dh times the partial
+derivative; n = 1), so n u S.  A 32-bit sum of K terms is off by at most K 2^-24 of the sum of the magnitudes, the activation's functions by less than
 2^-16 of their value; with `SMALL` = K 2^-24 + 2^-15 (K the longest sum; the second-order terms of the roundings, below 2^-15, are in it) that is SMALL S, and SMALL
 times the sum of the magnitudes inside dh.  gate and up are 32-bit sums too: their error enters h by its derivatives and the derivatives by theirs, which
 are below 4 (1 + |gate| + |up|), or whole where a value lies so near a limit that the error may carry it across.  The result's own rounding adds u of it."""
@@ -56,8 +56,8 @@ def formulas(x, w13, w2, dy, activation, limit):
     errors = {
         "y": (STEP + small) * (h.abs() @ w2.abs().T) + h_slack @ w2.abs().T,
         "dw2": (STEP + small) * (dy.abs().T @ h.abs()) + dy.abs().T @ h_slack,
-        "dx": (2 * STEP + small) * (d.abs() @ w13.abs()) + (small * d_size + d_slack) @ w13.abs(),
-        "dw13": (2 * STEP + small) * (d.abs().T @ x.abs()) + (small * d_size + d_slack).T @ x.abs(),
+        "dx": (STEP + small) * (d.abs() @ w13.abs()) + (small * d_size + d_slack) @ w13.abs(),
+        "dw13": (STEP + small) * (d.abs().T @ x.abs()) + (small * d_size + d_slack).T @ x.abs(),
     }
     return results, errors
 
