@@ -44,6 +44,10 @@ int check_device() {
   if (!fmoe_device_supported(device)) {
     return fail(FMOE_ERR_UNSUPPORTED_DEVICE, "device %d is not a compute capability 10.x GPU; this library has no other path", device);
   }
+  // A thread's first call may encode a tensor map before it has made any runtime call that binds the device's context to it (an
+  // autograd worker's): the driver then refuses the encoding.
+  error = cudaSetDevice(device);
+  if (error != cudaSuccess) return cuda_fail(error, "cudaSetDevice");
   checked_device = device;
   fmoe::threshold_sms = fmoe::sm_count_of_current_device();
   return FMOE_OK;
@@ -1045,6 +1049,11 @@ int check_gated_shape(const char* what, int64_t rows, int hidden, int inter) {
   }
   return FMOE_OK;
 }
+// Up to so many rows the products of the gated block go to the kernel that splits the K range (gated_small.cu).
+int64_t gated_small_rows() {
+  const char* text = getenv("FUSED_CPP_GATED_SMALL_ROWS");
+  return text != nullptr ? atoll(text) : 128;
+}
 bool vector_aligned(const void* pointer) { return reinterpret_cast<uintptr_t>(pointer) % 16 == 0; }
 int check_rows(const char* what, const char* name, const void* data, int64_t stride, int columns) {
   if (data == nullptr || !vector_aligned(data) || stride % 8 != 0 || stride < columns) {
@@ -1075,6 +1084,15 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
   if (!vector_aligned(by_gate_up)) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: by_gate_up must be 16-byte aligned", what);
   int* words = nullptr;
   cudaError_t error = fmoe::dense_status_words(&words);
+  if (error == cudaSuccess && rows <= gated_small_rows()) {
+    error = fmoe::launch_gated_projection_small(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
+                                                swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(by_gate_up), words, stream, false);
+    if (error == cudaSuccess) {
+      error = fmoe::launch_dense_small(static_cast<const uint16_t*>(h), rows, inter, static_cast<const uint16_t*>(w2), hidden, false, static_cast<uint16_t*>(y), words,
+                                       stream, true);
+    }
+    return error == cudaSuccess ? FMOE_OK : cuda_fail(error, what);
+  }
   if (error == cudaSuccess) {
     error = fmoe::launch_gated_projection(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
                                           swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(by_gate_up), words, stream, false);
@@ -1110,15 +1128,19 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
   int* words = nullptr;
   cudaError_t error = fmoe::dense_status_words(&words);
   bool chained = false;
+  const bool small = rows <= gated_small_rows();
   if (error == cudaSuccess && needs_gate_up) {
-    error = fmoe::launch_gated_backward(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const float*>(by_gate_up),
-                                        rows, hidden, inter, static_cast<uint16_t*>(d_gate_up), words, stream, chained);
+    auto launch = small ? fmoe::launch_gated_backward_small : fmoe::launch_gated_backward;
+    error = launch(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const float*>(by_gate_up), rows, hidden, inter,
+                   static_cast<uint16_t*>(d_gate_up), words, stream, chained);
     chained = true;
   }
   if (error == cudaSuccess && dx != nullptr) {
     const fmoe::DenseProductArgs product = {{static_cast<const uint16_t*>(d_gate_up), 2 * static_cast<int64_t>(inter)},
                                             {static_cast<const uint16_t*>(w13), hidden}, static_cast<uint16_t*>(dx), rows, hidden, 2 * static_cast<int64_t>(inter)};
-    error = fmoe::launch_dense_products(fmoe::DenseForm::kRowsByK, &product, 1, words, stream, chained);
+    error = small ? fmoe::launch_dense_small(static_cast<const uint16_t*>(d_gate_up), rows, 2 * inter, static_cast<const uint16_t*>(w13), hidden, true,
+                                             static_cast<uint16_t*>(dx), words, stream, chained)
+                  : fmoe::launch_dense_products(fmoe::DenseForm::kRowsByK, &product, 1, words, stream, chained);
     chained = true;
   }
   // Both weight gradients in one launch: apart, each ends with a wave of tiles that does not fill the chip.

@@ -1,0 +1,42 @@
+// The gated activations with their partial derivatives, for the epilogues of gated_gemm.cu and gated_small.cu.
+#pragma once
+
+#include "common.cuh"
+
+namespace fmoe {
+
+namespace {
+
+__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
+  const __nv_bfloat162 pair = __floats2bfloat162_rn(low, high);
+  return *reinterpret_cast<const uint32_t*>(&pair);
+}
+
+// h and its partial derivatives (common: gate * act'(gate) forms; NaN stays NaN through the limits).
+template <typename Tag>
+__device__ __forceinline__ void gated_with_derivatives(Tag, float gate, float up, float limit, float* h, float* by_gate, float* by_up) {
+  if constexpr (Tag::value == FMOE_ACT_GELU) {
+    const float cdf = normcdff(gate);  // 0.5 (1 + erf) would lose the values of the left tail
+    const float density = 0.39894228040143267794f * __expf(-0.5f * gate * gate);
+    *h = gate * cdf * up;
+    *by_gate = up * (cdf + gate * density);
+    *by_up = gate * cdf;
+  } else {
+    constexpr bool kOai = Tag::value == FMOE_ACT_SWIGLUOAI;
+    const float bound = kOai ? 7.0f : (limit > 0.0f ? limit : __int_as_float(0x7f800000));
+    constexpr float kAlpha = kOai ? 1.702f : 1.0f;
+    const bool gate_cut = gate > bound;
+    const bool up_cut = fabsf(up) > bound;
+    const float g = gate_cut ? bound : gate;
+    const float u = (up_cut ? copysignf(bound, up) : up) + (kOai ? 1.0f : 0.0f);
+    const float s = __fdividef(1.0f, 1.0f + __expf(-kAlpha * g));  // e^-g = inf divides to 0
+    const float gs = g * s;
+    *h = gs * u;
+    *by_gate = gate_cut ? 0.0f : u * s * (1.0f + kAlpha * g * (1.0f - s));
+    *by_up = up_cut ? 0.0f : gs;
+  }
+}
+
+}  // namespace
+
+}  // namespace fmoe

@@ -20,6 +20,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "gated.cuh"
 #include "kernels.h"
 #include "pair_ptx.cuh"
 #include "ptx.cuh"
@@ -99,11 +100,6 @@ __device__ __forceinline__ Tile tile_at(const Args& args, int64_t index) {
   return t;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float low, float high) {
-  const __nv_bfloat162 pair = __floats2bfloat162_rn(low, high);
-  return *reinterpret_cast<const uint32_t*>(&pair);
-}
-
 // Up to 32 neighbouring channels of a row as bf16: `columns` of them exist, a multiple of 8.
 __device__ __forceinline__ void store_channels(uint16_t* to, const float (&v)[32], int columns) {
 #pragma unroll
@@ -119,31 +115,6 @@ __device__ __forceinline__ void store_channels(float* to, const float (&v)[32], 
   for (int q = 0; q < 8; ++q) {
     if (4 * q >= columns) break;
     *reinterpret_cast<float4*>(to + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  }
-}
-
-// h and its partial derivatives (common: gate * act'(gate) forms; NaN stays NaN through the limits).
-template <typename Tag>
-__device__ __forceinline__ void gated_with_derivatives(Tag, float gate, float up, float limit, float* h, float* by_gate, float* by_up) {
-  if constexpr (Tag::value == FMOE_ACT_GELU) {
-    const float cdf = normcdff(gate);  // 0.5 (1 + erf) would lose the values of the left tail
-    const float density = 0.39894228040143267794f * __expf(-0.5f * gate * gate);
-    *h = gate * cdf * up;
-    *by_gate = up * (cdf + gate * density);
-    *by_up = gate * cdf;
-  } else {
-    constexpr bool kOai = Tag::value == FMOE_ACT_SWIGLUOAI;
-    const float bound = kOai ? 7.0f : (limit > 0.0f ? limit : __int_as_float(0x7f800000));
-    constexpr float kAlpha = kOai ? 1.702f : 1.0f;
-    const bool gate_cut = gate > bound;
-    const bool up_cut = fabsf(up) > bound;
-    const float g = gate_cut ? bound : gate;
-    const float u = (up_cut ? copysignf(bound, up) : up) + (kOai ? 1.0f : 0.0f);
-    const float s = __fdividef(1.0f, 1.0f + __expf(-kAlpha * g));  // e^-g = inf divides to 0
-    const float gs = g * s;
-    *h = gs * u;
-    *by_gate = gate_cut ? 0.0f : u * s * (1.0f + kAlpha * g * (1.0f - s));
-    *by_up = up_cut ? 0.0f : gs;
   }
 }
 

@@ -317,6 +317,14 @@ cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const u
                                   int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained);
 // The status block (kStatusWords ints, zero unless a bounded wait gave up) of the current device for launches without a workspace.
 cudaError_t dense_status_words(int** words);
+// The same products over few rows (gated_small.cu): clusters that split the K range.  out [rows, n] = tokens [rows, k] times weight [n, k], or
+// [k, n] with weight_by_k.
+cudaError_t launch_gated_projection_small(const uint16_t* x, int64_t x_stride, const uint16_t* w13, int64_t rows, int hidden, int inter, int activation,
+                                          float limit, uint16_t* h, float* by_gate_up, int* status, cudaStream_t stream, bool chained);
+cudaError_t launch_gated_backward_small(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* by_gate_up, int64_t rows, int hidden,
+                                        int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained);
+cudaError_t launch_dense_small(const uint16_t* tokens, int64_t rows, int k, const uint16_t* weight, int n, bool weight_by_k, uint16_t* out, int* status,
+                               cudaStream_t stream, bool chained);
 // One or two products of one form in a launch.
 enum class DenseForm { kRowsRows, kRowsByK, kByKByK };  // how A and B lie: [m, k] and [n, k]; [m, k] and [k, n]; [k, m] and [k, n]
 cudaError_t launch_dense_products(DenseForm form, const DenseProductArgs* products, int count, int* status, cudaStream_t stream, bool chained);
