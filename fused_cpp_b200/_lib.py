@@ -6,7 +6,6 @@ ABI.  Workspaces come from torch's caching allocator and are cached per (device,
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
@@ -239,6 +238,11 @@ def _ptr(tensor: torch.Tensor | None) -> int | None:
     return None if tensor is None else tensor.data_ptr()
 
 
+def _stream_of(index: int) -> int:
+    """Raw handle of the current stream of device `index`."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
@@ -358,12 +362,12 @@ def _require_cuda(name: str, tensor: torch.Tensor, dtype: torch.dtype) -> torch.
     return tensor if tensor.is_contiguous() else tensor.contiguous()
 
 
-_NO_GUARD = contextlib.nullcontext()
-
-
-def on_device_of(tensor: torch.Tensor):
-    """Context in which the device of `tensor` is the current one, whose current stream `_stream` then gives."""
-    return _NO_GUARD if tensor.device.index == torch.cuda.current_device() else torch.cuda.device(tensor.device)
+def on_device(index: int, call, *args):
+    """call(*args) with device `index` as the current one, whose current stream and set-up the library then uses."""
+    if torch._C._cuda_getDevice() == index:
+        return call(*args)
+    with torch.cuda.device(index):
+        return call(*args)
 
 
 def dense_status() -> tuple[int, int]:

@@ -156,37 +156,36 @@ def dynamic_scaled_mm_lora(x: torch.Tensor, packed: PreparedI8GEMMWeight, adapte
     The low-rank product takes x as it is, not its quantised rows.  Its coefficients scaling * (A x) are rounded to bf16 for a bf16 result and kept
     to 24 bits for a float32 one.  The row scale is amax * (1/127) in 32 bits, as torch divides by a number, where dynamic_scaled_mm rounds the
     quotient: the two may differ in the scale's last bit, and with it in the integer of a value that is half of its row's largest."""
-    _require_backend()
-    name = "i8gemm.dynamic_scaled_mm_lora"
     if not isinstance(packed, PreparedI8GEMMWeight):
-        raise TypeError(f"{name}: packed must come from i8gemm.prepare")
+        raise TypeError("i8gemm.dynamic_scaled_mm_lora: packed must come from i8gemm.prepare")
     if not isinstance(adapters, lora.PreparedAdapters):
-        raise TypeError(f"{name}: adapters must come from lora.prepare_adapters")
-    if x.dtype != torch.bfloat16 or x.device.type != "cuda":
-        raise TypeError(f"{name}: x must be a CUDA bfloat16 tensor")
-    if x.shape[-1] != packed.k:
-        raise ValueError(f"{name}: x last dim must be K={packed.k}, got {x.shape[-1]}")
-    if adapters.k != packed.k or adapters.n != packed.n:
-        raise ValueError(f"{name}: adapters of a [{adapters.n}, {adapters.k}] projection beside a weight of [{packed.n}, {packed.k}]")
-    if out_dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"{name}: out_dtype must be float32/bfloat16, got {out_dtype}")
-    if adapter_ids.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"{name}: adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
-    if adapter_ids.shape != x.shape[:-1]:
-        raise ValueError(f"{name}: adapter_ids must be {tuple(x.shape[:-1])}, one per row, got {tuple(adapter_ids.shape)}")
-    if bias is not None and (bias.dim() != 1 or int(bias.shape[0]) != packed.n):
-        raise ValueError(f"{name}: bias must be shape [{packed.n}]")
+        raise TypeError("i8gemm.dynamic_scaled_mm_lora: adapters must come from lora.prepare_adapters")
+    if x.dtype is not torch.bfloat16 or not x.is_cuda:
+        raise TypeError("i8gemm.dynamic_scaled_mm_lora: x must be a CUDA bfloat16 tensor")
+    k, n = packed.k, packed.n
+    if x.shape[-1] != k:
+        raise ValueError(f"i8gemm.dynamic_scaled_mm_lora: x last dim must be K={k}, got {x.shape[-1]}")
+    if adapters.k != k or adapters.n != n:
+        raise ValueError(f"i8gemm.dynamic_scaled_mm_lora: adapters of a [{adapters.n}, {adapters.k}] projection beside a weight of [{n}, {k}]")
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+        raise ValueError(f"i8gemm.dynamic_scaled_mm_lora: out_dtype must be float32/bfloat16, got {out_dtype}")
+    if adapter_ids.dtype is not torch.int64 and adapter_ids.dtype is not torch.int32:
+        raise TypeError(f"i8gemm.dynamic_scaled_mm_lora: adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
+    shape = x.shape[:-1]
+    if adapter_ids.shape != shape:
+        raise ValueError(f"i8gemm.dynamic_scaled_mm_lora: adapter_ids must be {tuple(shape)}, one per row, got {tuple(adapter_ids.shape)}")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n):
+        raise ValueError(f"i8gemm.dynamic_scaled_mm_lora: bias must be shape [{n}]")
+    index = x.get_device()
     for what, tensor in (("weight", packed.packed_weight), ("adapters", adapters.a), ("adapter_ids", adapter_ids)):
-        if tensor.device != x.device:
-            raise ValueError(f"{name}: {what} must lie on the input's device")
-    if int(nthreads) < 0:
+        if tensor.get_device() != index:
+            raise ValueError(f"i8gemm.dynamic_scaled_mm_lora: {what} must lie on the input's device")
+    if nthreads < 0:
         raise ValueError("nthreads must be non-negative; zero selects the backend default")
-    out = torch.empty((*x.shape[:-1], packed.n), dtype=out_dtype, device=x.device)
+    out = x.new_empty((*shape, n), dtype=out_dtype)
     if x.numel() == 0:
         return out
-    with _lib.on_device_of(x):
-        bias_f32 = None if bias is None else bias.to(device=x.device, dtype=torch.float32).contiguous()
-        lora.projection(x.contiguous().view(-1, packed.k), packed, adapters, adapter_ids.contiguous(), bias_f32, out)
+    _lib.on_device(index, lora.projection, index, x, packed, adapters, adapter_ids, bias, out)
     return out
 
 

@@ -9,7 +9,6 @@ Row m of a batch gets scaling[a] * B[a] (A[a] x[m]) added to its projection, a =
 """
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass, field
 from typing import Sequence
 
@@ -111,18 +110,23 @@ def set_adapter(adapters: PreparedAdapters, index: int, a: torch.Tensor, b: torc
         adapters.scaling[index] = float(scaling)
 
 
-def projection(x: torch.Tensor, packed, adapters: PreparedAdapters, adapter_ids: torch.Tensor, bias: torch.Tensor | None,
+def projection(index: int, x: torch.Tensor, packed, adapters: PreparedAdapters, adapter_ids: torch.Tensor, bias: torch.Tensor | None,
                out: torch.Tensor) -> None:
-    """out [M, N] of bf16 rows x [M, K], checked by the caller; the workspace is the call's own, so that calls on several streams and
-    captured ones do not share it."""
-    rows, k = x.shape
+    """out [..., N] of bf16 rows x [..., K] on CUDA device `index`, checked by the caller; the workspace is the call's own, so that calls on
+    several streams and captured ones do not share it."""
+    x = x if x.is_contiguous() else x.contiguous()
+    adapter_ids = adapter_ids if adapter_ids.is_contiguous() else adapter_ids.contiguous()
+    if bias is not None:
+        bias = _lib.as_dtype(bias.to(x.device), torch.float32)
+    rows, k = x.numel() // packed.k, packed.k
     lib = _lib.load()
-    out_is_bf16 = 1 if out.dtype == torch.bfloat16 else 0
+    out_is_bf16 = 1 if out.dtype is torch.bfloat16 else 0
     nbytes = lib.fmoe_i8gemm_lora_workspace_bytes(rows, k, adapters.rank, out_is_bf16)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    workspace = x.new_empty(nbytes, dtype=torch.uint8)
     _lib.check(lib.fmoe_i8gemm_dynamic_scaled_mm_lora(
-        x.data_ptr(), rows, k, packed.packed_weight.data_ptr(), packed.weight_scale.data_ptr(), _lib._ptr(bias), packed.n, ctypes.byref(adapters.native),
-        adapter_ids.data_ptr(), 1 if adapter_ids.dtype == torch.int64 else 0, out.data_ptr(), out_is_bf16, workspace.data_ptr(), nbytes, _lib._stream()))
+        x.data_ptr(), rows, k, packed.packed_weight.data_ptr(), packed.weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), packed.n,
+        adapters.native, adapter_ids.data_ptr(), 1 if adapter_ids.dtype is torch.int64 else 0, out.data_ptr(), out_is_bf16, workspace.data_ptr(), nbytes,
+        _lib._stream_of(index)))
 
 
 __all__ = ["MAX_RANK", "PreparedAdapters", "prepare_adapters", "set_adapter"]

@@ -19,6 +19,7 @@ import torch
 from .. import _lib
 from .bf16_tiled import _native_activation_name
 
+_BF16 = torch.bfloat16
 _ACTIVATIONS = {"silu": (_lib.ACTIVATION_SILU, 0.0), "silu_clamp10": (_lib.ACTIVATION_SILU, 10.0), "gelu": (_lib.ACTIVATION_GELU, 0.0),
                 "swigluoai": (_lib.ACTIVATION_SWIGLUOAI, 0.0)}
 
@@ -30,38 +31,42 @@ def _activation(activation: Any, swiglu_limit: float | None) -> tuple[int, float
     return _ACTIVATIONS[name]
 
 
-def _check_tensor(name: str, tensor: Any, device: torch.device | None) -> None:
+def _check_tensor(name: str, tensor: Any, index: int | None) -> None:
     if not isinstance(tensor, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if tensor.dtype is not torch.bfloat16:
+    if tensor.dtype is not _BF16:
         raise TypeError(f"{name} must be torch.bfloat16, got {tensor.dtype}")
-    if device is not None and tensor.device != device:
+    if index is not None and tensor.get_device() != index:
         raise ValueError(f"{name} must lie on the input's device")
 
 
-def _check(input, w13, w2) -> tuple[int, int]:
+def _check(input, w13, w2) -> tuple[int, int, int]:
+    """(H, F, the CUDA device's index or -1) of tensors that go together."""
     _check_tensor("input", input, None)
-    _check_tensor("w13", w13, input.device)
-    _check_tensor("w2", w2, input.device)
+    index = input.get_device()
+    _check_tensor("w13", w13, index)
+    _check_tensor("w2", w2, index)
     if w13.dim() != 2 or w2.dim() != 2:
         raise ValueError("gated_mlp weights must be [2F, H] and [H, F]")
-    hidden, inter = int(w2.shape[0]), int(w2.shape[1])
-    if tuple(w13.shape) != (2 * inter, hidden):
+    hidden, inter = w2.shape
+    if w13.shape != (2 * inter, hidden):
         raise ValueError(f"w13 must be [2F, H] = [{2 * inter}, {hidden}] beside w2 [H, F], got {tuple(w13.shape)}")
     if input.dim() < 1 or input.shape[-1] != hidden:
         raise ValueError(f"input must be [..., H={hidden}], got {tuple(input.shape)}")
     if hidden % 8 or inter % 8 or not hidden or not inter:
         raise ValueError(f"H and F must be positive multiples of 8 (H={hidden}, F={inter})")
-    return hidden, inter
+    return hidden, inter, index
 
 
-def _require_cuda(tensor: torch.Tensor) -> None:
-    if not tensor.is_cuda:
+def _require_cuda(index: int) -> None:
+    if index < 0:
         raise ValueError("gated_mlp takes CUDA tensors (this build has no CPU path)")
 
 
 def _rows(tensor: torch.Tensor, columns: int) -> torch.Tensor:
     """[..., columns] as rows that the kernels can read where they are: unit column stride, every row on a 16-byte boundary."""
+    if tensor.dim() == 2 and tensor.is_contiguous() and tensor.data_ptr() % 16 == 0:
+        return tensor
     rows = tensor.reshape(-1, columns)
     if rows.stride(1) == 1 and rows.data_ptr() % 16 == 0 and (rows.shape[0] == 1 or (rows.stride(0) % 8 == 0 and rows.stride(0) >= columns)):
         return rows
@@ -80,51 +85,62 @@ def _whole(tensor: torch.Tensor) -> torch.Tensor:
     return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()
 
 
-def _forward(rows, w13, w2, code: int, limit: float, keep: bool, y):
+def _forward(index: int, rows, w13, w2, code: int, limit: float, keep: bool, y):
     count, hidden = rows.shape
     inter = w2.shape[1]
-    h = torch.empty((count, inter), dtype=torch.bfloat16, device=rows.device)
-    derivatives = torch.empty((count, 2 * inter), dtype=torch.float32, device=rows.device) if keep else None
+    h = rows.new_empty((count, inter))
+    derivatives = rows.new_empty((count, 2 * inter), dtype=torch.float32) if keep else None
     _lib.check(_lib.load().fmoe_gated_mlp_forward(rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), count, hidden, inter, code, limit,
-                                                  h.data_ptr(), _lib._ptr(derivatives), y.data_ptr(), _lib._stream()))
+                                                  h.data_ptr(), derivatives.data_ptr() if keep else None, y.data_ptr(), _lib._stream_of(index)))
     return h, derivatives
 
 
-def _backward(dy, rows, w13, w2, h, derivatives, needs):
+def _backward(index: int, dy, rows, w13, w2, h, derivatives, need_x: bool, need_w13: bool, need_w2: bool):
     count, hidden = rows.shape
     inter = w2.shape[1]
     if count == 0:
-        return tuple(torch.zeros_like(t, memory_format=torch.contiguous_format) if need else None for need, t in zip(needs, (rows, w13, w2)))
-    dx = torch.empty((count, hidden), dtype=torch.bfloat16, device=rows.device) if needs[0] else None
-    dw13 = torch.empty((2 * inter, hidden), dtype=torch.bfloat16, device=rows.device) if needs[1] else None
-    dw2 = torch.empty((hidden, inter), dtype=torch.bfloat16, device=rows.device) if needs[2] else None
-    d_gate_up = torch.empty((count, 2 * inter), dtype=torch.bfloat16, device=rows.device) if needs[0] or needs[1] else None
+        return (rows.new_zeros((0, hidden)) if need_x else None, w13.new_zeros(w13.shape) if need_w13 else None,
+                w2.new_zeros(w2.shape) if need_w2 else None)
+    dx = rows.new_empty((count, hidden)) if need_x else None
+    dw13 = rows.new_empty((2 * inter, hidden)) if need_w13 else None
+    dw2 = rows.new_empty((hidden, inter)) if need_w2 else None
+    scratch = rows.new_empty((count, 2 * inter)) if need_x or need_w13 else None
+    pointer = _lib._ptr
     _lib.check(_lib.load().fmoe_gated_mlp_backward(dy.data_ptr(), _stride(dy), rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), h.data_ptr(),
-                                                   _lib._ptr(derivatives), count, hidden, inter, _lib._ptr(d_gate_up), _lib._ptr(dx), _lib._ptr(dw13),
-                                                   _lib._ptr(dw2), _lib._stream()))
+                                                   pointer(derivatives), count, hidden, inter, pointer(scratch), pointer(dx), pointer(dw13),
+                                                   pointer(dw2), _lib._stream_of(index)))
     return dx, dw13, dw2
 
 
 class _GatedMLP(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, input, w13, w2, code, limit):
-        with _lib.on_device_of(input):
-            rows, w13_rows, w2_rows = _rows(input, w2.shape[0]), _whole(w13), _whole(w2)
-            y = torch.empty(input.shape, dtype=torch.bfloat16, device=input.device)
-            # dW2 needs h alone, dx and dW13 the derivatives.
-            h, derivatives = _forward(rows, w13_rows, w2_rows, code, limit, ctx.needs_input_grad[0] or ctx.needs_input_grad[1], y)
+    def forward(ctx, input, w13, w2, code, limit, index):
+        return _lib.on_device(index, _GatedMLP._forward, ctx, input, w13, w2, code, limit, index)
+
+    @staticmethod
+    def _forward(ctx, input, w13, w2, code, limit, index):
+        rows = _rows(input, w2.shape[0])
+        y = rows.new_empty(input.shape)
+        need_x, need_w13 = ctx.needs_input_grad[:2]
+        # dW2 needs h alone, dx and dW13 the derivatives.
+        h, derivatives = _forward(index, rows, _whole(w13), _whole(w2), code, limit, need_x or need_w13, y)
         ctx.save_for_backward(input, w13, w2, h, derivatives)
+        ctx.index = index
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_mlp is differentiable once: its backward pass has no gradient (create_graph)")
+        return _lib.on_device(ctx.index, _GatedMLP._backward, ctx, dy)
+
+    @staticmethod
+    def _backward(ctx, dy):
         input, w13, w2, h, derivatives = ctx.saved_tensors
-        with _lib.on_device_of(input):
-            hidden = w2.shape[0]
-            dx, dw13, dw2 = _backward(_rows(dy, hidden), _rows(input, hidden), _whole(w13), _whole(w2), h,
-                                      derivatives, ctx.needs_input_grad[:3])
-        return None if dx is None else dx.view(input.shape), dw13, dw2, None, None
+        hidden = w2.shape[0]
+        needs = ctx.needs_input_grad
+        dx, dw13, dw2 = _backward(ctx.index, _rows(dy, hidden), _rows(input, hidden), _whole(w13), _whole(w2), h, derivatives, needs[0], needs[1], needs[2])
+        return dx if dx is None or input.dim() == 2 else dx.view(input.shape), dw13, dw2, None, None, None
 
 
 def gated_mlp(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float | None = None, out=None):
@@ -132,52 +148,62 @@ def gated_mlp(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float |
 
     activation: "silu", "gelu" or "swigluoai"; swiglu_limit: None, 0 or 10.0 (with "silu").  H and F are multiples of 8.  With `out`
     (contiguous, no gradients asked for) the result is written there and `out` returned."""
-    _check(input, w13, w2)
+    _, _, index = _check(input, w13, w2)
     code, limit = _activation(activation, swiglu_limit)
-    _require_cuda(input)
-    if torch.is_grad_enabled() and (input.requires_grad or w13.requires_grad or w2.requires_grad):
+    _require_cuda(index)
+    if (input.requires_grad or w13.requires_grad or w2.requires_grad) and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out cannot be given where gradients are asked for")
-        return _GatedMLP.apply(input, w13, w2, code, limit)
+        return _GatedMLP.apply(input, w13, w2, code, limit, index)
+    return _lib.on_device(index, _serve, index, input, w13, w2, code, limit, out)
+
+
+def _serve(index: int, input, w13, w2, code: int, limit: float, out):
+    rows = _rows(input, w2.shape[0])
     if out is None:
-        out = torch.empty(input.shape, dtype=torch.bfloat16, device=input.device)
-        y = out
+        y = out = rows.new_empty(input.shape)
     else:
-        _check_tensor("out", out, input.device)
+        _check_tensor("out", out, index)
         if out.shape != input.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and match the input shape")
-        y = out if out.data_ptr() % 16 == 0 else torch.empty(out.shape, dtype=out.dtype, device=out.device)
-    with _lib.on_device_of(input):
-        _forward(_rows(input, w2.shape[0]), _whole(w13), _whole(w2), code, limit, False, y)
+        y = out if out.data_ptr() % 16 == 0 else rows.new_empty(input.shape)
+    _forward(index, rows, _whole(w13), _whole(w2), code, limit, False, y)
     return out if y is out else out.copy_(y)
 
 
 def gated_mlp_forward(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float | None = None):
     """The forward pass without a tape: (y, h, derivatives), the last two for `gated_mlp_backward`."""
-    _check(input, w13, w2)
+    hidden, _, index = _check(input, w13, w2)
     code, limit = _activation(activation, swiglu_limit)
-    _require_cuda(input)
-    with torch.no_grad(), _lib.on_device_of(input):
-        y = torch.empty(input.shape, dtype=torch.bfloat16, device=input.device)
-        h, derivatives = _forward(_rows(input, w2.shape[0]), _whole(w13), _whole(w2), code, limit, True, y)
-    return y, h, derivatives
+    _require_cuda(index)
+
+    def call():
+        rows = _rows(input.detach(), hidden)
+        y = rows.new_empty(input.shape)
+        return (y, *_forward(index, rows, _whole(w13.detach()), _whole(w2.detach()), code, limit, True, y))
+
+    return _lib.on_device(index, call)
 
 
 def gated_mlp_backward(dy, input, w13, w2, h, derivatives, *, needs: tuple = (True, True, True)):
     """(dx, dw13, dw2) from dy [..., H] and what `gated_mlp_forward` returned; None where `needs` says so."""
-    hidden, inter = _check(input, w13, w2)
-    _check_tensor("dy", dy, input.device)
-    _check_tensor("h", h, input.device)
-    if not isinstance(derivatives, torch.Tensor) or derivatives.dtype is not torch.float32 or derivatives.device != input.device:
+    hidden, inter, index = _check(input, w13, w2)
+    _check_tensor("dy", dy, index)
+    _check_tensor("h", h, index)
+    if not isinstance(derivatives, torch.Tensor) or derivatives.dtype is not torch.float32 or derivatives.get_device() != index:
         raise TypeError("derivatives must be the float32 tensor that gated_mlp_forward returned")
     if dy.shape != input.shape:
         raise ValueError(f"dy must have the input's shape {tuple(input.shape)}, got {tuple(dy.shape)}")
     rows = input.numel() // hidden
-    if tuple(h.shape) != (rows, inter) or tuple(derivatives.shape) != (rows, 2 * inter) or not h.is_contiguous() or not derivatives.is_contiguous():
+    if h.shape != (rows, inter) or derivatives.shape != (rows, 2 * inter) or not h.is_contiguous() or not derivatives.is_contiguous():
         raise ValueError("h and derivatives must be what gated_mlp_forward returned for this input")
     if len(needs) != 3:
         raise ValueError("needs must say for dx, dw13 and dw2 whether they are wanted")
-    _require_cuda(input)
-    with torch.no_grad(), _lib.on_device_of(input):
-        dx, dw13, dw2 = _backward(_rows(dy, hidden), _rows(input, hidden), _whole(w13), _whole(w2), _whole(h), _whole(derivatives), tuple(bool(n) for n in needs))
-    return None if dx is None else dx.view(input.shape), dw13, dw2
+    _require_cuda(index)
+
+    def call():
+        dx, dw13, dw2 = _backward(index, _rows(dy.detach(), hidden), _rows(input.detach(), hidden), _whole(w13.detach()), _whole(w2.detach()),
+                                  _whole(h.detach()), _whole(derivatives), *(bool(need) for need in needs))
+        return None if dx is None else dx.view(input.shape), dw13, dw2
+
+    return _lib.on_device(index, call)

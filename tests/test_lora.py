@@ -57,8 +57,7 @@ def test_set_adapter_refusals(index, a, b, scaling, error, text):
         lora.set_adapter(_holder(), index, a, b, scaling)
 
 
-def test_projection_refusals(monkeypatch):
-    monkeypatch.setattr(i8gemm, "_require_backend", lambda: None)
+def test_projection_refusals():
     packed = i8gemm.PreparedI8GEMMWeight(torch.zeros(24, 16, dtype=torch.int8), torch.ones(24), 16, 24, 16, 24, "x")
     ids = torch.zeros(3, dtype=torch.int64)
     with pytest.raises(TypeError, match="CUDA bfloat16"):
