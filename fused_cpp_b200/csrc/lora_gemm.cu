@@ -14,6 +14,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "gated.cuh"
 #include "kernels.h"
 #include "lora.h"
 #include "ptx.cuh"
@@ -25,12 +26,13 @@ namespace {
 constexpr int kBlockM = 128;        // output channels per CTA (TMEM lanes)
 constexpr int kBlockKBytes = 128;   // bytes of K per pipeline stage = one 128-byte swizzle row
 constexpr int kUmmaKBytes = 32;     // bytes of K per tcgen05.mma, of either kind
-constexpr int kThreads = 224;       // warp 0: TMA, warp 1: tensor memory and MMA, warps 2..5: epilogue, warp 6: masked coefficients
+constexpr int kThreads = 192;       // warp 0: TMA, warp 1: tensor memory and MMA, warps 2..5: masked coefficients, then epilogue
 constexpr int kWeightBytes = kBlockM * kBlockKBytes;
 constexpr int kMaxStages = 10;
 constexpr int kMaxParts = 8;
 constexpr int kMinPartBlocks = 2;
 constexpr int kTileRows = 128;
+constexpr int kWriters = 4;         // warps that write masked coefficients
 
 template <int kRowTile, bool kDeep>
 struct LoraConfig {
@@ -40,7 +42,8 @@ struct LoraConfig {
   static constexpr int kStages = kBudget / kStageBytes < kMaxStages ? kBudget / kStageBytes : kMaxStages;
   static constexpr int kTmemColumns = 2 * kRowTile;  // the int32 and the fp32 accumulator
   static constexpr size_t kSmemBytes = 1024 /*alignment slack*/ + static_cast<size_t>(kStages) * kStageBytes + 4096 /*control block*/;
-  static_assert(kStages * kStageBytes >= kRowTile * kBlockM * 4, "the accumulator exchange reuses the stages");
+  // With two parts and more a CTA finishes at most half of the rows (in whole sixteens).
+  static_assert(kStages * kStageBytes >= (kRowTile + (kRowTile > 16 ? kRowTile / 2 : 16)) * kBlockM * 4, "the accumulator exchange and the adapters' sums reuse the stages");
 };
 
 struct LoraControl {
@@ -49,6 +52,7 @@ struct LoraControl {
   uint64_t vacant[kMaxStages];        // the producer found the stage empty and leaves its token tile to the coefficients
   uint64_t coefficients[kMaxStages];  // the masked coefficients of the stage are written
   uint64_t acc_full;
+  uint64_t listed;  // the list of adapters is there
   uint32_t tmem_base;
   volatile int abort_flag;
   int slots;
@@ -70,6 +74,14 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ int4 load_cluster_int4(uint32_t smem_address, int cta) {
+  uint32_t remote;
+  int4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_address), "r"(cta));
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -80,6 +92,14 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
 
 __device__ __forceinline__ float finish(int acc, float row_scale, float channel_scale, float bias, float delta) {
   return __fadd_rn(__fadd_rn(dequantize(acc, row_scale, channel_scale, FMOE_NUMERICS_TORCHREF), bias), delta);
+}
+
+__device__ __forceinline__ void store_value(const LoraGemmArgs& g, int64_t index, float value) {
+  if (g.out_bf16) {
+    static_cast<uint16_t*>(g.out)[index] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
+  } else {
+    static_cast<float*>(g.out)[index] = value;
+  }
 }
 
 template <int kRowTile, bool kDeep>
@@ -112,9 +132,11 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
       ptx::mbar_init(&ctl->full[s], 1);
       ptx::mbar_init(&ctl->empty[s], 1);
       ptx::mbar_init(&ctl->vacant[s], 1);
-      ptx::mbar_init(&ctl->coefficients[s], 1);
+      ptx::mbar_init(&ctl->coefficients[s], kWriters);
     }
     ptx::mbar_init(&ctl->acc_full, 1);
+    ptx::mbar_init(&ctl->listed, 1);
+    ctl->slots = 0;
     ctl->abort_flag = 0;
     ptx::fence_barrier_init();
   }
@@ -122,7 +144,12 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
     ptx::tmem_alloc(&ctl->tmem_base, Cfg::kTmemColumns);
     ptx::tmem_relinquish();
   }
-  if (warp == 6) {
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  volatile int* abort_flag = &ctl->abort_flag;
+  if (warp == 2) {
     // The adapters of the own rows, each once, in the order of their first rows.
     int slots = 0;
     for (int base = 0; base < own; base += 32) {
@@ -140,30 +167,30 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
       slots += __popc(firsts);
       __syncwarp();
     }
-    if (lane == 0) ctl->slots = slots;
+    if (lane == 0) {
+      ctl->slots = slots;
+      ptx::mbar_arrive(&ctl->listed);
+    }
+  } else if (warp == 0) {
+    // Weights of the first stages: they depend neither on the ids nor on the kernels that may still be running.
+    if (ptx::elect_one()) {
+      for (int i = 0; i < (count < Cfg::kStages ? count : Cfg::kStages); ++i) {
+        ptx::mbar_arrive_expect_tx(&ctl->full[i], Cfg::kStageBytes);
+        ptx::tma_load_2d(smem + static_cast<size_t>(i) * Cfg::kStageBytes, &weight_map, &ctl->full[i], (kb_begin + i) * kBlockKBytes, n0);
+      }
+    }
+    __syncwarp();
   }
-  ptx::tcgen05_fence_before();
-  __syncthreads();
-  ptx::tcgen05_fence_after();
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
-  volatile int* abort_flag = &ctl->abort_flag;
+  ptx::mbar_wait(&ctl->listed, 0, abort_flag, status, 56);
   const int slots = __shfl_sync(0xffffffffu, ctl->slots, 0);
-  // K blocks of the adapters' product: every adapter's rank blocks, the planes of each.
-  const int per_slot = args.rank_blocks * args.g.planes;
-  const int extra = slots * per_slot;
+  // K blocks of the adapters' product: for every plane of every 64 ranks, the adapters one after the other.
+  const int extra = slots * args.rank_blocks * args.g.planes;
   const int all = count + extra;
 
   if (warp == 0) {
     // ---------------- TMA producer (the whole warp walks the loops, one elected lane issues) ----------------
     const bool issuer = ptx::elect_one();
     const int ahead = count < Cfg::kStages ? count : Cfg::kStages;
-    // Weights of the first stages: they do not depend on the kernels that may still be running.
-    for (int i = 0; i < ahead; ++i) {
-      if (issuer) {
-        ptx::mbar_arrive_expect_tx(&ctl->full[i], Cfg::kStageBytes);
-        ptx::tma_load_2d(smem + static_cast<size_t>(i) * Cfg::kStageBytes, &weight_map, &ctl->full[i], (kb_begin + i) * kBlockKBytes, n0);
-      }
-    }
     ptx::grid_dependency_wait();
     for (int i = 0; i < ahead; ++i) {
       if (issuer) {
@@ -183,10 +210,10 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
           ptx::tma_load_2d(stage_base + kWeightBytes, &token_map, &ctl->full[stage], (kb_begin + i) * kBlockKBytes, static_cast<int>(row0));
         } else {
           const int u = i - count;
-          const int rank_block = u % per_slot / args.g.planes;
+          const int rank_block = u / slots / args.g.planes;
           ptx::mbar_arrive(&ctl->vacant[stage]);
           ptx::mbar_arrive_expect_tx(&ctl->full[stage], kWeightBytes);
-          tma_load_3d(stage_base, &b_map, &ctl->full[stage], rank_block * kLoraRankBlock, n0, ctl->slot_adapter[u / per_slot]);
+          tma_load_3d(stage_base, &b_map, &ctl->full[stage], rank_block * kLoraRankBlock, n0, ctl->slot_adapter[u % slots]);
         }
       }
       if (++stage == Cfg::kStages) {
@@ -232,7 +259,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
                                ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + ks * kUmmaKBytes), idesc, (i > 0 || ks > 0) ? 1u : 0u);
           }
         } else {
-          const int rank_block = (i - count) % per_slot / args.g.planes;
+          const int rank_block = (i - count) / slots / args.g.planes;
           const int steps = (min(kLoraRankBlock, args.g.adapters.rank - rank_block * kLoraRankBlock) + 15) >> 4;
           for (int ks = 0; ks < steps; ++ks) {
             ptx::umma_ss<false>(tmem_base + kRowTile, ptx::make_smem_desc_sw128(stage_addr + ks * kUmmaKBytes),
@@ -247,36 +274,51 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
       }
     }
     if (issuer) ptx::tcgen05_commit(&ctl->acc_full);
-  } else if (warp == 6) {
-    // ---------------- masked coefficients ----------------
+  } else if (extra > 0) {
+    // ---------------- masked coefficients (warps 2..5) ----------------
+    // A thread holds up to eight 16-byte pieces of the own rows' coefficients, and for each adapter in turn writes those of its rows and zeros
+    // for the others.  (Loaded again for every adapter, by one warp: 201 rows of 1536 -> 24576 with four adapters of rank 64 97.6 us.)
     ptx::grid_dependency_wait();
+    const int thread = static_cast<int>(threadIdx.x) - 64;
     const int rank_padded = lora_rank_padded(args.g.adapters.rank);
     const int own16 = (own + 15) & ~15;
     const uint16_t* const t_rows = args.g.t + (row0 + own_first) * rank_padded;
+    constexpr int kPieces = kRowTile * 8 / 128;  // of a thread
     int stage = count % Cfg::kStages;
     uint32_t used = 0;  // stages, one bit each, whose vacant barrier is in its odd phase
-    for (int u = 0; u < extra; ++u) {
-      const int adapter = ctl->slot_adapter[u / per_slot];
-      const int inside = u % per_slot;
-      const int rank0 = inside / args.g.planes * kLoraRankBlock;
-      const int plane = inside % args.g.planes;
-      const int pieces = 2 * ((min(kLoraRankBlock, args.g.adapters.rank - rank0) + 15) >> 4);  // of 16 bytes in a row: a power of two but for 6
+    for (int outer = 0; outer < args.rank_blocks * args.g.planes; ++outer) {
+      const int rank0 = outer / args.g.planes * kLoraRankBlock;
+      const int plane = outer % args.g.planes;
+      const int pieces = 2 * ((min(kLoraRankBlock, args.g.adapters.rank - rank0) + 15) >> 4);  // of 16 bytes in a row
       const uint16_t* const from = t_rows + static_cast<int64_t>(plane) * args.g.rows * rank_padded + rank0;
-      // (Not the empty barrier itself: this warp does not see its earlier phases, and would take one for another.)
-      ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 54);
-      used ^= 1u << stage;
-      uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + kWeightBytes;
-      for (int e = lane; e < own16 * pieces; e += 32) {
+      uint4 value[kPieces];
+      int id[kPieces];
+      uint32_t offset[kPieces];
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        const int e = thread + 128 * p;
         const int row = e / pieces, piece = e - row * pieces;
-        uint4 value = make_uint4(0, 0, 0, 0);
-        if (row < own && ctl->id[row] == adapter) value = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(row) * rank_padded) + piece);
+        value[p] = make_uint4(0, 0, 0, 0);
+        id[p] = row < own ? ctl->id[row] : -1;
         // The 128-byte swizzle that the operand tiles have: the 16-byte piece's number is xor-ed with the row's in its group of eight.
-        *reinterpret_cast<uint4*>(to + row * kBlockKBytes + ((piece ^ (row & 7)) << 4)) = value;
+        offset[p] = row < own16 ? static_cast<uint32_t>(row * kBlockKBytes + ((piece ^ (row & 7)) << 4)) : ~0u;
+        if (id[p] >= 0) value[p] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(row) * rank_padded) + piece);
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&ctl->coefficients[stage]);
-      if (++stage == Cfg::kStages) stage = 0;
+      for (int slot = 0; slot < slots; ++slot) {
+        const int adapter = ctl->slot_adapter[slot];
+        // (Not the empty barrier itself: these warps do not see its earlier phases, and would take one for another.)
+        ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 54);
+        used ^= 1u << stage;
+        uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + kWeightBytes;
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          if (offset[p] != ~0u) *reinterpret_cast<uint4*>(to + offset[p]) = id[p] == adapter ? value[p] : make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&ctl->coefficients[stage]);
+        if (++stage == Cfg::kStages) stage = 0;
+      }
     }
   }
 
@@ -284,9 +326,10 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
   const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id % 4
   const int channel = quarter * 32 + lane;
   const bool channel_ok = n0 + channel < n;
-  const bool epilogue = warp >= 2 && warp < 6;
+  const bool epilogue = warp >= 2;
   float channel_scale = 1.0f, bias = 0.0f;
-  int* exchange = reinterpret_cast<int*>(smem);  // [rows][128 channels], once the stages are done with
+  int* exchange = reinterpret_cast<int*>(smem);                          // [rows][128 channels], once the stages are done with
+  float* deltas = reinterpret_cast<float*>(smem) + kRowTile * kBlockM;  // [own rows][128 channels]: the adapters' sums
   const uint32_t acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
   if (epilogue) {
     const int thread = static_cast<int>(threadIdx.x) - 64;
@@ -321,58 +364,75 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
         for (int j = 0; j < 16; ++j) {
           if (j >= count16) break;
           const float value = finish(static_cast<int>(bits[j]), ctl->row_scale[c0 + j], channel_scale, bias, extra > 0 ? __uint_as_float(delta[j]) : 0.0f);
-          if (args.g.out_bf16) {
-            static_cast<uint16_t*>(args.g.out)[index + static_cast<int64_t>(j) * n] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
-          } else {
-            static_cast<float*>(args.g.out)[index + static_cast<int64_t>(j) * n] = value;
-          }
+          store_value(args.g, index + static_cast<int64_t>(j) * n, value);
         }
       }
       __syncwarp();  // the next tensor-memory load wants the whole warp
+    }
+    if (parts > 1 && extra > 0) {
+      for (int c0 = 0; c0 < own; c0 += 16) {
+        uint32_t bits[16];
+        ptx::tmem_ld_x8(acc + kRowTile + c0, bits);
+        ptx::tmem_ld_x8(acc + kRowTile + c0 + 8, bits + 8);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) deltas[(c0 + j) * kBlockM + channel] = __uint_as_float(bits[j]);
+        __syncwarp();
+      }
     }
   }
   if (parts > 1) {
     __syncwarp();
     cluster_sync();  // every part's accumulators lie in its shared memory
     if (epilogue) {
-      // A thread finishes its channel of the own rows, sixteen at a time: their adapters' sums lie in its lane of tensor memory.
-      const uint32_t mine = ptx::smem_u32(exchange) + 4u * static_cast<uint32_t>(channel);
-      for (int c0 = 0; c0 < own; c0 += 16) {
-        uint32_t delta[16];
-        if (extra > 0) {
-          ptx::tmem_ld_x8(acc + kRowTile + c0, delta);
-          ptx::tmem_ld_x8(acc + kRowTile + c0 + 8, delta + 8);
-          ptx::tmem_ld_wait();
-        }
-        const int count16 = min(16, own - c0);
-        int sums[16];
+      // A warp finishes a row at a time, four channels per lane: 16-byte loads, all parts' in flight together.
+      const int c4 = 4 * lane;
+      const uint32_t mine = ptx::smem_u32(exchange) + 4u * static_cast<uint32_t>(c4);
+      const int columns = n - (n0 + c4);  // channels of this lane that exist, if below four
+      const float4 scales = *reinterpret_cast<const float4*>(ctl->channel_scale + c4);
+      const float4 biases = *reinterpret_cast<const float4*>(ctl->channel_bias + c4);
+      constexpr int kBatch = 2;  // rows of a warp whose loads are in flight together
+      for (int first = warp - 2; first < own; first += 4 * kBatch) {
+        int4 values[kBatch][kMaxParts];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sums[j] = 0;
-        for (int c = 0; c < parts; ++c) {
-          uint32_t remote;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(mine), "r"(c));
+        for (int b = 0; b < kBatch; ++b) {
+          const int row = first + 4 * b;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (j >= count16) break;
-            int value;
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(value) : "r"(remote + static_cast<uint32_t>(own_first + c0 + j) * (kBlockM * 4)) : "memory");
-            sums[j] += value;
+          for (int c = 0; c < kMaxParts; ++c) {
+            values[b][c] = make_int4(0, 0, 0, 0);
+            if (c < parts && row < own) values[b][c] = load_cluster_int4(mine + static_cast<uint32_t>(own_first + row) * (kBlockM * 4), c);
           }
         }
-        if (channel_ok) {
-          const int64_t index = (row0 + own_first + c0) * n + n0 + channel;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (j >= count16) break;
-            const float value = finish(sums[j], ctl->row_scale[own_first + c0 + j], channel_scale, bias, extra > 0 ? __uint_as_float(delta[j]) : 0.0f);
-            if (args.g.out_bf16) {
-              static_cast<uint16_t*>(args.g.out)[index + static_cast<int64_t>(j) * n] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
-            } else {
-              static_cast<float*>(args.g.out)[index + static_cast<int64_t>(j) * n] = value;
+        for (int b = 0; b < kBatch; ++b) {
+          const int row = first + 4 * b;
+          if (row >= own || columns <= 0) continue;
+          int4 sum = values[b][0];
+#pragma unroll
+          for (int c = 1; c < kMaxParts; ++c) {
+            sum.x += values[b][c].x;
+            sum.y += values[b][c].y;
+            sum.z += values[b][c].z;
+            sum.w += values[b][c].w;
+          }
+          float4 delta = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (extra > 0) delta = *reinterpret_cast<const float4*>(deltas + row * kBlockM + c4);
+          const float row_scale = ctl->row_scale[own_first + row];
+          const float out[4] = {finish(sum.x, row_scale, scales.x, biases.x, delta.x), finish(sum.y, row_scale, scales.y, biases.y, delta.y),
+                                finish(sum.z, row_scale, scales.z, biases.z, delta.z), finish(sum.w, row_scale, scales.w, biases.w, delta.w)};
+          const int64_t index = (row0 + own_first + row) * n + n0 + c4;
+          if (args.vector_store && args.g.out_bf16) {
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(args.g.out) + index) = make_uint2(pack_bf16(out[0], out[1]), pack_bf16(out[2], out[3]));
+          } else if (args.vector_store) {
+            *reinterpret_cast<float4*>(static_cast<float*>(args.g.out) + index) = make_float4(out[0], out[1], out[2], out[3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (j >= columns) break;
+              store_value(args.g, index + j, out[j]);
             }
           }
         }
-        __syncwarp();
       }
     }
     __syncwarp();
@@ -487,6 +547,7 @@ cudaError_t launch_lora_gemm(const LoraGemmArgs& g, cudaStream_t stream) {
   args.g = g;
   args.k_blocks = (g.k_padded + kBlockKBytes - 1) / kBlockKBytes;
   args.rank_blocks = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  args.vector_store = dense_vector_store(g.out, g.n, g.out_bf16 != 0) ? 1 : 0;
   if (g.rows <= 16) return launch_tile<16>(args, stream);
   if (g.rows <= 32) return launch_tile<32>(args, stream);
   if (g.rows <= 64) return launch_tile<64>(args, stream);
