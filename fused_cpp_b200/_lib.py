@@ -45,7 +45,7 @@ EXPORTS = (
     "fmoe_stage_timer_create", "fmoe_stage_timer_destroy", "fmoe_stage_timer_reset", "fmoe_stage_timer_calls",
     "fmoe_stage_timer_read", "fmoe_route_build_noalloc", "fmoe_ep_dispatch_workspace_bytes", "fmoe_ep_dispatch_prepare",
     "fmoe_w8a8_expert_rows_forward", "fmoe_bf16_expert_rows_forward", "fmoe_ep_combine_finish",
-    "fmoe_i8gemm_dynamic_scaled_mm_pair", "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward",
+    "fmoe_i8gemm_dynamic_scaled_mm_pair", "fmoe_gated_mlp_derivative_count", "fmoe_gated_mlp_forward", "fmoe_gated_mlp_backward",
     "fmoe_i8gemm_lora_workspace_bytes", "fmoe_i8gemm_dynamic_scaled_mm_lora", "fmoe_dense_status",
     "fmoe_router_topk", "fmoe_append_shared_route",
     "fmoe_ep_peer_create", "fmoe_ep_peer_handle", "fmoe_ep_peer_connect", "fmoe_ep_peer_destroy", "fmoe_ep_peer_slab_bytes",
@@ -190,6 +190,8 @@ def _open(path: str) -> ctypes.CDLL:
     lib.fmoe_i8gemm_lora_workspace_bytes.restype = ctypes.c_size_t
     lib.fmoe_i8gemm_lora_workspace_bytes.argtypes = [i64, i32, i32, i32]
     lib.fmoe_i8gemm_dynamic_scaled_mm_lora.argtypes = [p, i64, i32, p, p, p, i32, ctypes.POINTER(LoraAdapters), p, i32, p, i32, p, ctypes.c_size_t, p]
+    lib.fmoe_gated_mlp_derivative_count.argtypes = [i64, i32]
+    lib.fmoe_gated_mlp_derivative_count.restype = i64
     lib.fmoe_gated_mlp_forward.argtypes = [p, i64, p, p, i64, i32, i32, i32, ctypes.c_float, p, p, p, p]
     lib.fmoe_gated_mlp_backward.argtypes = [p, i64, p, i64, p, p, p, p, i64, i32, i32, p, p, p, p, p]
     lib.fmoe_dense_status.argtypes = [p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]

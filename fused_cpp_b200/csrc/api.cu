@@ -1063,8 +1063,12 @@ int check_rows(const char* what, const char* name, const void* data, int64_t str
 }
 }  // namespace
 
+int64_t fmoe_gated_mlp_derivative_count(int64_t rows, int32_t inter) {
+  return rows <= 0 || inter <= 0 ? 0 : (rows + 31) / 32 * ((static_cast<int64_t>(inter) + 31) / 32) * 2048;
+}
+
 int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, const void* w2, int64_t rows, int32_t hidden, int32_t inter,
-                           int32_t activation, float swiglu_limit, void* h, void* by_gate_up, void* y, void* stream_ptr) {
+                           int32_t activation, float swiglu_limit, void* h, void* derivatives, void* y, void* stream_ptr) {
   static const char* const what = "gated_mlp_forward";
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   int status = check_gated_shape(what, rows, hidden, inter);
@@ -1081,12 +1085,12 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
       (status = check_rows(what, "y", y, hidden, hidden)) != FMOE_OK) {
     return status;
   }
-  if (!vector_aligned(by_gate_up)) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: by_gate_up must be 16-byte aligned", what);
+  if (!vector_aligned(derivatives)) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: derivatives must be 16-byte aligned", what);
   int* words = nullptr;
   cudaError_t error = fmoe::dense_status_words(&words);
   if (error == cudaSuccess && rows <= gated_small_rows()) {
     error = fmoe::launch_gated_projection_small(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
-                                                swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(by_gate_up), words, stream, false);
+                                                swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(derivatives), words, stream, false);
     if (error == cudaSuccess) {
       error = fmoe::launch_dense_small(static_cast<const uint16_t*>(h), rows, inter, static_cast<const uint16_t*>(w2), hidden, false, static_cast<uint16_t*>(y), words,
                                        stream, true);
@@ -1095,7 +1099,7 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
   }
   if (error == cudaSuccess) {
     error = fmoe::launch_gated_projection(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
-                                          swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(by_gate_up), words, stream, false);
+                                          swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(derivatives), words, stream, false);
   }
   if (error == cudaSuccess) {
     const fmoe::DenseProductArgs down = {{static_cast<const uint16_t*>(h), inter}, {static_cast<const uint16_t*>(w2), inter}, static_cast<uint16_t*>(y), rows, hidden, inter};
@@ -1105,7 +1109,7 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
 }
 
 int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w13, const void* w2, const void* h,
-                            const void* by_gate_up, int64_t rows, int32_t hidden, int32_t inter, void* d_gate_up, void* dx, void* dw13, void* dw2,
+                            const void* derivatives, int64_t rows, int32_t hidden, int32_t inter, void* d_gate_up, void* dx, void* dw13, void* dw2,
                             void* stream_ptr) {
   static const char* const what = "gated_mlp_backward";
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
@@ -1118,7 +1122,7 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
   if (dx != nullptr && (status = check_rows(what, "w13", w13, hidden, hidden)) != FMOE_OK) return status;
   if (dw2 != nullptr && (status = check_rows(what, "h", h, inter, inter)) != FMOE_OK) return status;
   if (needs_gate_up && ((status = check_rows(what, "w2", w2, inter, inter)) != FMOE_OK ||
-                        (status = check_rows(what, "by_gate_up", by_gate_up, 2 * static_cast<int64_t>(inter), 2 * inter)) != FMOE_OK ||
+                        (status = check_rows(what, "derivatives", derivatives, 2 * static_cast<int64_t>(inter), 2 * inter)) != FMOE_OK ||
                         (status = check_rows(what, "d_gate_up", d_gate_up, 2 * static_cast<int64_t>(inter), 2 * inter)) != FMOE_OK)) {
     return status;
   }
@@ -1131,7 +1135,7 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
   const bool small = rows <= gated_small_rows();
   if (error == cudaSuccess && needs_gate_up) {
     auto launch = small ? fmoe::launch_gated_backward_small : fmoe::launch_gated_backward;
-    error = launch(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const float*>(by_gate_up), rows, hidden, inter,
+    error = launch(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const float*>(derivatives), rows, hidden, inter,
                    static_cast<uint16_t*>(d_gate_up), words, stream, chained);
     chained = true;
   }

@@ -9,8 +9,9 @@
 //
 // Two CTAs of a cluster drive one 256 x 256 tile (cta_group::2): each stages its 128 A rows and its half of the B rows (64 KB a K block of
 // 64 for the pair), which is what an SM can take from L2 while the tensor pipe works (umma2_gemm.cu has the figures).  D rows are token or weight rows and lie in
-// the lanes of tensor memory; its columns are output channels, so that a lane holds 32 neighbouring channels of one row and stores them as
-// four 16-byte vectors.  For the gated projection CTA 0 stages 128 gate rows and CTA 1 the 128 up rows of the same channels: gate and up of
+// the lanes of tensor memory; its columns are output channels.  An epilogue warp turns 64 of them at a time into 128-byte rows of its 4 KB of shared
+// memory, and TMA stores the 32 x 64 block (and clips what lies behind the matrix).  Stored by the lanes, 16 bytes of a row each, the weight gradients of 40 rows
+// of 7168 x 2048, which write 88 MB behind one K block a tile, took 42 us.  For the gated projection CTA 0 stages 128 gate rows and CTA 1 the 128 up rows of the same channels: gate and up of
 // a channel are columns c and 128 + c of the same lane.  Two accumulators of 256 columns take turns: the epilogue of a tile runs under the products of the
 // next.
 //
@@ -36,6 +37,7 @@ constexpr int kUmmaK = 16;
 constexpr int kEpilogueWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kTmemColumns = 512;
+constexpr int kStagingBytes = 32 * 128;           // of an epilogue warp: 32 rows of 128 bytes
 constexpr int kMaxStages = 8;
 constexpr int kTileGroup = 8;  // row tiles that are walked together (see tile_at)
 
@@ -49,7 +51,8 @@ struct TileConfig {
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = 192 * 1024 / kStageBytes;
   static_assert(kStages <= kMaxStages, "the barriers of all stages");
-  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + 1024;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;
+  static_assert(kSmemBytes <= 227 * 1024, "a CTA has 227 KB of shared memory");
 };
 
 struct Control {
@@ -63,7 +66,6 @@ struct Control {
 static_assert(sizeof(Control) <= 1024, "control block exceeds its shared-memory reservation");
 
 struct Problem {
-  uint16_t* out;
   int64_t m;
   int n;         // output channels
   int k_blocks;
@@ -73,8 +75,8 @@ struct Problem {
 struct Args {
   Problem problem[2];
   int64_t tiles[2];  // tiles of the first problem, and of both
-  float* by_gate_up_out;
-  const float* by_gate_up;
+  int keep;             // the forward pass stores the derivatives
+  float4* derivatives;  // see derivative_block
   int activation;
   float limit;
   int* status;
@@ -100,35 +102,57 @@ __device__ __forceinline__ Tile tile_at(const Args& args, int64_t index) {
   return t;
 }
 
-// Up to 32 neighbouring channels of a row as bf16: `columns` of them exist, a multiple of 8.
-__device__ __forceinline__ void store_channels(uint16_t* to, const float (&v)[32], int columns) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (8 * q >= columns) break;
-    *reinterpret_cast<uint4*>(to + 8 * q) = make_uint4(pack_bf16(v[8 * q], v[8 * q + 1]), pack_bf16(v[8 * q + 2], v[8 * q + 3]),
-                                                       pack_bf16(v[8 * q + 4], v[8 * q + 5]), pack_bf16(v[8 * q + 6], v[8 * q + 7]));
-  }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               :
+               : "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(x), "r"(y)
+               : "memory");
 }
 
-__device__ __forceinline__ void store_channels(float* to, const float (&v)[32], int columns) {
-#pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    if (4 * q >= columns) break;
-    *reinterpret_cast<float4*>(to + 4 * q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               :
+               : "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(x), "r"(y), "r"(z)
+               : "memory");
 }
+
+// A warp's 4 KB of shared memory on the way to a block of 32 rows of 128 bytes, in the 128-byte swizzle: lane r fills row r.
+struct Staging {
+  uint8_t* base;
+  int lane;
+
+  // The block before has been read out of shared memory.
+  __device__ __forceinline__ void begin() const {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+  }
+  __device__ __forceinline__ void put(int piece, uint4 value) const {
+    *reinterpret_cast<uint4*>(base + lane * 128 + ((piece ^ (lane & 7)) << 4)) = value;
+  }
+  // All rows are written: store(shared-memory address) issues the copy.
+  template <typename Store>
+  __device__ __forceinline__ void end(Store&& store) const {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      store(ptx::smem_u32(base));
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+};
 
 template <Epilogue kEpilogue, bool kAByK, bool kBByK, int kTileN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_constant__ CUtensorMap b_map0,
                        const __grid_constant__ CUtensorMap a_map1, const __grid_constant__ CUtensorMap b_map1,
-                       const __grid_constant__ Args args) {
+                       const __grid_constant__ CUtensorMap out_map0, const __grid_constant__ CUtensorMap out_map1, const __grid_constant__ Args args) {
   using Cfg = TileConfig<kTileN>;
   constexpr int kStages = Cfg::kStages;
   constexpr int kColumns = kEpilogue == Epilogue::kGated ? kTileN / 2 : kTileN;  // output channels of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Control* ctl = reinterpret_cast<Control*>(smem + static_cast<size_t>(kStages) * Cfg::kStageBytes);
+  uint8_t* const staging_base = smem + static_cast<size_t>(kStages) * Cfg::kStageBytes;
+  Control* ctl = reinterpret_cast<Control*>(staging_base + kEpilogueWarps * kStagingBytes);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
@@ -287,81 +311,107 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
     const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id % 4
     const int chunk_first = (warp - 2) >> 2;
     constexpr int kChunkStep = kEpilogueWarps / 4;
-    constexpr int kChunks = kColumns / 32;
+    constexpr int kChunks = kColumns / 64;
+    const Staging staging = {staging_base + (warp - 2) * kStagingBytes, lane};
     const uint32_t acc_lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t acc_empty_leader = map_to_cta(ptx::smem_u32(&ctl->acc_empty[0]), 0);
     int local = 0;
     for (int64_t index = first_tile; index < tiles; index += tile_stride, ++local) {
       const Tile tile = tile_at(args, index);
       const Problem& p = args.problem[tile.problem];
+      const CUtensorMap* const out_map = tile.problem ? &out_map1 : &out_map0;
       const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
       const uint32_t use = static_cast<uint32_t>(local) >> 1;
-      const int64_t row = static_cast<int64_t>(tile.m) * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + quarter * 32 + lane;
-      const bool row_ok = row < p.m;
+      const int warp_row = tile.m * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + quarter * 32;  // below 2^31 (check_gated_shape)
       const int n0 = tile.n * kColumns;
       const uint32_t acc = acc_lane_base + kTileN * buffer;
+      const bool rows_exist = warp_row < p.m;  // of this warp's 32; a block may begin nowhere behind the matrix
       ptx::mbar_wait(&ctl->acc_full[buffer], use & 1u, abort_flag, status, 44);
       ptx::tcgen05_fence_after();
       for (int chunk = chunk_first; chunk < kChunks; chunk += kChunkStep) {
-        const int col = n0 + 32 * chunk;
-        const int columns = row_ok ? p.n - col : 0;  // of this lane's chunk that exist, if below 32
-        uint32_t bits[32];
-        tmem_ld_x32(acc + 32u * static_cast<uint32_t>(chunk), bits);
+        const int col = n0 + 64 * chunk;
+        if (!rows_exist || col >= p.n) break;
+        const uint32_t from = acc + 64u * static_cast<uint32_t>(chunk);
         if constexpr (kEpilogue == Epilogue::kGated) {
-          uint32_t up_bits[32];
-          tmem_ld_x32(acc + static_cast<uint32_t>(kTileN / 2) + 32u * static_cast<uint32_t>(chunk), up_bits);
-          ptx::tmem_ld_wait();
-          float h[32], by_gate[32], by_up[32];
-          with_activation<false>(args.activation, [&](auto act) {
+          staging.begin();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              gated_with_derivatives(act, __uint_as_float(bits[j]), __uint_as_float(up_bits[j]), args.limit, &h[j], &by_gate[j], &by_up[j]);
-            }
-          });
-          store_channels(p.out + row * p.n + col, h, columns);
-          if (args.by_gate_up_out != nullptr) {
-            float* const by = args.by_gate_up_out + row * 2 * p.n + col;
-            store_channels(by, by_gate, columns);
-            store_channels(by + p.n, by_up, columns);
+          for (int half = 0; half < 2; ++half) {
+            uint32_t bits[32], up_bits[32];
+            tmem_ld_x32(from + 32u * half, bits);
+            tmem_ld_x32(from + static_cast<uint32_t>(kTileN / 2) + 32u * half, up_bits);
+            ptx::tmem_ld_wait();
+            float4* const by = args.keep && warp_row + lane < p.m && col + 32 * half < p.n ? args.derivatives + derivative_block(warp_row, col + 32 * half, p.n) + lane : nullptr;
+            with_activation<false>(args.activation, [&](auto act) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float h[8], by_gate[8], by_up[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  gated_with_derivatives(act, __uint_as_float(bits[8 * q + j]), __uint_as_float(up_bits[8 * q + j]), args.limit, &h[j], &by_gate[j], &by_up[j]);
+                }
+                staging.put(4 * half + q, make_uint4(pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3]), pack_bf16(h[4], h[5]), pack_bf16(h[6], h[7])));
+                if (by != nullptr) {
+                  by[64 * q] = make_float4(by_gate[0], by_gate[1], by_gate[2], by_gate[3]);
+                  by[64 * q + 32] = make_float4(by_gate[4], by_gate[5], by_gate[6], by_gate[7]);
+                  by[256 + 64 * q] = make_float4(by_up[0], by_up[1], by_up[2], by_up[3]);
+                  by[256 + 64 * q + 32] = make_float4(by_up[4], by_up[5], by_up[6], by_up[7]);
+                }
+              }
+            });
           }
+          staging.end([&](uint32_t block) { tma_store_2d(&out_map0, block, col, warp_row); });
         } else if constexpr (kEpilogue == Epilogue::kGatedBack) {
-          const float* const by = args.by_gate_up + row * 2 * p.n + col;
-          uint16_t* const to = p.out + row * 2 * p.n + col;
-          float4 factors[2][8];
+          uint32_t d_up[32];  // 64 channels, kept while those of d_gate are on their way out
+          staging.begin();
 #pragma unroll
-          for (int side = 0; side < 2; ++side) {
+          for (int half = 0; half < 2; ++half) {
+            const bool exists = warp_row + lane < p.m && col + 32 * half < p.n;
+            const float4* const by = args.derivatives + derivative_block(warp_row, col + 32 * half, p.n) + lane;
+            float4 factors[16];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              factors[side][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              if (4 * q < columns) factors[side][q] = __ldcs(reinterpret_cast<const float4*>(by + side * p.n) + q);
-            }
-          }
-          ptx::tmem_ld_wait();
-#pragma unroll
-          for (int side = 0; side < 2; ++side) {
-            float v[32];
+            for (int q = 0; q < 16; ++q) factors[q] = exists ? __ldcs(by + 32 * q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            uint32_t bits[32];
+            tmem_ld_x32(from + 32u * half, bits);
+            ptx::tmem_ld_wait();
+            uint32_t d_gate[16];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-              v[4 * q] = __uint_as_float(bits[4 * q]) * factors[side][q].x;
-              v[4 * q + 1] = __uint_as_float(bits[4 * q + 1]) * factors[side][q].y;
-              v[4 * q + 2] = __uint_as_float(bits[4 * q + 2]) * factors[side][q].z;
-              v[4 * q + 3] = __uint_as_float(bits[4 * q + 3]) * factors[side][q].w;
+              const float v[4] = {__uint_as_float(bits[4 * q]), __uint_as_float(bits[4 * q + 1]), __uint_as_float(bits[4 * q + 2]), __uint_as_float(bits[4 * q + 3])};
+              d_gate[2 * q] = pack_bf16(v[0] * factors[q].x, v[1] * factors[q].y);
+              d_gate[2 * q + 1] = pack_bf16(v[2] * factors[q].z, v[3] * factors[q].w);
+              d_up[16 * half + 2 * q] = pack_bf16(v[0] * factors[8 + q].x, v[1] * factors[8 + q].y);
+              d_up[16 * half + 2 * q + 1] = pack_bf16(v[2] * factors[8 + q].z, v[3] * factors[8 + q].w);
             }
-            store_channels(to + side * p.n, v, columns);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) staging.put(4 * half + q, make_uint4(d_gate[4 * q], d_gate[4 * q + 1], d_gate[4 * q + 2], d_gate[4 * q + 3]));
           }
+          staging.end([&](uint32_t block) { tma_store_3d(&out_map0, block, col, 0, warp_row); });
+          staging.begin();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) staging.put(q, make_uint4(d_up[4 * q], d_up[4 * q + 1], d_up[4 * q + 2], d_up[4 * q + 3]));
+          staging.end([&](uint32_t block) { tma_store_3d(&out_map0, block, col, 1, warp_row); });
         } else {
+          uint32_t bits[64];
+          tmem_ld_x32(from, bits);
+          tmem_ld_x32(from + 32u, bits + 32);
           ptx::tmem_ld_wait();
-          float v[32];
+          staging.begin();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(bits[j]);
-          store_channels(p.out + row * p.n + col, v, columns);
+          for (int q = 0; q < 8; ++q) {
+            uint32_t words[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) words[j] = pack_bf16(__uint_as_float(bits[8 * q + 2 * j]), __uint_as_float(bits[8 * q + 2 * j + 1]));
+            staging.put(q, make_uint4(words[0], words[1], words[2], words[3]));
+          }
+          staging.end([&](uint32_t block) { tma_store_2d(out_map, block, col, warp_row); });
         }
-        __syncwarp();  // the next tensor-memory load wants the whole warp
       }
       ptx::tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * buffer);
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // every block has arrived
+    __syncwarp();
   }
 
   ptx::tcgen05_fence_before();
@@ -377,6 +427,7 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
 struct Operands {
   DenseOperand a, b;
   int64_t b_rows;  // rows of B along its n axis in memory (2 * inter for the gated projection)
+  uint16_t* out;   // [m, n], or [m, 2, n] for the gated backward product
 };
 
 template <Epilogue kEpilogue, bool kAByK, bool kBByK, int kTileN>
@@ -391,7 +442,7 @@ cudaError_t launch_tiles(Args args, const Operands* operands, int count, const i
     configured.mark(device);
   }
   constexpr int kColumns = kEpilogue == Epilogue::kGated ? kTileN / 2 : kTileN;
-  CUtensorMap maps[4];
+  CUtensorMap maps[6];
   int64_t total = 0;
   for (int i = 0; i < 2; ++i) {
     const int from = i < count ? i : 0;
@@ -402,6 +453,13 @@ cudaError_t launch_tiles(Args args, const Operands* operands, int count, const i
     const bool ok = make_sw128_map(&maps[2 * i], o.a.data, false, kAByK ? k : m, kAByK ? m : k, kAByK ? kBlockK : kRowsPerCta, o.a.stride) &&
                     make_sw128_map(&maps[2 * i + 1], o.b.data, false, kBByK ? k : n, kBByK ? n : k, kBByK ? kBlockK : Cfg::kBRows, o.b.stride);
     if (!ok) return cudaErrorInvalidValue;
+    bool out_ok;
+    if (kEpilogue == Epilogue::kGatedBack) {
+      out_ok = make_store_map(&maps[4 + i], o.out, false, static_cast<uint64_t>(p.n), 2, m);
+    } else {
+      out_ok = make_store_map(&maps[4 + i], o.out, false, static_cast<uint64_t>(p.n), 1, m);
+    }
+    if (!out_ok) return cudaErrorInvalidValue;
     p.k_blocks = static_cast<int>((k + kBlockK - 1) / kBlockK);
     p.m_tiles = static_cast<int>((p.m + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta));
     p.n_tiles = (p.n + kColumns - 1) / kColumns;
@@ -412,7 +470,7 @@ cudaError_t launch_tiles(Args args, const Operands* operands, int count, const i
   if (total > (1ll << 30)) return cudaErrorInvalidValue;
   int64_t pairs = sm_count_of_current_device() / 2;
   if (pairs > total) pairs = total;
-  return launch_chained(kernel, dim3(static_cast<unsigned>(2 * pairs)), kThreads, Cfg::kSmemBytes, stream, chained, maps[0], maps[1], maps[2], maps[3], args);
+  return launch_chained(kernel, dim3(static_cast<unsigned>(2 * pairs)), kThreads, Cfg::kSmemBytes, stream, chained, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], args);
 }
 
 template <Epilogue kEpilogue, bool kAByK, bool kBByK>
@@ -441,29 +499,28 @@ cudaError_t dense_status_words(int** words) {
 }
 
 cudaError_t launch_gated_projection(const uint16_t* x, int64_t x_stride, const uint16_t* w13, int64_t rows, int hidden, int inter, int activation,
-                                    float limit, uint16_t* h, float* by_gate_up, int* status, cudaStream_t stream, bool chained) {
+                                    float limit, uint16_t* h, float* derivatives, int* status, cudaStream_t stream, bool chained) {
   Args args = {};
-  args.problem[0].out = h;
   args.problem[0].m = rows;
   args.problem[0].n = inter;
-  args.by_gate_up_out = by_gate_up;
+  args.keep = derivatives != nullptr ? 1 : 0;
+  args.derivatives = reinterpret_cast<float4*>(derivatives);
   args.activation = activation;
   args.limit = limit;
   args.status = status;
-  const Operands operands = {{x, x_stride}, {w13, hidden}, 2 * static_cast<int64_t>(inter)};
+  const Operands operands = {{x, x_stride}, {w13, hidden}, 2 * static_cast<int64_t>(inter), h};
   const int64_t depth = hidden;
   return launch_form<Epilogue::kGated, false, false>(args, &operands, 1, &depth, stream, chained);
 }
 
-cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* by_gate_up, int64_t rows, int hidden,
+cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* derivatives, int64_t rows, int hidden,
                                   int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained) {
   Args args = {};
-  args.problem[0].out = d_gate_up;
   args.problem[0].m = rows;
   args.problem[0].n = inter;
-  args.by_gate_up = by_gate_up;
+  args.derivatives = reinterpret_cast<float4*>(const_cast<float*>(derivatives));
   args.status = status;
-  const Operands operands = {{dy, dy_stride}, {w2, inter}, inter};
+  const Operands operands = {{dy, dy_stride}, {w2, inter}, inter, d_gate_up};
   const int64_t depth = hidden;
   return launch_form<Epilogue::kGatedBack, false, true>(args, &operands, 1, &depth, stream, chained);
 }
@@ -475,10 +532,9 @@ cudaError_t launch_dense_products(DenseForm form, const DenseProductArgs* produc
   int64_t depth[2];
   for (int i = 0; i < count; ++i) {
     const DenseProductArgs& p = products[i];
-    args.problem[i].out = p.out;
     args.problem[i].m = p.m;
     args.problem[i].n = p.n;
-    operands[i] = {p.a, p.b, p.n};
+    operands[i] = {p.a, p.b, p.n, p.out};
     depth[i] = p.k;
   }
   args.status = status;

@@ -59,8 +59,8 @@ struct Args {
   int n;           // output channels
   int k_blocks;
   int row_tiles, parts;
-  float* by_gate_up_out;
-  const float* by_gate_up;
+  int keep;             // the forward pass stores the derivatives
+  float4* derivatives;  // see derivative_block
   int activation;
   float limit;
   int* status;
@@ -274,10 +274,10 @@ gated_small_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_
           for (int j = 0; j < 4; ++j) gated_with_derivatives(act, gate[j], up[j], args.limit, &h[j], &by_gate[j], &by_up[j]);
         });
         store4(args.out + (row0 + row) * args.n + n, h);
-        if (args.by_gate_up_out != nullptr) {
-          float* const by = args.by_gate_up_out + (row0 + row) * 2 * args.n + n;
-          *reinterpret_cast<float4*>(by) = make_float4(by_gate[0], by_gate[1], by_gate[2], by_gate[3]);
-          *reinterpret_cast<float4*>(by + args.n) = make_float4(by_up[0], by_up[1], by_up[2], by_up[3]);
+        if (args.keep) {
+          float4* const by = args.derivatives + derivative_block(row0 + row, n, args.n) + (n & 31) / 4 * 32 + ((row0 + row) & 31);
+          by[0] = make_float4(by_gate[0], by_gate[1], by_gate[2], by_gate[3]);
+          by[256] = make_float4(by_up[0], by_up[1], by_up[2], by_up[3]);
         }
       }
     } else {
@@ -287,9 +287,9 @@ gated_small_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_
         float4 by_gate = make_float4(0.0f, 0.0f, 0.0f, 0.0f), by_up = by_gate;
         if constexpr (kEpilogue == Epilogue::kGatedBack) {
           if (n < args.n) {
-            const float* const by = args.by_gate_up + (row0 + row) * 2 * args.n + n;
-            by_gate = __ldcs(reinterpret_cast<const float4*>(by));
-            by_up = __ldcs(reinterpret_cast<const float4*>(by + args.n));
+            const float4* const by = args.derivatives + derivative_block(row0 + row, n, args.n) + (n & 31) / 4 * 32 + ((row0 + row) & 31);
+            by_gate = __ldcs(by);
+            by_up = __ldcs(by + 256);
           }
         }
         float sum[4];
@@ -431,25 +431,26 @@ cudaError_t launch(const Args& args, const Operands& operands, cudaStream_t stre
 }  // namespace
 
 cudaError_t launch_gated_projection_small(const uint16_t* x, int64_t x_stride, const uint16_t* w13, int64_t rows, int hidden, int inter, int activation,
-                                          float limit, uint16_t* h, float* by_gate_up, int* status, cudaStream_t stream, bool chained) {
+                                          float limit, uint16_t* h, float* derivatives, int* status, cudaStream_t stream, bool chained) {
   Args args = {};
   args.out = h;
   args.rows = rows;
   args.n = inter;
-  args.by_gate_up_out = by_gate_up;
+  args.keep = derivatives != nullptr ? 1 : 0;
+  args.derivatives = reinterpret_cast<float4*>(derivatives);
   args.activation = activation;
   args.limit = limit;
   args.status = status;
   return launch<Epilogue::kGated, false>(args, {w13, 2 * static_cast<int64_t>(inter), hidden, x, x_stride, hidden}, stream, chained);
 }
 
-cudaError_t launch_gated_backward_small(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* by_gate_up, int64_t rows, int hidden,
+cudaError_t launch_gated_backward_small(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* derivatives, int64_t rows, int hidden,
                                         int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained) {
   Args args = {};
   args.out = d_gate_up;
   args.rows = rows;
   args.n = inter;
-  args.by_gate_up = by_gate_up;
+  args.derivatives = reinterpret_cast<float4*>(const_cast<float*>(derivatives));
   args.status = status;
   return launch<Epilogue::kGatedBack, true>(args, {w2, hidden, inter, dy, dy_stride, hidden}, stream, chained);
 }

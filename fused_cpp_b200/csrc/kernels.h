@@ -295,6 +295,9 @@ bool make_sw128_map(CUtensorMap* map, const void* base, bool int8, uint64_t rows
 // 3-D bf16 tensor [planes, rows, columns], row_stride elements from a row to the next, boxes of {128 bytes of a row, box_rows} of one plane.
 bool make_sw128_map_3d(CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows, uint64_t planes, uint64_t row_stride, uint32_t box_rows);
 
+// Result rows [rows, columns] (sides = 1) or [rows, sides, columns] of bf16 or fp32, for stores of swizzled boxes of {128 bytes, 32 rows} of a side.
+bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows);
+
 // ---- gated_gemm.cu: dense bf16 products of the gated feed-forward block over many rows (two-SM kernel).
 // out[m, n] = sum over k of A[m, k] B[n, k]; an operand marked `by_k` lies in memory as [k, m] or [k, n].
 struct DenseOperand {
@@ -308,20 +311,20 @@ struct DenseProductArgs {
   int n;
   int64_t k;
 };
-// h = act(x Wg^T, x Wu^T) for rows x [rows, hidden] and w13 [2 * inter, hidden]; by_gate_up (nullable): the partial derivatives of h by gate
-// and up, fp32 [rows, 2 * inter].
+// h = act(x Wg^T, x Wu^T) for rows x [rows, hidden] and w13 [2 * inter, hidden]; derivatives (nullable): the partial derivatives of h by gate
+// and up, fp32 in the blocks of gated.cuh.
 cudaError_t launch_gated_projection(const uint16_t* x, int64_t x_stride, const uint16_t* w13, int64_t rows, int hidden, int inter, int activation,
-                                    float limit, uint16_t* h, float* by_gate_up, int* status, cudaStream_t stream, bool chained);
+                                    float limit, uint16_t* h, float* derivatives, int* status, cudaStream_t stream, bool chained);
 // d_gate_up = (dy W2) times the partial derivatives, [rows, 2 * inter], for w2 [hidden, inter].
-cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* by_gate_up, int64_t rows, int hidden,
+cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* derivatives, int64_t rows, int hidden,
                                   int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained);
 // The status block (kStatusWords ints, zero unless a bounded wait gave up) of the current device for launches without a workspace.
 cudaError_t dense_status_words(int** words);
 // The same products over few rows (gated_small.cu): clusters that split the K range.  out [rows, n] = tokens [rows, k] times weight [n, k], or
 // [k, n] with weight_by_k.
 cudaError_t launch_gated_projection_small(const uint16_t* x, int64_t x_stride, const uint16_t* w13, int64_t rows, int hidden, int inter, int activation,
-                                          float limit, uint16_t* h, float* by_gate_up, int* status, cudaStream_t stream, bool chained);
-cudaError_t launch_gated_backward_small(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* by_gate_up, int64_t rows, int hidden,
+                                          float limit, uint16_t* h, float* derivatives, int* status, cudaStream_t stream, bool chained);
+cudaError_t launch_gated_backward_small(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* derivatives, int64_t rows, int hidden,
                                         int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained);
 cudaError_t launch_dense_small(const uint16_t* tokens, int64_t rows, int k, const uint16_t* weight, int n, bool weight_by_k, uint16_t* out, int* status,
                                cudaStream_t stream, bool chained);

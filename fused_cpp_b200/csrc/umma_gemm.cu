@@ -764,6 +764,23 @@ bool make_sw128_map_3d(CUtensorMap* map, const void* base, uint64_t columns, uin
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr) return false;
+  const uint64_t elem_bytes = f32 ? 4 : 2;
+  const cuuint64_t dims3[3] = {columns, sides, rows};
+  const cuuint64_t strides3[2] = {columns * elem_bytes, sides * columns * elem_bytes};
+  const cuuint64_t dims2[2] = {columns, rows};
+  const cuuint64_t strides2[1] = {columns * elem_bytes};
+  const cuuint32_t inner = static_cast<cuuint32_t>(kBlockKBytes / elem_bytes);
+  const cuuint32_t box3[3] = {inner, 1, 32};
+  const cuuint32_t box2[2] = {inner, 32};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  return encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sides > 1 ? 3 : 2, base, sides > 1 ? dims3 : dims2,
+                sides > 1 ? strides3 : strides2, sides > 1 ? box3 : box2, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 namespace {
 
 // W8A16 landing loads: int8 weight rows [rows, k] as plain (unswizzled) boxes of {64 bytes of K, 128 rows}.

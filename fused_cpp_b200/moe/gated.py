@@ -8,7 +8,8 @@ activations, as plain tensors that an optimiser updates.  Both projections, the 
 second; the backward pass is three launches.  Sums are fp32; h = act(..) is rounded to bf16 for the down projection, as in the fused MoE
 operators.  `gated_mlp_forward` and `gated_mlp_backward` are the two passes for programs that keep their own tape.
 
-What a forward pass keeps for the backward pass besides its inputs: h [T, F] and the partial derivatives of h by gate and by up, fp32 [T, 2F].
+What a forward pass keeps for the backward pass besides its inputs: h [T, F] and the partial derivatives of h by gate and by up, 2 TF
+fp32 values in an order of the library's own.
 """
 from __future__ import annotations
 
@@ -85,11 +86,16 @@ def _whole(tensor: torch.Tensor) -> torch.Tensor:
     return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()
 
 
+def _derivative_count(rows: int, inter: int) -> int:
+    """fmoe_gated_mlp_derivative_count: whole blocks of 32 rows x 32 channels x 2."""
+    return -(-rows // 32) * -(-inter // 32) * 2048
+
+
 def _forward(index: int, rows, w13, w2, code: int, limit: float, keep: bool, y):
     count, hidden = rows.shape
     inter = w2.shape[1]
     h = rows.new_empty((count, inter))
-    derivatives = rows.new_empty((count, 2 * inter), dtype=torch.float32) if keep else None
+    derivatives = rows.new_empty(_derivative_count(count, inter), dtype=torch.float32) if keep else None
     _lib.check(_lib.load().fmoe_gated_mlp_forward(rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), count, hidden, inter, code, limit,
                                                   h.data_ptr(), derivatives.data_ptr() if keep else None, y.data_ptr(), _lib._stream_of(index)))
     return h, derivatives
@@ -195,7 +201,7 @@ def gated_mlp_backward(dy, input, w13, w2, h, derivatives, *, needs: tuple = (Tr
     if dy.shape != input.shape:
         raise ValueError(f"dy must have the input's shape {tuple(input.shape)}, got {tuple(dy.shape)}")
     rows = input.numel() // hidden
-    if h.shape != (rows, inter) or derivatives.shape != (rows, 2 * inter) or not h.is_contiguous() or not derivatives.is_contiguous():
+    if h.shape != (rows, inter) or derivatives.shape != (_derivative_count(rows, inter),) or not h.is_contiguous() or not derivatives.is_contiguous():
         raise ValueError("h and derivatives must be what gated_mlp_forward returned for this input")
     if len(needs) != 3:
         raise ValueError("needs must say for dx, dw13 and dw2 whether they are wanted")

@@ -346,15 +346,16 @@ FMOE_API int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows
  * x [rows, H] with x_stride elements from a row to the next, w13 [2F, H] (gate rows, then up rows), w2 [H, F]:
  *   h = act(x Wg^T, x Wu^T) (bf16),  y = h W2^T.
  * activation: FMOE_ACTIVATION_SILU (swiglu_limit > 0: gate clamped from above and up to +-limit first), _GELU, _SWIGLUOAI.
- * h [rows, F] and y [rows, H] are written; by_gate_up fp32 [rows, 2F] (nullable) takes the partial derivatives of h by gate and by up
- * for a backward pass.  H and F are multiples of 8, every row starts on a 16-byte boundary.  Enqueues two launches. */
+ * h [rows, F] and y [rows, H] are written; derivatives (nullable, fmoe_gated_mlp_derivative_count
+ * floats in the library's own order) takes the partial derivatives of h by gate and by up for a backward pass.  H and F are multiples of 8, every row starts on a 16-byte boundary.  Enqueues two launches. */
+FMOE_API int64_t fmoe_gated_mlp_derivative_count(int64_t rows, int32_t inter);
 FMOE_API int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, const void* w2, int64_t rows, int32_t hidden,
-                                    int32_t inter, int32_t activation, float swiglu_limit, void* h, void* by_gate_up, void* y,
+                                    int32_t inter, int32_t activation, float swiglu_limit, void* h, void* derivatives, void* y,
                                     void* stream);
 /* Gradients from dy [rows, H] and what the forward call kept: dx [rows, H], dw13 [2F, H], dw2 [H, F], each left out where null.
  * d_gate_up [rows, 2F] is scratch (needed for dx and dw13).  rows >= 1.  Enqueues up to three launches. */
 FMOE_API int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w13,
-                                     const void* w2, const void* h, const void* by_gate_up, int64_t rows, int32_t hidden,
+                                     const void* w2, const void* h, const void* derivatives, int64_t rows, int32_t hidden,
                                      int32_t inter, void* d_gate_up, void* dx, void* dw13, void* dw2, void* stream);
 /* First device-side error (FMOE_ERR_DEVICE_WAIT: a bounded wait gave up, detail = its site) of the calls on the current device that
  * have no workspace of their own, since the last time it was asked.  Synchronises the stream and clears the record. */

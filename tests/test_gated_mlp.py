@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from fused_cpp_b200 import moe
+from fused_cpp_b200 import _lib, moe
+from fused_cpp_b200.moe import gated
 
 
 def _call(**changes):
@@ -32,9 +33,14 @@ def test_refusals(changes, error, text):
         _call(**changes)
 
 
+@pytest.mark.parametrize("rows, inter", [(0, 8), (1, 8), (32, 32), (33, 40), (1333, 1024)])
+def test_kept_derivatives_have_the_size_the_library_wants(rows, inter):
+    assert gated._derivative_count(rows, inter) == _lib.load().fmoe_gated_mlp_derivative_count(rows, inter)
+
+
 def test_backward_refusals():
     x, w13, w2 = (torch.zeros(*shape, dtype=torch.bfloat16) for shape in ((3, 16), (48, 16), (16, 24)))
-    h, derivatives = torch.zeros(3, 24, dtype=torch.bfloat16), torch.zeros(3, 48)
+    h, derivatives = torch.zeros(3, 24, dtype=torch.bfloat16), torch.zeros(2048)
     with pytest.raises(ValueError, match="input's shape"):
         moe.gated_mlp_backward(x[:2], x, w13, w2, h, derivatives)
     with pytest.raises(ValueError, match="what gated_mlp_forward returned"):
