@@ -980,10 +980,16 @@ int fmoe_i8gemm_dynamic_scaled_mm_pair(const void* x_bf16, int64_t rows, int32_t
   return error == cudaSuccess ? FMOE_OK : cuda_fail(error, "i8gemm pair GEMM");
 }
 
+namespace {
+size_t lora_list_bytes(int64_t rows) {
+  return align_up(static_cast<size_t>((rows + fmoe::kLoraListRows - 1) / fmoe::kLoraListRows) * fmoe::kLoraListInts * sizeof(int), 256);
+}
+}  // namespace
+
 size_t fmoe_i8gemm_lora_workspace_bytes(int64_t rows, int32_t k, int32_t rank, int32_t out_is_bf16) {
   if (rows < 0 || k <= 0 || rank <= 0 || rank > fmoe::kLoraMaxRank) return 0;
   const size_t planes = out_is_bf16 ? 1 : fmoe::kLoraPlanes;
-  return align_up(dense_layout(rows, k).total, 256) + planes * static_cast<size_t>(rows) * fmoe::lora_rank_padded(rank) * 2;
+  return align_up(dense_layout(rows, k).total, 256) + lora_list_bytes(rows) + planes * static_cast<size_t>(rows) * fmoe::lora_rank_padded(rank) * 2;
 }
 
 int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t k, const int8_t* w, const float* w_scale, const float* bias,
@@ -1016,10 +1022,13 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
   fmoe::LoraGemmArgs args = {};
   args.adapters = {static_cast<const uint16_t*>(adapters->a), static_cast<const uint16_t*>(adapters->b), adapters->a_stride, adapters->b_stride, adapters->scaling,
                    adapter_ids, ids_are_64, adapters->count, adapters->rank};
-  uint16_t* const t = reinterpret_cast<uint16_t*>(base + align_up(layout.total, 256));
+  int* const lists = reinterpret_cast<int*>(base + align_up(layout.total, 256));
+  uint16_t* const t = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(lists) + lora_list_bytes(rows));
+  const char* text = getenv("LP");
+  const bool many = rows > (text != nullptr ? atoi(text) : 256);
   args.planes = out_is_bf16 ? 1 : fmoe::kLoraPlanes;
   cudaError_t error = fmoe::launch_lora_quantize(static_cast<const uint16_t*>(x_bf16), rows, k, layout.k_padded, reinterpret_cast<int8_t*>(base + layout.xq),
-                                                 reinterpret_cast<float*>(base + layout.scale), reinterpret_cast<int*>(base + layout.status), stream);
+                                                 reinterpret_cast<float*>(base + layout.scale), reinterpret_cast<int*>(base + layout.status), args.adapters, many ? lists : nullptr, stream);
   if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora activation quantisation");
   error = fmoe::launch_lora_shrink(static_cast<const uint16_t*>(x_bf16), rows, k, args.adapters, t, args.planes, stream);
   if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora coefficients");
@@ -1035,7 +1044,8 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
   args.k_padded = layout.k_padded;
   args.t = t;
   args.status = reinterpret_cast<int*>(base + layout.status);
-  error = fmoe::launch_lora_gemm(args, stream);
+  args.lists = lists;
+  error = many ? fmoe::launch_lora_pair_gemm(args, stream) : fmoe::launch_lora_gemm(args, stream);
   return error == cudaSuccess ? FMOE_OK : cuda_fail(error, "i8gemm lora GEMM");
 }
 
@@ -1049,11 +1059,9 @@ int check_gated_shape(const char* what, int64_t rows, int hidden, int inter) {
   }
   return FMOE_OK;
 }
-// Up to so many rows the products of the gated block go to the kernel that splits the K range (gated_small.cu).
-int64_t gated_small_rows() {
-  const char* text = getenv("FUSED_CPP_GATED_SMALL_ROWS");
-  return text != nullptr ? atoll(text) : 128;
-}
+// Up to so many rows the products of the gated block go to the kernel that splits the K range (gated_small.cu).  7168 x 2048, forward, split / whole
+// K range: 64 rows 25.8 / 53 us (wide tiles), 256 rows 37.7 / 38.4, 512 rows 56.9 / 45.0; 4096 x 512: 256 rows 19.9 / 22.4, 512 rows 24.0 / 23.2.
+constexpr int64_t kGatedSmallRows = 256;
 bool vector_aligned(const void* pointer) { return reinterpret_cast<uintptr_t>(pointer) % 16 == 0; }
 int check_rows(const char* what, const char* name, const void* data, int64_t stride, int columns) {
   if (data == nullptr || !vector_aligned(data) || stride % 8 != 0 || stride < columns) {
@@ -1088,7 +1096,7 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
   if (!vector_aligned(derivatives)) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: derivatives must be 16-byte aligned", what);
   int* words = nullptr;
   cudaError_t error = fmoe::dense_status_words(&words);
-  if (error == cudaSuccess && rows <= gated_small_rows()) {
+  if (error == cudaSuccess && rows <= kGatedSmallRows) {
     error = fmoe::launch_gated_projection_small(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
                                                 swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(derivatives), words, stream, false);
     if (error == cudaSuccess) {
@@ -1132,7 +1140,7 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
   int* words = nullptr;
   cudaError_t error = fmoe::dense_status_words(&words);
   bool chained = false;
-  const bool small = rows <= gated_small_rows();
+  const bool small = rows <= kGatedSmallRows;
   if (error == cudaSuccess && needs_gate_up) {
     auto launch = small ? fmoe::launch_gated_backward_small : fmoe::launch_gated_backward;
     error = launch(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const float*>(derivatives), rows, hidden, inter,

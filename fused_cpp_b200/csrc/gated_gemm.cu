@@ -475,6 +475,22 @@ cudaError_t launch_tiles(Args args, const Operands* operands, int count, const i
 
 template <Epilogue kEpilogue, bool kAByK, bool kBByK>
 cudaError_t launch_form(const Args& args, const Operands* operands, int count, const int64_t* depth, cudaStream_t stream, bool chained) {
+  // Tiles of 256 columns, or of 128 where those end sooner: they take 0.55 of the time each (one pair brings 48 KB instead of 64 KB a K
+  // block, for half the products), and few or unlucky numbers of the wide ones leave pairs without work.  512 rows of 7168 x 2048
+  // (32 and 56 wide tiles): forward 58.0 -> 45.0 us; 1111 rows of 2880 x 1416: backward 66.8 -> 58.8; 2048 rows of 7168 x 2048 (128 and 224) stay
+  // wide: 131.9 us, 141.2 in narrow tiles.
+  constexpr int kWide = kEpilogue == Epilogue::kGated ? 128 : 256;  // output channels
+  int64_t wide = 0, narrow = 0;
+  for (int i = 0; i < count; ++i) {
+    const Problem& p = args.problem[i];
+    const int64_t m_tiles = (p.m + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta);
+    wide += m_tiles * ((p.n + kWide - 1) / kWide);
+    narrow += m_tiles * ((p.n + kWide / 2 - 1) / (kWide / 2));
+  }
+  const int64_t pairs = sm_count_of_current_device() / 2;
+  if ((narrow + pairs - 1) / pairs * 11 < (wide + pairs - 1) / pairs * 20) {
+    return launch_tiles<kEpilogue, kAByK, kBByK, 128>(args, operands, count, depth, stream, chained);
+  }
   return launch_tiles<kEpilogue, kAByK, kBByK, 256>(args, operands, count, depth, stream, chained);
 }
 

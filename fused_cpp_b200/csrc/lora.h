@@ -34,8 +34,13 @@ __device__ __forceinline__ int load_adapter_id(const LoraAdapters& adapters, int
 }
 #endif
 
-// Rows of x as int8 [rows, k_padded] with a scale each, zeros behind k; clears the status block of the call.
-cudaError_t launch_lora_quantize(const uint16_t* x, int64_t rows, int k, int k_padded, int8_t* q, float* scale, int* status, cudaStream_t stream);
+constexpr int kLoraListRows = 256;                   // rows of a list of adapters
+constexpr int kLoraListInts = kLoraListRows + 4;  // of a list in memory: the number of adapters in use by its rows, then their ids
+
+// Rows of x as int8 [rows, k_padded] with a scale each, zeros behind k; clears the status block of the call.  lists (nullable): the
+// adapters in use by every kLoraListRows rows.
+cudaError_t launch_lora_quantize(const uint16_t* x, int64_t rows, int k, int k_padded, int8_t* q, float* scale, int* status,
+                                 const LoraAdapters& adapters, int* lists, cudaStream_t stream);
 
 // t[plane][row][rank] = scaling[id] * (A[id] x[row]) for the rows that have an adapter (the others' are left as they are), as `planes` bf16
 // terms.  A programmatic dependent of the kernel in front, of which it needs nothing.
@@ -56,8 +61,11 @@ struct LoraGemmArgs {
   LoraAdapters adapters;
   const uint16_t* t;
   int planes;
+  const int* lists;  // of launch_lora_quantize
   int* status;
 };
 cudaError_t launch_lora_gemm(const LoraGemmArgs& args, cudaStream_t stream);
+// The same over many rows, by lists.
+cudaError_t launch_lora_pair_gemm(const LoraGemmArgs& args, cudaStream_t stream);
 
 }  // namespace fmoe

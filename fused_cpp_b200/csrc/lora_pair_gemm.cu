@@ -1,0 +1,590 @@
+// Dense W8A8 linear with the low-rank adapters of many requests over many rows (lora_gemm.cu has it over few):
+//   out[row, n] = (acc * row scale) * channel scale (+ bias[n]) + sum over r of t[row, r] B[a, n, r],   acc = Xq W^T.
+//
+// Two CTAs of a cluster drive one tile of 256 rows x 256 (or 128) channels (cta_group::2, gated_gemm.cu has the layout): rows are the lanes of tensor memory, channels its
+// columns, two accumulators take turns.  Both products end in the same accumulator:
+//   1. The int32 sums of the quantised product are complete: the epilogue warps turn them into the fp32 result of the base projection in place.
+//   2. The adapters' product is accumulated onto it by bf16 MMAs: for every adapter that rows of the tile use, a K block of [t of its rows,
+//      zeros for the others] x B[a]^T for each 64 ranks.  An own accumulator for it would leave tensor memory for one tile, and its epilogue no product to run under.
+//   3. The epilogue stores the accumulator.
+// Between 1 and 2 the tensor pipe works on the next tile: the adapters' K blocks of a tile stand behind the first kDelay K blocks of the next one, in the
+// order of every role's loop.  A tile whose rows have no adapter goes from 1 to 3.
+// The lists of adapters, one for each 256 rows, come from the quantiser's launch.  Four warps of each CTA write the masked coefficients of its 128 rows
+// where the token tile would lie.
+#include <cuda.h>
+#include <stdlib.h>
+
+#include "common.cuh"
+#include "gated.cuh"
+#include "kernels.h"
+#include "lora.h"
+#include "pair_ptx.cuh"
+#include "ptx.cuh"
+
+namespace fmoe {
+
+namespace {
+
+constexpr int kRowsPerCta = 128;
+constexpr int kBlockKBytes = 128;
+constexpr int kUmmaKBytes = 32;
+constexpr int kEpilogueWarps = 8;   // warps 2 .. 9
+constexpr int kWriterWarps = 4;     // warps 10 .. 13
+constexpr int kThreads = 64 + 32 * (kEpilogueWarps + kWriterWarps);
+constexpr int kTmemColumns = 512;
+constexpr int kStagingBytes = 32 * 128;
+constexpr int kMaxStages = 8;
+constexpr int kTileGroup = 8;  // row tiles that are walked together (gated_gemm.cu)
+constexpr int kDelay = 4;      // K blocks of the next tile in front of a tile's adapters: what the epilogue takes for step 1
+
+template <int kTileN>
+struct TileConfig {
+  static constexpr int kABytes = kRowsPerCta * kBlockKBytes;
+  static constexpr int kBRows = kTileN / 2;  // of one CTA
+  static constexpr int kBBytes = kBRows * kBlockKBytes;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = 184 * 1024 / kStageBytes < kMaxStages ? 184 * 1024 / kStageBytes : kMaxStages;
+  static constexpr size_t kSmemBytes = 1024 + static_cast<size_t>(kStages) * kStageBytes + kEpilogueWarps * kStagingBytes + 6144;
+  static_assert(kSmemBytes <= 227 * 1024, "a CTA has 227 KB of shared memory");
+};
+
+struct Control {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t vacant[kMaxStages];        // the producer leaves the stage's token tile to the coefficients
+  uint64_t coefficients[kMaxStages];  // leader: both CTAs' coefficients of the stage are written
+  uint64_t base_full[2];
+  uint64_t converted[2];
+  uint64_t all_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  volatile int abort_flag;
+  alignas(16) float channel_scale[2][256];
+  alignas(16) float channel_bias[2][256];
+};
+static_assert(sizeof(Control) <= 6144, "control block exceeds its shared-memory reservation");
+
+struct Args {
+  LoraGemmArgs g;
+  int k_blocks, m_tiles, n_tiles, rank_blocks;
+  int tma_store;
+};
+
+struct Tile {
+  int m, n;
+};
+
+__device__ __forceinline__ Tile tile_at(const Args& args, int index) {
+  const int per_group = kTileGroup * args.n_tiles;
+  const int group = index / per_group;
+  const int rest = index - group * per_group;
+  const int group_m = min(kTileGroup, args.m_tiles - group * kTileGroup);
+  Tile t;
+  t.n = rest / group_m;
+  t.m = group * kTileGroup + rest - t.n * group_m;
+  return t;
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar_cluster_address, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      :
+      : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_address), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t smem_src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               :
+               : "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(x), "r"(y)
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t address, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(address),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
+      "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+
+// Arrival on an mbarrier of either CTA that publishes what this warp wrote (shared memory of its CTA, tensor memory), and the bounded wait that
+// takes it over: writer and reader are in different CTAs.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_address) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(done)
+      : "r"(ptx::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ void mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int site) {
+  if (mbar_try_wait_cluster(bar, parity)) return;
+  const unsigned long long start = ptx::global_timer_ns();
+  while (true) {
+    for (int spin = 0; spin < 64; ++spin) {
+      if (mbar_try_wait_cluster(bar, parity)) return;
+    }
+    if (*abort_flag) return;
+    if (ptx::global_timer_ns() - start > ptx::kWaitLimitNs) {
+      *abort_flag = 1;
+      raise_error(status, FMOE_ERR_DEVICE_WAIT, static_cast<int>(blockIdx.x), site);
+      return;
+    }
+  }
+}
+
+// The list of the adapters in use by 256 rows: their number, then their ids.
+__device__ __forceinline__ const int* adapter_list(const Args& args, int m_tile) { return args.g.lists + static_cast<int64_t>(m_tile) * kLoraListInts; }
+
+template <int kTileN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap b_map,
+                      const __grid_constant__ CUtensorMap out_map, const __grid_constant__ Args args) {
+  using Cfg = TileConfig<kTileN>;
+  constexpr int kStages = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* const staging_base = smem + static_cast<size_t>(kStages) * Cfg::kStageBytes;
+  Control* ctl = reinterpret_cast<Control*>(staging_base + kEpilogueWarps * kStagingBytes);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_cta_rank();
+  const bool leader = cta == 0;
+  int* status = args.g.status;
+  const int tiles = args.m_tiles * args.n_tiles;
+  const int first_tile = static_cast<int>(blockIdx.x >> 1);
+  const int tile_stride = static_cast<int>(gridDim.x >> 1);
+  const int k_blocks = args.k_blocks;
+  const int outer = args.rank_blocks * args.g.planes;  // K blocks of one adapter
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&ctl->full[s], 1);
+      ptx::mbar_init(&ctl->empty[s], 1);
+      ptx::mbar_init(&ctl->vacant[s], 1);
+      ptx::mbar_init(&ctl->coefficients[s], 2 * kWriterWarps);  // of both CTAs
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(&ctl->base_full[b], 1);
+      ptx::mbar_init(&ctl->converted[b], 2 * kEpilogueWarps);
+      ptx::mbar_init(&ctl->all_full[b], 1);
+      ptx::mbar_init(&ctl->acc_empty[b], 2 * kEpilogueWarps);
+    }
+    ctl->abort_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&ctl->tmem_base, kTmemColumns);
+    tmem_relinquish_pair();
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers are initialised before anything signals them
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  volatile int* abort_flag = &ctl->abort_flag;
+  const uint32_t smem_base = ptx::smem_u32(smem);
+  ptx::grid_dependency_wait();
+  auto slots_of = [&](int m_tile) { return __shfl_sync(0xffffffffu, __ldcg(adapter_list(args, m_tile)), 0); };
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs; the whole warp walks the loop, one elected lane issues) ----------------
+    const bool issuer = ptx::elect_one();
+    const uint32_t full_leader0 = map_to_cta(ptx::smem_u32(&ctl->full[0]), 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    auto advance = [&]() {
+      ++issued;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    };
+    auto load_adapters = [&](const Tile& tile, int slots) {
+      const int* const list = adapter_list(args, tile.m) + 1;
+      for (int o = 0; o < outer; ++o) {
+        for (int slot = 0; slot < slots; ++slot) {
+          const int adapter = __ldcg(list + slot);
+          ptx::mbar_wait(&ctl->empty[stage], phase ^ 1u, abort_flag, status, 71);
+          if (issuer) {
+            ptx::mbar_arrive(&ctl->vacant[stage]);
+            if (leader) ptx::mbar_arrive_expect_tx(&ctl->full[stage], 2 * Cfg::kBBytes);
+            tma_load_3d_pair(smem_base + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes, &b_map, full_leader0 + 8u * static_cast<uint32_t>(stage),
+                             o / args.g.planes * kLoraRankBlock, tile.n * kTileN + Cfg::kBRows * static_cast<int>(cta), adapter);
+          }
+          advance();
+        }
+      }
+    };
+    Tile before = {0, 0};
+    int slots_before = 0;
+    for (int index = first_tile; index < tiles; index += tile_stride) {
+      const Tile tile = tile_at(args, index);
+      const int slots = slots_of(tile.m);
+      const int a_row = tile.m * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta);
+      const int b_row = tile.n * kTileN + Cfg::kBRows * static_cast<int>(cta);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (kb == kDelay) load_adapters(before, slots_before);
+        ptx::mbar_wait(&ctl->empty[stage], phase ^ 1u, abort_flag, status, 72);
+        if (issuer) {
+          const uint32_t dst = smem_base + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+          const uint32_t bar = full_leader0 + 8u * static_cast<uint32_t>(stage);
+          if (leader) ptx::mbar_arrive_expect_tx(&ctl->full[stage], 2 * Cfg::kStageBytes);
+          tma_load_2d_pair(dst, &token_map, bar, kb * kBlockKBytes, a_row);
+          tma_load_2d_pair(dst + Cfg::kABytes, &weight_map, bar, kb * kBlockKBytes, b_row);
+        }
+        advance();
+      }
+      if (k_blocks <= kDelay) load_adapters(before, slots_before);
+      before = tile;
+      slots_before = slots;
+    }
+    load_adapters(before, slots_before);
+    if (leader) {
+      // Drain: the leader's full barriers count both CTAs' bytes, so this also covers the follower's loads.
+      const int pending = issued < kStages ? issued : kStages;
+      for (int back = 0; back < pending; ++back) {
+        int s = stage - 1 - back;
+        uint32_t p = phase;
+        if (s < 0) {
+          s += kStages;
+          p ^= 1u;
+        }
+        const unsigned long long start = ptx::global_timer_ns();
+        while (!ptx::mbar_try_wait(&ctl->full[s], p)) {
+          if (ptx::global_timer_ns() - start > ptx::kWaitLimitNs) break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader CTA only) ----------------
+    if (leader) {
+      const bool issuer = ptx::elect_one();
+      constexpr uint32_t kIdesc = ptx::make_instr_desc(true, 2 * kRowsPerCta, kTileN);
+      constexpr uint32_t kIdescAdapters = ptx::make_instr_desc(false, 2 * kRowsPerCta, kTileN);
+      const uint32_t desc_hi = static_cast<uint32_t>(1024 >> 4) | (1u << 14) | (2u << 29);
+      const uint32_t stage0 = ((smem_base & 0x3ffffu) >> 4) | (1u << 16);
+      auto both = [&](uint64_t* bar, int which) {
+        const uint32_t here = ptx::smem_u32(bar + which);
+        tcgen05_commit_pair(map_to_cta(here, 0));
+        tcgen05_commit_pair(map_to_cta(here, 1));
+      };
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t written = 0;             // stages, one bit each, whose coefficients barrier is in its odd phase
+      uint32_t converted_phase = 0;     // one bit for each accumulator
+      auto advance = [&]() {
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      };
+      auto multiply_adapters = [&](int slots, uint32_t buffer) {
+        if (slots == 0) return;
+        mbar_wait_cluster(&ctl->converted[buffer], (converted_phase >> buffer) & 1u, abort_flag, status, 73);
+        converted_phase ^= 1u << buffer;
+        for (int o = 0; o < outer; ++o) {
+          const int steps = (min(kLoraRankBlock, args.g.adapters.rank - o / args.g.planes * kLoraRankBlock) + 15) >> 4;
+          for (int slot = 0; slot < slots; ++slot) {
+            ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 74);
+            mbar_wait_cluster(&ctl->coefficients[stage], (written >> stage) & 1u, abort_flag, status, 75);
+            written ^= 1u << stage;
+            ptx::tcgen05_fence_after();
+            if (issuer) {
+              const uint32_t a_lo = stage0 + static_cast<uint32_t>(stage) * (Cfg::kStageBytes >> 4);
+              for (int ks = 0; ks < steps; ++ks) {
+                umma_pair<false>(tmem_base + kTileN * buffer, a_lo + 2u * ks, a_lo + (Cfg::kABytes >> 4) + 2u * ks, desc_hi, kIdescAdapters, 1u);
+              }
+              both(ctl->empty, stage);
+            }
+            advance();
+          }
+        }
+        if (issuer) both(ctl->all_full, buffer);
+      };
+      int local = 0;
+      int slots_before = 0;
+      for (int index = first_tile; index < tiles; index += tile_stride, ++local) {
+        const int slots = slots_of(tile_at(args, index).m);
+        const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
+        const uint32_t use = static_cast<uint32_t>(local) >> 1;
+        ptx::mbar_wait(&ctl->acc_empty[buffer], (use & 1u) ^ 1u, abort_flag, status, 76);
+        ptx::tcgen05_fence_after();
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (kb == kDelay) multiply_adapters(slots_before, buffer ^ 1u);
+          ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 77);
+          ptx::tcgen05_fence_after();
+          if (issuer) {
+            const uint32_t a_lo = stage0 + static_cast<uint32_t>(stage) * (Cfg::kStageBytes >> 4);
+#pragma unroll
+            for (uint32_t ks = 0; ks < kBlockKBytes / kUmmaKBytes; ++ks) {
+              umma_pair<true>(tmem_base + kTileN * buffer, a_lo + 2u * ks, a_lo + (Cfg::kABytes >> 4) + 2u * ks, desc_hi, kIdesc, kb > 0 || ks > 0 ? 1u : 0u);
+            }
+            both(ctl->empty, stage);
+          }
+          advance();
+        }
+        if (issuer) both(ctl->base_full, buffer);
+        if (k_blocks <= kDelay) multiply_adapters(slots_before, buffer ^ 1u);
+        slots_before = slots;
+      }
+      if (local > 0) multiply_adapters(slots_before, static_cast<uint32_t>(local - 1) & 1u);
+    }
+  } else if (warp < 2 + kEpilogueWarps) {
+    // ---------------- epilogue (both CTAs) ----------------
+    const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id % 4
+    const int chunk_first = (warp - 2) >> 2;
+    constexpr int kChunkStep = kEpilogueWarps / 4;
+    constexpr int kChunks = kTileN / 64;
+    const int thread = static_cast<int>(threadIdx.x) - 64;  // of 256
+    uint8_t* const staging = staging_base + (warp - 2) * kStagingBytes;
+    const uint32_t acc_lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t acc_empty_leader = map_to_cta(ptx::smem_u32(&ctl->acc_empty[0]), 0);
+    const uint32_t converted_leader = map_to_cta(ptx::smem_u32(&ctl->converted[0]), 0);
+    const int n = args.g.n;
+    uint32_t all_phase = 0;  // one bit for each accumulator
+    int local = 0;
+    for (int index = first_tile; index < tiles; index += tile_stride, ++local) {
+      const Tile tile = tile_at(args, index);
+      const int slots = slots_of(tile.m);
+      const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
+      const uint32_t use = static_cast<uint32_t>(local) >> 1;
+      const int warp_row = tile.m * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + quarter * 32;
+      const int64_t row = static_cast<int64_t>(warp_row) + lane;
+      const bool row_ok = row < args.g.rows;
+      const int n0 = tile.n * kTileN;
+      const uint32_t acc = acc_lane_base + kTileN * buffer;
+      // This tile's channel values; the buffer was last read two tiles ago, in front of the barrier of the tile in between.
+      const float* const scales = ctl->channel_scale[buffer];
+      const float* const biases = ctl->channel_bias[buffer];
+      if (thread < kTileN) {
+        const bool exists = n0 + thread < n;
+        ctl->channel_scale[buffer][thread] = exists ? __ldcg(args.g.w_scale + n0 + thread) : 0.0f;
+        ctl->channel_bias[buffer][thread] = exists && args.g.bias != nullptr ? __ldcg(args.g.bias + n0 + thread) : 0.0f;
+      }
+      const float row_scale = row_ok ? __ldcg(args.g.a_scale + row) : 0.0f;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory");
+      auto dequantise = [&](uint32_t (&bits)[32], int column) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 s = *reinterpret_cast<const float4*>(scales + column + 4 * q);
+          const float4 b = *reinterpret_cast<const float4*>(biases + column + 4 * q);
+          const float ss[4] = {s.x, s.y, s.z, s.w}, bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float value = dequantize(static_cast<int>(bits[4 * q + j]), row_scale, ss[j], FMOE_NUMERICS_TORCHREF);
+            bits[4 * q + j] = __float_as_uint(__fadd_rn(value, bb[j]));
+          }
+        }
+      };
+      ptx::mbar_wait(&ctl->base_full[buffer], use & 1u, abort_flag, status, 78);
+      ptx::tcgen05_fence_after();
+      if (slots > 0) {
+        for (int chunk = chunk_first; chunk < kChunks; chunk += kChunkStep) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t bits[32];
+            tmem_ld_x32(acc + 64u * chunk + 32u * half, bits);
+            ptx::tmem_ld_wait();
+            dequantise(bits, 64 * chunk + 32 * half);
+            tmem_st_x32(acc + 64u * chunk + 32u * half, bits);
+          }
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        ptx::tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_release_cluster(converted_leader + 8u * buffer);
+        ptx::mbar_wait(&ctl->all_full[buffer], (all_phase >> buffer) & 1u, abort_flag, status, 79);
+        all_phase ^= 1u << buffer;
+        ptx::tcgen05_fence_after();
+      }
+      for (int chunk = chunk_first; chunk < kChunks; chunk += kChunkStep) {
+        const int col = n0 + 64 * chunk;
+        if (warp_row >= args.g.rows || col >= n) break;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t bits[32];
+          tmem_ld_x32(acc + 64u * chunk + 32u * half, bits);
+          ptx::tmem_ld_wait();
+          if (slots == 0) dequantise(bits, 64 * chunk + 32 * half);
+          const int first = col + 32 * half;
+          if (args.tma_store) {
+            if (!args.g.out_bf16 || half == 0) {
+              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the block before has been read out of shared memory
+              __syncwarp();
+            }
+            auto put = [&](int piece, uint4 value) { *reinterpret_cast<uint4*>(staging + lane * 128 + ((piece ^ (lane & 7)) << 4)) = value; };
+            if (args.g.out_bf16) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                uint32_t words[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) words[j] = pack_bf16(__uint_as_float(bits[8 * q + 2 * j]), __uint_as_float(bits[8 * q + 2 * j + 1]));
+                put(4 * half + q, make_uint4(words[0], words[1], words[2], words[3]));
+              }
+            } else {
+#pragma unroll
+              for (int q = 0; q < 8; ++q) put(q, make_uint4(bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]));
+            }
+            if (!args.g.out_bf16 || half == 1) {
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0 && (args.g.out_bf16 || first < n)) {
+                tma_store_2d(&out_map, ptx::smem_u32(staging), args.g.out_bf16 ? col : first, warp_row);
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              }
+            }
+          } else if (row_ok) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (first + j >= n) break;
+              const float value = __uint_as_float(bits[j]);
+              if (args.g.out_bf16) {
+                static_cast<uint16_t*>(args.g.out)[row * n + first + j] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
+              } else {
+                static_cast<float*>(args.g.out)[row * n + first + j] = value;
+              }
+            }
+          }
+          __syncwarp();  // the next tensor-memory load wants the whole warp
+        }
+      }
+      ptx::tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * buffer);
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // every block has arrived
+    __syncwarp();
+  } else {
+    // ---------------- masked coefficients: a thread for each of the CTA's rows ----------------
+    const int row_in_cta = static_cast<int>(threadIdx.x) - 64 - 32 * kEpilogueWarps;
+    const uint32_t coefficients_leader = map_to_cta(ptx::smem_u32(&ctl->coefficients[0]), 0);
+    const int rank_padded = lora_rank_padded(args.g.adapters.rank);
+    int stage = 0;
+    uint32_t used = 0;  // stages, one bit each, whose vacant barrier is in its odd phase
+    auto skip = [&](int blocks) { stage = (stage + blocks) % kStages; };
+    auto write = [&](const Tile& tile, int slots) {
+      if (slots == 0) return;
+      const int* const list = adapter_list(args, tile.m) + 1;
+      const int64_t row = static_cast<int64_t>(tile.m) * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + row_in_cta;
+      const int id = row < args.g.rows ? load_adapter_id(args.g.adapters, row) : -1;
+      for (int o = 0; o < outer; ++o) {
+        const int rank0 = o / args.g.planes * kLoraRankBlock;
+        const int pieces = 2 * ((min(kLoraRankBlock, args.g.adapters.rank - rank0) + 15) >> 4);
+        const uint16_t* const from = args.g.t + (o % args.g.planes * args.g.rows + row) * rank_padded + rank0;
+        uint4 value[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          value[p] = make_uint4(0, 0, 0, 0);
+          if (id >= 0 && p < pieces) value[p] = __ldcg(reinterpret_cast<const uint4*>(from) + p);
+        }
+        for (int slot = 0; slot < slots; ++slot) {
+          const bool mine = id == __ldcg(list + slot);
+          ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 80);
+          used ^= 1u << stage;
+          uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + row_in_cta * 128;
+#pragma unroll
+          for (int p = 0; p < 8; ++p) {
+            if (p < pieces) *reinterpret_cast<uint4*>(to + ((p ^ (row_in_cta & 7)) << 4)) = mine ? value[p] : make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive_release_cluster(coefficients_leader + 8u * static_cast<uint32_t>(stage));
+          skip(1);
+        }
+      }
+    };
+    Tile before = {0, 0};
+    int slots_before = 0;
+    bool any = false;
+    for (int index = first_tile; index < tiles; index += tile_stride) {
+      const Tile tile = tile_at(args, index);
+      const int slots = slots_of(tile.m);
+      if (k_blocks <= kDelay) {
+        skip(k_blocks);
+        write(before, slots_before);
+      } else {
+        skip(kDelay);
+        write(before, slots_before);
+        skip(k_blocks - kDelay);
+      }
+      before = tile;
+      slots_before = slots;
+      any = true;
+    }
+    if (any) write(before, slots_before);
+  }
+
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while its peer may still signal its barriers or read its operands
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tcgen05_fence_after();
+    tmem_dealloc_pair(tmem_base, kTmemColumns);
+  }
+}
+
+template <int kTileN>
+cudaError_t launch(Args args, cudaStream_t stream) {
+  using Cfg = TileConfig<kTileN>;
+  auto kernel = lora_pair_gemm_kernel<kTileN>;
+  static PerDeviceOnce configured;
+  const int device = current_device_ordinal();
+  if (configured.needed(device)) {
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg::kSmemBytes));
+    if (error != cudaSuccess) return error;
+    configured.mark(device);
+  }
+  const LoraGemmArgs& g = args.g;
+  const uint64_t k = static_cast<uint64_t>(g.k_padded);
+  CUtensorMap maps[4];
+  if (!make_sw128_map(&maps[0], g.xq, true, static_cast<uint64_t>(g.rows), k, kRowsPerCta) ||
+      !make_sw128_map(&maps[1], g.weight, true, static_cast<uint64_t>(g.n), k, Cfg::kBRows) ||
+      !make_sw128_map_3d(&maps[2], g.adapters.b, g.adapters.rank, g.n, g.adapters.count, g.adapters.b_stride, Cfg::kBRows)) {
+    return cudaErrorInvalidValue;
+  }
+  args.tma_store = static_cast<int64_t>(g.n) * (g.out_bf16 ? 2 : 4) % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
+  if (!args.tma_store) {
+    maps[3] = maps[0];
+  } else if (!make_store_map(&maps[3], g.out, !g.out_bf16, static_cast<uint64_t>(g.n), 1, static_cast<uint64_t>(g.rows))) {
+    return cudaErrorInvalidValue;
+  }
+  args.n_tiles = (g.n + kTileN - 1) / kTileN;
+  const int64_t total = static_cast<int64_t>(args.m_tiles) * args.n_tiles;
+  if (total > (1ll << 30)) return cudaErrorInvalidValue;
+  int64_t pairs = sm_count_of_current_device() / 2;
+  if (pairs > total) pairs = total;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(2 * pairs)), kThreads, Cfg::kSmemBytes, stream, true, maps[0], maps[1], maps[2], maps[3], args);
+}
+
+}  // namespace
+
+cudaError_t launch_lora_pair_gemm(const LoraGemmArgs& g, cudaStream_t stream) {
+  Args args = {};
+  args.g = g;
+  args.k_blocks = (g.k_padded + kBlockKBytes - 1) / kBlockKBytes;
+  args.rank_blocks = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  args.m_tiles = static_cast<int>((g.rows + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta));
+  const int64_t pairs = sm_count_of_current_device() / 2;
+  const int64_t wide = static_cast<int64_t>(args.m_tiles) * ((g.n + 255) / 256), narrow = static_cast<int64_t>(args.m_tiles) * ((g.n + 127) / 128);
+  const char* text = getenv("GT");
+  if (text != nullptr ? text[0] == '1' : (narrow + pairs - 1) / pairs * 11 < (wide + pairs - 1) / pairs * 20) return launch<128>(args, stream);
+  return launch<256>(args, stream);
+}
+
+}  // namespace fmoe

@@ -317,12 +317,45 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
 // Rows of x as int8 with a scale each: scale = amax * (1/127) in 32 bits (1 for a row of zeros), q = clamp(rint(x / scale), -128, 127).
 constexpr int kQuantThreads = 256;
 
+// The adapters in use by 256 rows, each once, in the order of their first rows.
+__device__ void list_adapters(const ShrinkArgs& args, int64_t tile, int* lists) {
+  static_assert(kQuantThreads == kLoraListRows, "a thread for each row");
+  __shared__ alignas(16) int ids[kLoraListRows];
+  __shared__ int warp_count[kLoraListRows / 32];
+  const int i = threadIdx.x;
+  const int64_t row = tile * kLoraListRows + i;
+  const int mine = row < args.rows ? load_adapter_id(args.adapters, row) : -1;
+  ids[i] = mine;
+  __syncthreads();
+  bool first = mine >= 0;
+  for (int j = 0; first && j < i; j += 4) {
+    const int4 others = *reinterpret_cast<const int4*>(&ids[j]);
+    first = !(others.x == mine || (others.y == mine && j + 1 < i) || (others.z == mine && j + 2 < i) || (others.w == mine && j + 3 < i));
+  }
+  const unsigned firsts = __ballot_sync(0xffffffffu, first);
+  if ((i & 31) == 0) warp_count[i >> 5] = __popc(firsts);
+  __syncthreads();
+  int slot = __popc(firsts & ((1u << (i & 31)) - 1)), slots = 0;
+  for (int w = 0; w < kLoraListRows / 32; ++w) {
+    if (w < (i >> 5)) slot += warp_count[w];
+    slots += warp_count[w];
+  }
+  int* const list = lists + tile * kLoraListInts;
+  if (i == 0) list[0] = slots;
+  if (first) list[1 + slot] = mine;
+}
+
 template <bool kVector>
 __global__ void __launch_bounds__(kQuantThreads)
-lora_quantize_kernel(const uint16_t* __restrict__ x, int cols, int cols_padded, int8_t* __restrict__ q, float* __restrict__ scale_out, int* status) {
+lora_quantize_kernel(const uint16_t* __restrict__ x, int cols, int cols_padded, int8_t* __restrict__ q, float* __restrict__ scale_out, int* status,
+                     const __grid_constant__ ShrinkArgs args, int* lists) {
   ptx::launch_dependents();
   __shared__ float smem[32];
   if (blockIdx.x == 0 && threadIdx.x < kStatusWords) status[threadIdx.x] = 0;
+  if (blockIdx.x >= args.rows) {
+    list_adapters(args, static_cast<int64_t>(blockIdx.x) - args.rows, lists);
+    return;
+  }
   const int64_t row = blockIdx.x;
   const uint16_t* const src = x + row * cols;
   float local = 0.0f;
@@ -345,10 +378,15 @@ lora_quantize_kernel(const uint16_t* __restrict__ x, int cols, int cols_padded, 
 
 }  // namespace
 
-cudaError_t launch_lora_quantize(const uint16_t* x, int64_t rows, int k, int k_padded, int8_t* q, float* scale, int* status, cudaStream_t stream) {
+cudaError_t launch_lora_quantize(const uint16_t* x, int64_t rows, int k, int k_padded, int8_t* q, float* scale, int* status,
+                                 const LoraAdapters& adapters, int* lists, cudaStream_t stream) {
+  ShrinkArgs args = {};
+  args.rows = rows;
+  args.adapters = adapters;
+  const int64_t tiles = lists != nullptr ? (rows + kLoraListRows - 1) / kLoraListRows : 0;
   const bool vector = k % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   auto kernel = vector ? lora_quantize_kernel<true> : lora_quantize_kernel<false>;
-  kernel<<<static_cast<unsigned>(rows), kQuantThreads, 0, stream>>>(x, k, k_padded, q, scale, status);
+  kernel<<<static_cast<unsigned>(rows + tiles), kQuantThreads, 0, stream>>>(x, k, k_padded, q, scale, status, args, lists);
   return cudaGetLastError();
 }
 
