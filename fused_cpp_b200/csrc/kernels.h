@@ -292,8 +292,10 @@ inline cudaError_t launch_streaming(void (*kernel)(Params...), dim3 grid, unsign
 // 2-D tensor [rows, k] with 128-byte-swizzled boxes of {128 bytes of a row, box_rows} (umma_gemm.cu); row_stride: elements from a row
 // to the next, 0 = k.
 bool make_sw128_map(CUtensorMap* map, const void* base, bool int8, uint64_t rows, uint64_t k, uint32_t box_rows, uint64_t row_stride = 0);
-// 3-D bf16 tensor [planes, rows, columns], row_stride elements from a row to the next, boxes of {128 bytes of a row, box_rows} of one plane.
-bool make_sw128_map_3d(CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows, uint64_t planes, uint64_t row_stride, uint32_t box_rows);
+// 3-D bf16 tensor [planes, rows, columns], row_stride elements from a row to the next, boxes of {box_columns (16, 32 or 64), box_rows} of one
+// plane in the swizzle of their row length.
+bool make_adapter_map(CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows, uint64_t planes, uint64_t row_stride, uint32_t box_columns,
+                      uint32_t box_rows);
 
 // Result rows [rows, columns] (sides = 1) or [rows, sides, columns] of bf16 or fp32, for stores of swizzled boxes of {128 bytes, 32 rows} of a side.
 bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows);

@@ -16,6 +16,16 @@ __host__ __device__
 #endif
 constexpr int lora_rank_padded(int rank) { return (rank + 15) / 16 * 16; }
 
+// Adapters of low rank share a K block of their product: the block is 128 bytes of coefficients a row, and up to `adapters` tiles of B that are `ranks` wide each.
+struct LoraBlock {
+  int ranks;     // of an adapter in a block: 16, 32 or 64
+  int adapters;  // of a block: 4, 2 or 1
+};
+inline LoraBlock lora_block(int rank) {
+  const int ranks = rank <= 16 ? 16 : rank <= 32 ? 32 : kLoraRankBlock;
+  return LoraBlock{ranks, kLoraRankBlock / ranks};
+}
+
 struct LoraAdapters {
   const uint16_t* a;  // bf16 [count, rank, a_stride], a_stride >= k a multiple of 8, zeros behind k
   const uint16_t* b;  // bf16 [count, n, b_stride], b_stride >= rank a multiple of 8, zeros behind rank
@@ -27,6 +37,11 @@ struct LoraAdapters {
 };
 
 #ifdef __CUDACC__
+// High word of the shared-memory descriptor of a K-major tile whose rows are `ranks` bf16 long, in the swizzle of that row length (what a TMA load of
+// such a box writes): groups of eight rows are 16 ranks bytes apart; layout types 6, 4, 2 = swizzles of 32, 64, 128 bytes.
+__device__ __forceinline__ uint32_t lora_desc_hi(int ranks) {
+  return static_cast<uint32_t>(ranks) | (1u << 14) | ((ranks == 16 ? 6u : ranks == 32 ? 4u : 2u) << 29);
+}
 // (Through L2: the kernels read ids in front of their wait, see launch_chained.)
 __device__ __forceinline__ int load_adapter_id(const LoraAdapters& adapters, int64_t row) {
   const int64_t id = adapters.ids_are_64 ? __ldcg(static_cast<const long long*>(adapters.ids) + row) : __ldcg(static_cast<const int*>(adapters.ids) + row);

@@ -3,8 +3,8 @@
 // with the coefficients t of lora_shrink.cu.  The kernel of dense_gemm.cu (128 output channels of a cluster of `parts` CTAs that split the K
 // range; their int32 sums meet in distributed shared memory) with the adapters' product beside it, in a second accumulator of tensor memory:
 //   * Rows of a tile may have any adapters in any order.  For each adapter in use by the rows, [t of its rows, zeros for the others] x B[a]^T
-//     is a K block of bf16 MMAs: 64 ranks are one 128-byte row as the weights' K blocks are, B[a] comes by the same ring of
-//     stages, and a warp writes the masked coefficients where the token tile would lie.  A row's sum has only its own adapter's products and exact
+//     is one of bf16 MMAs: a K block of 128-byte rows, as the weights' are, holds 64 ranks of one adapter or two or four adapters of up to 32 or 16
+//     ranks, B[a] comes by the same ring of stages, and four warps write the masked coefficients where the token tile would lie.  A row's sum has only its own adapter's products and exact
 //     zeros in it (adapters are finite by contract), whatever its neighbours ask for.
 //   * A CTA finishes the rows [part * R, part * R + R) of its tile (R = rows / parts): it multiplies the adapters of those rows alone, so that
 //     nothing of that product is exchanged, and every adapter's channels are read by the CTAs whose rows use it.
@@ -59,7 +59,7 @@ struct LoraControl {
   alignas(16) float row_scale[kTileRows];
   alignas(16) float channel_scale[kBlockM];
   alignas(16) float channel_bias[kBlockM];
-  int id[kTileRows];
+  int slot[kTileRows];  // of the own rows: place of their adapter in the list, -1 = none
   int slot_adapter[kTileRows];
 };
 static_assert(sizeof(LoraControl) <= 4096, "control block exceeds its shared-memory reservation");
@@ -67,6 +67,7 @@ static_assert(sizeof(LoraControl) <= 4096, "control block exceeds its shared-mem
 struct KernelArgs {
   LoraGemmArgs g;
   int row_tiles, k_blocks, parts, vector_store, rank_blocks;
+  LoraBlock block;
 };
 
 __device__ __forceinline__ void cluster_sync() {
@@ -155,15 +156,17 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
     for (int base = 0; base < own; base += 32) {
       const int i = base + lane;
       const int id = i < own ? load_adapter_id(args.g.adapters, row0 + own_first + i) : -1;
-      if (i < own) ctl->id[i] = id;
       const unsigned same = __match_any_sync(0xffffffffu, id);
-      bool first = id >= 0 && (same & ((1u << lane) - 1)) == 0;
-      __syncwarp();
-      if (first) {
-        for (int j = 0; j < slots; ++j) first = first && ctl->slot_adapter[j] != id;
+      int slot = -1;  // of an earlier row's
+      if (id >= 0) {
+        for (int j = 0; j < slots; ++j) slot = ctl->slot_adapter[j] == id ? j : slot;
       }
+      const bool first = id >= 0 && slot < 0 && (same & ((1u << lane) - 1)) == 0;
       const unsigned firsts = __ballot_sync(0xffffffffu, first);
       if (first) ctl->slot_adapter[slots + __popc(firsts & ((1u << lane) - 1))] = id;
+      // A row whose adapter appears first in these 32 has the slot of that first row.
+      if (id >= 0 && slot < 0) slot = slots + __popc(firsts & ((1u << (__ffs(same) - 1)) - 1));
+      if (i < own) ctl->slot[i] = slot;
       slots += __popc(firsts);
       __syncwarp();
     }
@@ -183,8 +186,11 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
   }
   ptx::mbar_wait(&ctl->listed, 0, abort_flag, status, 56);
   const int slots = __shfl_sync(0xffffffffu, ctl->slots, 0);
-  // K blocks of the adapters' product: for every plane of every 64 ranks, the adapters one after the other.
-  const int extra = slots * args.rank_blocks * args.g.planes;
+  // K blocks of the adapters' product: for every plane of every 64 ranks, the adapters one after the other, per_block in a block.
+  const int per_block = args.block.adapters;
+  const int slot_blocks = (slots + per_block - 1) / per_block;
+  const uint32_t adapter_bytes = static_cast<uint32_t>(kBlockM) * args.block.ranks * 2;  // of one adapter's tile
+  const int extra = slot_blocks * args.rank_blocks * args.g.planes;
   const int all = count + extra;
 
   if (warp == 0) {
@@ -210,10 +216,14 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
           ptx::tma_load_2d(stage_base + kWeightBytes, &token_map, &ctl->full[stage], (kb_begin + i) * kBlockKBytes, static_cast<int>(row0));
         } else {
           const int u = i - count;
-          const int rank_block = u / slots / args.g.planes;
+          const int rank_block = u / slot_blocks / args.g.planes;
+          const int slot = u % slot_blocks * per_block;
+          const int here = min(per_block, slots - slot);
           ptx::mbar_arrive(&ctl->vacant[stage]);
-          ptx::mbar_arrive_expect_tx(&ctl->full[stage], kWeightBytes);
-          tma_load_3d(stage_base, &b_map, &ctl->full[stage], rank_block * kLoraRankBlock, n0, ctl->slot_adapter[u % slots]);
+          ptx::mbar_arrive_expect_tx(&ctl->full[stage], here * adapter_bytes);
+          for (int g = 0; g < here; ++g) {
+            tma_load_3d(stage_base + g * adapter_bytes, &b_map, &ctl->full[stage], rank_block * kLoraRankBlock, n0, ctl->slot_adapter[slot + g]);
+          }
         }
       }
       if (++stage == Cfg::kStages) {
@@ -239,6 +249,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
     // ---------------- MMA issuer ----------------
     const bool issuer = ptx::elect_one();
     const uint32_t idesc = ptx::make_instr_desc(true, kBlockM, (rows + 15) & ~15);
+    const uint32_t b_desc_hi = lora_desc_hi(args.block.ranks);
     const uint32_t idesc_extra = ptx::make_instr_desc(false, kBlockM, (own + 15) & ~15);
     int stage = 0;
     uint32_t phase = 0;
@@ -259,11 +270,17 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
                                ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + ks * kUmmaKBytes), idesc, (i > 0 || ks > 0) ? 1u : 0u);
           }
         } else {
-          const int rank_block = (i - count) / slots / args.g.planes;
-          const int steps = (min(kLoraRankBlock, args.g.adapters.rank - rank_block * kLoraRankBlock) + 15) >> 4;
-          for (int ks = 0; ks < steps; ++ks) {
-            ptx::umma_ss<false>(tmem_base + kRowTile, ptx::make_smem_desc_sw128(stage_addr + ks * kUmmaKBytes),
-                                ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + ks * kUmmaKBytes), idesc_extra, (i > count || ks > 0) ? 1u : 0u);
+          const int rank_block = (i - count) / slot_blocks / args.g.planes;
+          const int here = min(per_block, slots - (i - count) % slot_blocks * per_block);
+          const int steps = (min(args.block.ranks, args.g.adapters.rank - rank_block * kLoraRankBlock) + 15) >> 4;  // of an adapter
+          for (int g = 0; g < here; ++g) {
+            const uint32_t b_lo = (((stage_addr + g * adapter_bytes) & 0x3ffffu) >> 4) | (1u << 16);
+            for (int ks = 0; ks < steps; ++ks) {
+              // (B is this MMA's A operand: channels are the lanes.)
+              ptx::umma_ss<false>(tmem_base + kRowTile, static_cast<uint64_t>(b_desc_hi) << 32 | (b_lo + 2u * ks),
+                                  ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + (g * steps + ks) * kUmmaKBytes), idesc_extra,
+                                  (i > count || g > 0 || ks > 0) ? 1u : 0u);
+            }
           }
         }
         ptx::tcgen05_commit(&ctl->empty[stage]);
@@ -284,35 +301,39 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
     const int own16 = (own + 15) & ~15;
     const uint16_t* const t_rows = args.g.t + (row0 + own_first) * rank_padded;
     constexpr int kPieces = kRowTile * 8 / 128;  // of a thread
+    const int share = args.block.ranks / 8;       // 16-byte pieces of an adapter in a row of 128 bytes: 2, 4 or 8
     int stage = count % Cfg::kStages;
     uint32_t used = 0;  // stages, one bit each, whose vacant barrier is in its odd phase
     for (int outer = 0; outer < args.rank_blocks * args.g.planes; ++outer) {
       const int rank0 = outer / args.g.planes * kLoraRankBlock;
       const int plane = outer % args.g.planes;
-      const int pieces = 2 * ((min(kLoraRankBlock, args.g.adapters.rank - rank0) + 15) >> 4);  // of 16 bytes in a row
+      const int pieces = 2 * ((min(args.block.ranks, args.g.adapters.rank - rank0) + 15) >> 4);  // of 16 bytes with ranks, in an adapter's share of a row
       const uint16_t* const from = t_rows + static_cast<int64_t>(plane) * args.g.rows * rank_padded + rank0;
       uint4 value[kPieces];
-      int id[kPieces];
-      uint32_t offset[kPieces];
+      int block[kPieces];  // the row's adapter is in this block, at this piece (or in none)
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) {
         const int e = thread + 128 * p;
-        const int row = e / pieces, piece = e - row * pieces;
+        const int row = e / 8, piece = e % 8;
         value[p] = make_uint4(0, 0, 0, 0);
-        id[p] = row < own ? ctl->id[row] : -1;
-        // The 128-byte swizzle that the operand tiles have: the 16-byte piece's number is xor-ed with the row's in its group of eight.
-        offset[p] = row < own16 ? static_cast<uint32_t>(row * kBlockKBytes + ((piece ^ (row & 7)) << 4)) : ~0u;
-        if (id[p] >= 0) value[p] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(row) * rank_padded) + piece);
+        block[p] = -1;
+        const int slot = row < own ? ctl->slot[row] : -1;
+        if (slot >= 0 && slot % per_block == piece / share) {
+          block[p] = slot / per_block;
+          if (piece % share < pieces) value[p] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(row) * rank_padded) + piece % share);
+        }
       }
-      for (int slot = 0; slot < slots; ++slot) {
-        const int adapter = ctl->slot_adapter[slot];
+      for (int b = 0; b < slot_blocks; ++b) {
         // (Not the empty barrier itself: these warps do not see its earlier phases, and would take one for another.)
         ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 54);
         used ^= 1u << stage;
         uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + kWeightBytes;
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
-          if (offset[p] != ~0u) *reinterpret_cast<uint4*>(to + offset[p]) = id[p] == adapter ? value[p] : make_uint4(0, 0, 0, 0);
+          const int e = thread + 128 * p;
+          const int row = e / 8, piece = e % 8;
+          // The 128-byte swizzle that the operand tiles have: the 16-byte piece's number is xor-ed with the row's in its group of eight.
+          if (row < own16) *reinterpret_cast<uint4*>(to + row * kBlockKBytes + ((piece ^ (row & 7)) << 4)) = block[p] == b ? value[p] : make_uint4(0, 0, 0, 0);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -519,7 +540,7 @@ cudaError_t launch_tile(KernelArgs args, cudaStream_t stream) {
   const uint64_t k = static_cast<uint64_t>(g.k_padded);
   CUtensorMap maps[3];
   if (!make_sw128_map(&maps[0], g.weight, true, g.n, k, kBlockM) || !make_sw128_map(&maps[1], g.xq, true, g.rows, k, kRowTile) ||
-      !make_sw128_map_3d(&maps[2], g.adapters.b, g.adapters.rank, g.n, g.adapters.count, g.adapters.b_stride, kBlockM)) {
+      !make_adapter_map(&maps[2], g.adapters.b, g.adapters.rank, g.n, g.adapters.count, g.adapters.b_stride, args.block.ranks, kBlockM)) {
     return cudaErrorInvalidValue;
   }
   Residency one_per_sm;
@@ -547,6 +568,7 @@ cudaError_t launch_lora_gemm(const LoraGemmArgs& g, cudaStream_t stream) {
   args.g = g;
   args.k_blocks = (g.k_padded + kBlockKBytes - 1) / kBlockKBytes;
   args.rank_blocks = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  args.block = lora_block(g.adapters.rank);
   args.vector_store = dense_vector_store(g.out, g.n, g.out_bf16 != 0) ? 1 : 0;
   if (g.rows <= 16) return launch_tile<16>(args, stream);
   if (g.rows <= 32) return launch_tile<32>(args, stream);

@@ -4,8 +4,8 @@
 // Two CTAs of a cluster drive one tile of 256 rows x 256 (or 128) channels (cta_group::2, gated_gemm.cu has the layout): rows are the lanes of tensor memory, channels its
 // columns, two accumulators take turns.  Both products end in the same accumulator:
 //   1. The int32 sums of the quantised product are complete: the epilogue warps turn them into the fp32 result of the base projection in place.
-//   2. The adapters' product is accumulated onto it by bf16 MMAs: for every adapter that rows of the tile use, a K block of [t of its rows,
-//      zeros for the others] x B[a]^T for each 64 ranks.  An own accumulator for it would leave tensor memory for one tile, and its epilogue no product to run under.
+//   2. The adapters' product is accumulated onto it by bf16 MMAs: for every adapter that rows of the tile use, [t of its rows, zeros for the
+//      others] x B[a]^T; a K block holds 64 ranks of one adapter, or two or four adapters of up to 32 or 16 ranks.  An own accumulator for it would leave tensor memory for one tile, and its epilogue no product to run under.
 //   3. The epilogue stores the accumulator.
 // Between 1 and 2 the tensor pipe works on the next tile: the adapters' K blocks of a tile stand behind the first kDelay K blocks of the next one, in the
 // order of every role's loop.  A tile whose rows have no adapter goes from 1 to 3.
@@ -67,6 +67,7 @@ static_assert(sizeof(Control) <= 6144, "control block exceeds its shared-memory 
 struct Args {
   LoraGemmArgs g;
   int k_blocks, m_tiles, n_tiles, rank_blocks;
+  LoraBlock block;
   int tma_store;
 };
 
@@ -168,7 +169,9 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
   const int first_tile = static_cast<int>(blockIdx.x >> 1);
   const int tile_stride = static_cast<int>(gridDim.x >> 1);
   const int k_blocks = args.k_blocks;
-  const int outer = args.rank_blocks * args.g.planes;  // K blocks of one adapter
+  const int outer = args.rank_blocks * args.g.planes;  // K blocks of one adapter, or of one group of them
+  const int per_block = args.block.adapters;
+  const uint32_t adapter_bytes = static_cast<uint32_t>(Cfg::kBRows) * args.block.ranks * 2;  // of one adapter's tile in a CTA
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -217,14 +220,17 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
     auto load_adapters = [&](const Tile& tile, int slots) {
       const int* const list = adapter_list(args, tile.m) + 1;
       for (int o = 0; o < outer; ++o) {
-        for (int slot = 0; slot < slots; ++slot) {
-          const int adapter = __ldcg(list + slot);
+        for (int slot = 0; slot < slots; slot += per_block) {
+          const int here = min(per_block, slots - slot);
           ptx::mbar_wait(&ctl->empty[stage], phase ^ 1u, abort_flag, status, 71);
           if (issuer) {
             ptx::mbar_arrive(&ctl->vacant[stage]);
-            if (leader) ptx::mbar_arrive_expect_tx(&ctl->full[stage], 2 * Cfg::kBBytes);
-            tma_load_3d_pair(smem_base + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes, &b_map, full_leader0 + 8u * static_cast<uint32_t>(stage),
-                             o / args.g.planes * kLoraRankBlock, tile.n * kTileN + Cfg::kBRows * static_cast<int>(cta), adapter);
+            if (leader) ptx::mbar_arrive_expect_tx(&ctl->full[stage], 2 * here * adapter_bytes);
+            for (int g = 0; g < here; ++g) {
+              tma_load_3d_pair(smem_base + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes + g * adapter_bytes, &b_map,
+                               full_leader0 + 8u * static_cast<uint32_t>(stage), o / args.g.planes * kLoraRankBlock,
+                               tile.n * kTileN + Cfg::kBRows * static_cast<int>(cta), __ldcg(list + slot + g));
+            }
           }
           advance();
         }
@@ -277,6 +283,7 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
       constexpr uint32_t kIdesc = ptx::make_instr_desc(true, 2 * kRowsPerCta, kTileN);
       constexpr uint32_t kIdescAdapters = ptx::make_instr_desc(false, 2 * kRowsPerCta, kTileN);
       const uint32_t desc_hi = static_cast<uint32_t>(1024 >> 4) | (1u << 14) | (2u << 29);
+      const uint32_t b_desc_hi = lora_desc_hi(args.block.ranks);
       const uint32_t stage0 = ((smem_base & 0x3ffffu) >> 4) | (1u << 16);
       auto both = [&](uint64_t* bar, int which) {
         const uint32_t here = ptx::smem_u32(bar + which);
@@ -298,16 +305,20 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
         mbar_wait_cluster(&ctl->converted[buffer], (converted_phase >> buffer) & 1u, abort_flag, status, 73);
         converted_phase ^= 1u << buffer;
         for (int o = 0; o < outer; ++o) {
-          const int steps = (min(kLoraRankBlock, args.g.adapters.rank - o / args.g.planes * kLoraRankBlock) + 15) >> 4;
-          for (int slot = 0; slot < slots; ++slot) {
+          const int steps = (min(args.block.ranks, args.g.adapters.rank - o / args.g.planes * kLoraRankBlock) + 15) >> 4;  // of an adapter
+          for (int slot = 0; slot < slots; slot += per_block) {
+            const int here = min(per_block, slots - slot);
             ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 74);
             mbar_wait_cluster(&ctl->coefficients[stage], (written >> stage) & 1u, abort_flag, status, 75);
             written ^= 1u << stage;
             ptx::tcgen05_fence_after();
             if (issuer) {
               const uint32_t a_lo = stage0 + static_cast<uint32_t>(stage) * (Cfg::kStageBytes >> 4);
-              for (int ks = 0; ks < steps; ++ks) {
-                umma_pair<false>(tmem_base + kTileN * buffer, a_lo + 2u * ks, a_lo + (Cfg::kABytes >> 4) + 2u * ks, desc_hi, kIdescAdapters, 1u);
+              for (int g = 0; g < here; ++g) {
+                const uint32_t b_lo = a_lo + (Cfg::kABytes >> 4) + g * (adapter_bytes >> 4);
+                for (int ks = 0; ks < steps; ++ks) {
+                  umma_pair_mixed(tmem_base + kTileN * buffer, a_lo + 2u * (g * steps + ks), desc_hi, b_lo + 2u * ks, b_desc_hi, kIdescAdapters, 1u);
+                }
               }
               both(ctl->empty, stage);
             }
@@ -482,24 +493,26 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
       const int* const list = adapter_list(args, tile.m) + 1;
       const int64_t row = static_cast<int64_t>(tile.m) * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + row_in_cta;
       const int id = row < args.g.rows ? load_adapter_id(args.g.adapters, row) : -1;
+      int my_slot = -1;
+      for (int slot = 0; slot < slots; ++slot) my_slot = __ldcg(list + slot) == id ? slot : my_slot;  // no list holds -1
+      const int share = args.block.ranks / 8;  // 16-byte pieces of an adapter in a row of 128 bytes: 2, 4 or 8
       for (int o = 0; o < outer; ++o) {
         const int rank0 = o / args.g.planes * kLoraRankBlock;
-        const int pieces = 2 * ((min(kLoraRankBlock, args.g.adapters.rank - rank0) + 15) >> 4);
+        const int pieces = 2 * ((min(args.block.ranks, args.g.adapters.rank - rank0) + 15) >> 4);  // of them with ranks
         const uint16_t* const from = args.g.t + (o % args.g.planes * args.g.rows + row) * rank_padded + rank0;
         uint4 value[8];
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
           value[p] = make_uint4(0, 0, 0, 0);
-          if (id >= 0 && p < pieces) value[p] = __ldcg(reinterpret_cast<const uint4*>(from) + p);
+          if (my_slot >= 0 && p % share < pieces) value[p] = __ldcg(reinterpret_cast<const uint4*>(from) + p % share);
         }
-        for (int slot = 0; slot < slots; ++slot) {
-          const bool mine = id == __ldcg(list + slot);
+        for (int slot = 0; slot < slots; slot += per_block) {
           ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 80);
           used ^= 1u << stage;
           uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + row_in_cta * 128;
 #pragma unroll
           for (int p = 0; p < 8; ++p) {
-            if (p < pieces) *reinterpret_cast<uint4*>(to + ((p ^ (row_in_cta & 7)) << 4)) = mine ? value[p] : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(to + ((p ^ (row_in_cta & 7)) << 4)) = slot + p / share == my_slot ? value[p] : make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
@@ -555,7 +568,7 @@ cudaError_t launch(Args args, cudaStream_t stream) {
   CUtensorMap maps[4];
   if (!make_sw128_map(&maps[0], g.xq, true, static_cast<uint64_t>(g.rows), k, kRowsPerCta) ||
       !make_sw128_map(&maps[1], g.weight, true, static_cast<uint64_t>(g.n), k, Cfg::kBRows) ||
-      !make_sw128_map_3d(&maps[2], g.adapters.b, g.adapters.rank, g.n, g.adapters.count, g.adapters.b_stride, Cfg::kBRows)) {
+      !make_adapter_map(&maps[2], g.adapters.b, g.adapters.rank, g.n, g.adapters.count, g.adapters.b_stride, args.block.ranks, Cfg::kBRows)) {
     return cudaErrorInvalidValue;
   }
   args.tma_store = static_cast<int64_t>(g.n) * (g.out_bf16 ? 2 : 4) % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
@@ -579,6 +592,7 @@ cudaError_t launch_lora_pair_gemm(const LoraGemmArgs& g, cudaStream_t stream) {
   args.g = g;
   args.k_blocks = (g.k_padded + kBlockKBytes - 1) / kBlockKBytes;
   args.rank_blocks = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  args.block = lora_block(g.adapters.rank);
   args.m_tiles = static_cast<int>((g.rows + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta));
   const int64_t pairs = sm_count_of_current_device() / 2;
   const int64_t wide = static_cast<int64_t>(args.m_tiles) * ((g.n + 255) / 256), narrow = static_cast<int64_t>(args.m_tiles) * ((g.n + 127) / 128);

@@ -752,16 +752,17 @@ bool make_sw128_map(CUtensorMap* map, const void* base, bool int8, uint64_t rows
   return result == CUDA_SUCCESS;
 }
 
-bool make_sw128_map_3d(CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows, uint64_t planes, uint64_t row_stride, uint32_t box_rows) {
+bool make_adapter_map(CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows, uint64_t planes, uint64_t row_stride, uint32_t box_columns,
+                      uint32_t box_rows) {
   EncodeTiledFn encode = encode_tiled_fn();
   if (encode == nullptr) return false;
   const cuuint64_t dims[3] = {columns, rows, planes};
   const cuuint64_t strides[2] = {row_stride * 2, rows * row_stride * 2};
-  const cuuint32_t box[3] = {kBlockKBytes / 2, box_rows, 1};
+  const cuuint32_t box[3] = {box_columns, box_rows, 1};
   const cuuint32_t elem_strides[3] = {1, 1, 1};
+  const CUtensorMapSwizzle swizzle = box_columns == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : box_columns == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows) {
