@@ -981,9 +981,16 @@ int fmoe_i8gemm_dynamic_scaled_mm_pair(const void* x_bf16, int64_t rows, int32_t
 }
 
 namespace {
-size_t lora_list_bytes(int64_t rows) {
+// Lists of adapters, then the rows' places in them.
+size_t lora_slot_offset(int64_t rows) {
   return align_up(static_cast<size_t>((rows + fmoe::kLoraListRows - 1) / fmoe::kLoraListRows) * fmoe::kLoraListInts * sizeof(int), 256);
 }
+size_t lora_list_bytes(int64_t rows) { return lora_slot_offset(rows) + align_up(static_cast<size_t>(rows) * sizeof(int), 256); }
+
+// Which kernel: the two-SM one where its tiles of 256 x 256 fill two thirds of the chip, the split one (lora_gemm.cu) before.  Split / two-SM, whole op: 201 rows
+// of 1536 -> 24576 (96 tiles) 38 / 33 us; 384 rows 7168 -> 7168 (56) 47 / 43; 512 rows 16384 -> 7168 (56) 92 / 84; 256 rows of it (28) 64 / 62 to 77; 777 rows 2056 -> 1240
+// (20) 25 / 23 to 28; 201 rows 7168 -> 1536 (6) 23 / 28 to 35.
+bool lora_pair_pays(int64_t rows, int n) { return rows > 128 && 3 * ((rows + 255) / 256) * ((static_cast<int64_t>(n) + 255) / 256) >= fmoe::threshold_sms; }
 }  // namespace
 
 size_t fmoe_i8gemm_lora_workspace_bytes(int64_t rows, int32_t k, int32_t rank, int32_t out_is_bf16) {
@@ -1023,15 +1030,10 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
   args.adapters = {static_cast<const uint16_t*>(adapters->a), static_cast<const uint16_t*>(adapters->b), adapters->a_stride, adapters->b_stride, adapters->scaling,
                    adapter_ids, ids_are_64, adapters->count, adapters->rank};
   int* const lists = reinterpret_cast<int*>(base + align_up(layout.total, 256));
+  int* const row_slots = reinterpret_cast<int*>(reinterpret_cast<char*>(lists) + lora_slot_offset(rows));
   uint16_t* const t = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(lists) + lora_list_bytes(rows));
-  const char* text = getenv("LP");
-  const bool many = rows > (text != nullptr ? atoi(text) : 256);
+  const bool many = lora_pair_pays(rows, n);
   args.planes = out_is_bf16 ? 1 : fmoe::kLoraPlanes;
-  cudaError_t error = fmoe::launch_lora_quantize(static_cast<const uint16_t*>(x_bf16), rows, k, layout.k_padded, reinterpret_cast<int8_t*>(base + layout.xq),
-                                                 reinterpret_cast<float*>(base + layout.scale), reinterpret_cast<int*>(base + layout.status), args.adapters, many ? lists : nullptr, stream);
-  if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora activation quantisation");
-  error = fmoe::launch_lora_shrink(static_cast<const uint16_t*>(x_bf16), rows, k, args.adapters, t, args.planes, stream);
-  if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora coefficients");
   args.xq = reinterpret_cast<const int8_t*>(base + layout.xq);
   args.a_scale = reinterpret_cast<const float*>(base + layout.scale);
   args.weight = w;
@@ -1044,7 +1046,11 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
   args.k_padded = layout.k_padded;
   args.t = t;
   args.status = reinterpret_cast<int*>(base + layout.status);
+  cudaError_t error = fmoe::launch_lora_front(args, static_cast<const uint16_t*>(x_bf16), k, reinterpret_cast<int8_t*>(base + layout.xq),
+                                              reinterpret_cast<float*>(base + layout.scale), t, many ? lists : nullptr, row_slots, stream);
+  if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora rows and coefficients");
   args.lists = lists;
+  args.row_slots = row_slots;
   error = many ? fmoe::launch_lora_pair_gemm(args, stream) : fmoe::launch_lora_gemm(args, stream);
   return error == cudaSuccess ? FMOE_OK : cuda_fail(error, "i8gemm lora GEMM");
 }

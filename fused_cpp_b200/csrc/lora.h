@@ -1,4 +1,4 @@
-// Low-rank adapters of many requests beside a dense W8A8 projection: arguments of the kernels in lora_shrink.cu and lora_gemm.cu.
+// Low-rank adapters of many requests beside a dense W8A8 projection: arguments of the kernels in lora_front.cu, lora_gemm.cu and lora_pair_gemm.cu.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -52,17 +52,8 @@ __device__ __forceinline__ int load_adapter_id(const LoraAdapters& adapters, int
 constexpr int kLoraListRows = 256;                   // rows of a list of adapters
 constexpr int kLoraListInts = kLoraListRows + 4;  // of a list in memory: the number of adapters in use by its rows, then their ids
 
-// Rows of x as int8 [rows, k_padded] with a scale each, zeros behind k; clears the status block of the call.  lists (nullable): the
-// adapters in use by every kLoraListRows rows.
-cudaError_t launch_lora_quantize(const uint16_t* x, int64_t rows, int k, int k_padded, int8_t* q, float* scale, int* status,
-                                 const LoraAdapters& adapters, int* lists, cudaStream_t stream);
-
-// t[plane][row][rank] = scaling[id] * (A[id] x[row]) for the rows that have an adapter (the others' are left as they are), as `planes` bf16
-// terms.  A programmatic dependent of the kernel in front, of which it needs nothing.
-cudaError_t launch_lora_shrink(const uint16_t* x, int64_t rows, int k, const LoraAdapters& adapters, uint16_t* t, int planes, cudaStream_t stream);
-
 // out[row, n] = dequantised product (+ bias) + sum over ranks of t[row, rank] B[id, n, rank].  A programmatic dependent of
-// launch_lora_shrink.
+// launch_lora_front.
 struct LoraGemmArgs {
   const int8_t* xq;      // [rows, k_padded]
   const float* a_scale;  // [rows]
@@ -76,9 +67,15 @@ struct LoraGemmArgs {
   LoraAdapters adapters;
   const uint16_t* t;
   int planes;
-  const int* lists;  // of launch_lora_quantize
+  const int* lists;      // of launch_lora_front, as row_slots
+  const int* row_slots;
   int* status;
 };
+// Rows of x [rows, k] as int8 q [rows, k_padded] with a scale each, zeros behind k; t[plane][row][rank] = scaling[id] * (A[id] x[row]) for the rows that
+// have an adapter (the others' are left as they are), as `planes` bf16 terms; with lists, the adapters in use by every kLoraListRows rows and
+// each row's place among them.  Clears the status block.  What it writes is what the GEMM of the same arguments reads.
+cudaError_t launch_lora_front(const LoraGemmArgs& args, const uint16_t* x, int k, int8_t* q, float* scale, uint16_t* t, int* lists, int* row_slots,
+                              cudaStream_t stream);
 cudaError_t launch_lora_gemm(const LoraGemmArgs& args, cudaStream_t stream);
 // The same over many rows, by lists.
 cudaError_t launch_lora_pair_gemm(const LoraGemmArgs& args, cudaStream_t stream);

@@ -1,0 +1,572 @@
+// What stands in front of the GEMM of a projection with low-rank adapters: the rows of x as int8 with a scale each, the coefficients
+// t[row] = scaling[a] * (A[a] x[row]) with a = the row's adapter, rows in any order, and the lists of the adapters that every 256 rows use.
+//
+// Coefficients.  What is read is x once and every adapter in use once, and a batch has few rows per adapter and a long K (one row of 7168 values
+// against 16 to 64 ranks).  So the K range is split over the warps of a CTA, of a cluster if there are few rows, each warp keeps ranks x rows partial sums of
+// mma.sync.m16n8k16 (ranks are its M, rows its N), and the warps' sums meet in shared memory, the CTAs' in distributed shared memory, in a
+// fixed order.  Fragments come straight from global memory with 16-byte loads: the order of the K elements inside a group of 32 may be any as long
+// as both operands use the same, so that lane (g, q) takes elements 8q .. 8q + 7 of its row for two MMAs.  A unit is up to 32 rows of one adapter.
+//
+// Few rows (latency counts): one launch for rows and coefficients, units are made of 32 neighbouring rows by one match instruction (over 128 rows, in shared
+// memory, the list alone took 2.3 of 9.2 us of 201 rows of 1536 values, and the three of them that follow a loop of single loads are one now that
+// all loads of a warp's K range are in flight together).  Many rows (traffic counts): a unit is made of 128 rows' list, so that an adapter is read once
+// for them, in a launch of its own behind the one that quantises: with both kinds of CTA in one launch at two to an SM, 8192 rows of 16384 values took 180 us
+// instead of 150.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "lora.h"
+#include "ptx.cuh"
+#include "row_quant.cuh"
+
+namespace fmoe {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kTileRows = 128;            // rows of a list of units, where there are many
+constexpr int kUnitRows = 32;
+constexpr int kMaxCluster = 8;
+constexpr int kHeld = 8;                  // 16-byte vectors of a row that a thread holds
+constexpr int kFewRows = 256;
+
+struct FrontArgs {
+  const uint16_t* x;
+  int64_t rows;
+  int k, k_padded;
+  LoraAdapters adapters;
+  int8_t* q;
+  float* scale;
+  uint16_t* t;
+  int planes;
+  int* lists;      // nullable
+  int* row_slots;  // [rows], with lists
+  int* status;
+  int cluster;       // CTAs that share a unit's K range
+  int unit_groups;   // clusters that share a tile's units
+  int row_groups;    // few rows: clusters that share a tile's rows
+};
+
+// Partial sums of a unit, [rank][row].
+template <int kRankTiles>
+struct UnitSums {
+  static constexpr int kValues = 16 * kRankTiles * kUnitRows;
+  alignas(16) float total[kValues];
+  alignas(16) float part[kWarps][kValues];  // stored in pairs
+};
+
+struct UnitList {
+  alignas(16) int id[kTileRows];
+  int slot_adapter[kTileRows], slot_rows[kTileRows], slot_first[kTileRows];
+  int unit_slot[kTileRows], unit_row[kTileRows];  // unit -> slot, first row of it in `order`
+  int order[kTileRows];                           // rows of the tile, slot by slot
+  int warp_count[4];
+  int units;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Eight values of a row of x from element k on; k is a multiple of 8, what lies behind the row's end is zero.
+template <bool kVector>
+__device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int columns) {
+  if constexpr (kVector) {
+    return k < columns ? __ldcg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
+  } else {
+    uint32_t words[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t low = k + 2 * i < columns ? __ldcg(row + k + 2 * i) : 0;
+      const uint32_t high = k + 2 * i + 1 < columns ? __ldcg(row + k + 2 * i + 1) : 0;
+      words[i] = low | (high << 16);
+    }
+    return make_uint4(words[0], words[1], words[2], words[3]);
+  }
+}
+
+// The tile's units, in an order that the ids alone decide.
+__device__ __forceinline__ void list_units(UnitList& s, const FrontArgs& args, int64_t row0) {
+  const int i = threadIdx.x;
+  const int lane = i & 31;
+  const int tile_rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), args.rows - row0));
+  int before = 0, total = 0, first = kTileRows;
+  if (i < kTileRows) s.id[i] = i < tile_rows ? load_adapter_id(args.adapters, row0 + i) : -1;
+  __syncthreads();
+  const int mine = i < kTileRows ? s.id[i] : -1;
+  if (mine >= 0) {
+    for (int j = 0; j < tile_rows; j += 4) {
+      const int4 others = *reinterpret_cast<const int4*>(&s.id[j]);
+      const int four[4] = {others.x, others.y, others.z, others.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool same = four[k] == mine;
+        if (same && first == kTileRows) first = j + k;
+        before += same && j + k < i;
+        total += same;
+      }
+    }
+  }
+  const bool owner = mine >= 0 && first == i;
+  const unsigned owners = __ballot_sync(0xffffffffu, owner);
+  if (i < kTileRows && lane == 0) s.warp_count[i >> 5] = __popc(owners);
+  __syncthreads();
+  int slot = __popc(owners & ((1u << lane) - 1));
+  int slots = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < (i >> 5)) slot += s.warp_count[w];
+    slots += s.warp_count[w];
+  }
+  if (owner) {
+    s.slot_adapter[slot] = mine;
+    s.slot_rows[slot] = total;
+    s.unit_row[i] = slot;  // for a moment: the slot of the adapter's first row
+  }
+  __syncthreads();
+  const int my_slot = mine >= 0 ? s.unit_row[first] : 0;
+  // Rows (low half) and units (high half) of the slots in front of slot i.
+  const int rows = i < slots ? s.slot_rows[i] : 0;
+  const int packed = rows | ((rows + kUnitRows - 1) / kUnitRows) << 16;
+  int scan = packed;
+#pragma unroll
+  for (int offset = 1; offset < 32; offset <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, scan, offset);
+    if (lane >= offset) scan += other;
+  }
+  __syncthreads();  // unit_row and warp_count are read
+  if (i < kTileRows && lane == 31) s.warp_count[i >> 5] = scan;
+  __syncthreads();
+  int front = scan - packed;
+  for (int w = 0; w < 4 && w < (i >> 5); ++w) front += s.warp_count[w];
+  if (i < slots) {
+    const int row_first = front & 0xffff, unit_first = front >> 16;
+    s.slot_first[i] = row_first;
+    for (int u = 0; u < packed >> 16; ++u) {
+      s.unit_slot[unit_first + u] = i;
+      s.unit_row[unit_first + u] = row_first + u * kUnitRows;
+    }
+    if (i == slots - 1) s.units = unit_first + (packed >> 16);
+  }
+  if (slots == 0 && i == 0) s.units = 0;
+  __syncthreads();
+  if (mine >= 0) s.order[s.slot_first[my_slot] + before] = i;
+  __syncthreads();
+}
+
+// The warps' partial sums of a unit: the rows order[0 .. count) of x from `x` on, times the first `ranks` rows of `a`.
+// kUnroll groups of 32 K elements are in flight together.
+template <bool kVector, int kRankTiles, int kRowTiles, int kUnroll>
+__device__ __forceinline__ void multiply_unit(const FrontArgs& args, const uint16_t* x, const int* order, int count, const uint16_t* a, int ranks, int chunk_begin,
+                                              int chunk_end, float* part) {
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2, q = lane & 3;
+  float acc[kRankTiles][kRowTiles][4];
+#pragma unroll
+  for (int m = 0; m < kRankTiles; ++m)
+#pragma unroll
+    for (int n = 0; n < kRowTiles; ++n)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[m][n][v] = 0.0f;
+  const uint16_t* x_rows[kRowTiles];
+#pragma unroll
+  for (int n = 0; n < kRowTiles; ++n) {
+    const int local = 8 * n + g;
+    x_rows[n] = local < count ? x + static_cast<int64_t>(order[local]) * args.k : nullptr;
+  }
+  const int a_stride = args.adapters.a_stride;
+  for (int chunk0 = chunk_begin; chunk0 < chunk_end; chunk0 += kUnroll) {
+    uint4 xv[kUnroll][kRowTiles], low[kUnroll][kRankTiles], high[kUnroll][kRankTiles];
+#pragma unroll
+    for (int c = 0; c < kUnroll; ++c) {
+      const int k = (chunk0 + c) * 32 + 8 * q;
+      const bool inside = chunk0 + c < chunk_end;
+#pragma unroll
+      for (int n = 0; n < kRowTiles; ++n) xv[c][n] = inside && x_rows[n] != nullptr ? load_x8<kVector>(x_rows[n], k, args.k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int m = 0; m < kRankTiles; ++m) {
+        const int r = 16 * m + g;
+        const uint16_t* const from = a + static_cast<int64_t>(r) * a_stride + k;
+        low[c][m] = inside && k < a_stride && r < ranks ? __ldcg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
+        high[c][m] = inside && k < a_stride && r + 8 < ranks ? __ldcg(reinterpret_cast<const uint4*>(from + 8 * a_stride)) : make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kUnroll; ++c) {
+#pragma unroll
+      for (int n = 0; n < kRowTiles; ++n) {
+        if (8 * n >= count) break;
+#pragma unroll
+        for (int m = 0; m < kRankTiles; ++m) {
+          const uint32_t first[4] = {low[c][m].x, high[c][m].x, low[c][m].y, high[c][m].y};
+          const uint32_t second[4] = {low[c][m].z, high[c][m].z, low[c][m].w, high[c][m].w};
+          mma_bf16(acc[m][n], first, xv[c][n].x, xv[c][n].y);
+          mma_bf16(acc[m][n], second, xv[c][n].z, xv[c][n].w);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kRankTiles; ++m)
+#pragma unroll
+    for (int n = 0; n < kRowTiles; ++n) {
+      float* to = part + (16 * m + g) * kUnitRows + 8 * n + 2 * q;
+      *reinterpret_cast<float2*>(to) = make_float2(acc[m][n][0], acc[m][n][1]);
+      *reinterpret_cast<float2*>(to + 8 * kUnitRows) = make_float2(acc[m][n][2], acc[m][n][3]);
+    }
+}
+
+// One row as int8: scale = amax * (1/127) in 32 bits (1 for a row of zeros), q = clamp(rint(x / scale), -128, 127).
+template <bool kVector>
+__device__ __forceinline__ void quantise_row(const FrontArgs& args, int64_t row, float* smem) {
+  const uint16_t* const src = args.x + row * args.k;
+  const int vectors = args.k_padded >> 3;  // k_padded is a multiple of 16
+  uint4 held[kHeld];
+  float local = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int v = threadIdx.x + i * kThreads;
+    held[i] = v < vectors ? load_x8<kVector>(src, 8 * v, args.k) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) local = fmaxf(local, amax8(held[i]));
+  for (int v = threadIdx.x + kHeld * kThreads; v < vectors; v += kThreads) local = fmaxf(local, amax8(load_x8<kVector>(src, 8 * v, args.k)));
+  const float amax = block_max(local, smem);
+  const float scale = amax > 0.0f ? __fmul_rn(amax, 1.0f / 127.0f) : 1.0f;
+  if (threadIdx.x == 0) args.scale[row] = scale;
+  const float inverse = __fdiv_rn(1.0f, scale);
+  uint2* const dst = reinterpret_cast<uint2*>(args.q + row * args.k_padded);
+  auto store = [&](int v, const uint4& eight) {
+    float values[8];
+    unpack8(eight, values);
+    dst[v] = make_uint2(quantize4_torchref_fast(values, scale, inverse, -128.0f), quantize4_torchref_fast(values + 4, scale, inverse, -128.0f));
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int v = threadIdx.x + i * kThreads;
+    if (v < vectors) store(v, held[i]);
+  }
+  for (int v = threadIdx.x + kHeld * kThreads; v < vectors; v += kThreads) store(v, load_x8<kVector>(src, 8 * v, args.k));
+}
+
+// The same without holding it: more CTAs fit an SM.
+template <bool kVector>
+__device__ __forceinline__ void quantise_row_twice(const FrontArgs& args, int64_t row, float* smem) {
+  const uint16_t* const src = args.x + row * args.k;
+  const int vectors = args.k_padded >> 3;
+  float local = 0.0f;
+  for (int v = threadIdx.x; v < vectors; v += kThreads) local = fmaxf(local, amax8(load_x8<kVector>(src, 8 * v, args.k)));
+  const float amax = block_max(local, smem);
+  const float scale = amax > 0.0f ? __fmul_rn(amax, 1.0f / 127.0f) : 1.0f;
+  if (threadIdx.x == 0) args.scale[row] = scale;
+  const float inverse = __fdiv_rn(1.0f, scale);
+  uint2* const dst = reinterpret_cast<uint2*>(args.q + row * args.k_padded);
+  for (int v = threadIdx.x; v < vectors; v += kThreads) {
+    float values[8];
+    unpack8(load_x8<kVector>(src, 8 * v, args.k), values);
+    dst[v] = make_uint2(quantize4_torchref_fast<false>(values, scale, inverse, -128.0f), quantize4_torchref_fast<false>(values + 4, scale, inverse, -128.0f));
+  }
+}
+
+// The adapters in use by 256 rows, each once, in the order of their first rows, and every row's place in that list (-1: no adapter).
+__device__ void list_adapters(const FrontArgs& args, int64_t tile) {
+  static_assert(kThreads == kLoraListRows, "a thread for each row");
+  __shared__ alignas(16) int ids[kLoraListRows];
+  __shared__ int slot_of[kLoraListRows];
+  __shared__ int warp_count[kLoraListRows / 32];
+  const int i = threadIdx.x;
+  const int64_t row = tile * kLoraListRows + i;
+  const int mine = row < args.rows ? load_adapter_id(args.adapters, row) : -1;
+  ids[i] = mine;
+  __syncthreads();
+  int first = i;
+  for (int j = 0; j < i; j += 4) {
+    const int4 others = *reinterpret_cast<const int4*>(&ids[j]);
+    const int four[4] = {others.x, others.y, others.z, others.w};
+#pragma unroll
+    for (int c = 3; c >= 0; --c) {
+      if (four[c] == mine && j + c < first) first = j + c;
+    }
+  }
+  const bool owner = mine >= 0 && first == i;
+  const unsigned owners = __ballot_sync(0xffffffffu, owner);
+  if ((i & 31) == 0) warp_count[i >> 5] = __popc(owners);
+  __syncthreads();
+  int slot = __popc(owners & ((1u << (i & 31)) - 1)), slots = 0;
+  for (int w = 0; w < kLoraListRows / 32; ++w) {
+    if (w < (i >> 5)) slot += warp_count[w];
+    slots += warp_count[w];
+  }
+  int* const list = args.lists + tile * kLoraListInts;
+  if (i == 0) list[0] = slots;
+  if (owner) {
+    list[1 + slot] = mine;
+    slot_of[i] = slot;
+  }
+  __syncthreads();
+  if (row < args.rows) args.row_slots[row] = mine >= 0 ? slot_of[first] : -1;
+}
+
+// The sums of a unit of 8 kRowTiles rows at most: over the warps, over the CTAs of the cluster, times scaling, to t.
+template <int kRankTiles, int kRowTiles>
+__device__ __forceinline__ void finish_unit(const FrontArgs& args, UnitSums<kRankTiles>& s, int cluster_rank, int adapter, int64_t row0, const int* order, int count,
+                                            int rank0, int ranks) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  constexpr int kRanks = 16 * kRankTiles, kRows = 8 * kRowTiles;
+  const float scale = __ldcg(args.adapters.scaling + adapter);
+  const int rank_padded = lora_rank_padded(args.adapters.rank);
+  __syncthreads();
+  for (int e = threadIdx.x; e < kRanks * kRows; e += kThreads) {
+    const int at = e / kRows * kUnitRows + e % kRows;
+    float sum = s.part[0][at];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) sum += s.part[w][at];
+    s.total[at] = sum;
+  }
+  if (args.cluster > 1) {
+    cluster.sync();
+  } else {
+    __syncthreads();
+  }
+  // Element e = (row, rank), ranks side by side as they lie in t; every cluster-th one is this CTA's.
+  for (int e = threadIdx.x * args.cluster + cluster_rank; e < kRanks * count; e += kThreads * args.cluster) {
+    const int row = e / kRanks, r = e % kRanks;
+    if (rank0 + r >= rank_padded) continue;
+    const int at = r * kUnitRows + row;
+    float sum = 0.0f;
+    if (args.cluster > 1) {
+      float values[kMaxCluster];
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) values[c] = c < args.cluster ? cluster.map_shared_rank(s.total, c)[at] : 0.0f;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) sum += values[c];
+    } else {
+      sum = s.total[at];
+    }
+    float rest = r < ranks ? __fmul_rn(sum, scale) : 0.0f;
+    uint16_t* to = args.t + (row0 + order[row]) * rank_padded + rank0 + r;
+    for (int plane = 0; plane < args.planes; ++plane) {
+      const uint16_t bits = __bfloat16_as_ushort(__float2bfloat16_rn(rest));
+      *to = bits;
+      rest = __fsub_rn(rest, bf16_bits_to_f32(bits));  // exact; what is left of an infinity (NaN) is not wanted
+      if (!isfinite(rest)) rest = 0.0f;
+      to += args.rows * rank_padded;
+    }
+  }
+  if (args.cluster > 1) {
+    cluster.sync();  // nobody still reads these sums
+  } else {
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ void chunk_range(const FrontArgs& args, int cluster_rank, int* begin, int* end) {
+  const int k32 = (args.k + 31) / 32;
+  const int worker = cluster_rank * kWarps + static_cast<int>(threadIdx.x >> 5), workers = args.cluster * kWarps;
+  *begin = static_cast<int>(static_cast<int64_t>(k32) * worker / workers);
+  *end = static_cast<int>(static_cast<int64_t>(k32) * (worker + 1) / workers);
+}
+
+// Few rows.  Grid: for every 32 rows row_groups clusters that quantise and unit_groups that multiply, then the lists.
+template <bool kVector, int kRankTiles>
+__global__ void __launch_bounds__(kThreads, 2)
+lora_front_kernel(const __grid_constant__ FrontArgs args) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  UnitSums<kRankTiles>& s = *reinterpret_cast<UnitSums<kRankTiles>*>(smem_raw);
+  __shared__ float block_max_values[32];
+  __shared__ int order[kUnitRows];
+  ptx::launch_dependents();
+  if (blockIdx.x == 0 && threadIdx.x < kStatusWords) args.status[threadIdx.x] = 0;
+  const int cluster_rank = static_cast<int>(blockIdx.x) % args.cluster;
+  const int group = static_cast<int>(blockIdx.x) / args.cluster;
+  const int per_tile = args.row_groups + args.unit_groups;
+  const int tiles = static_cast<int>((args.rows + kUnitRows - 1) / kUnitRows);
+  const int tile = group / per_tile;
+  const int role = group - tile * per_tile;
+  const int64_t row0 = static_cast<int64_t>(tile) * kUnitRows;
+  if (tile >= tiles) {  // behind the tiles: the lists
+    const int64_t list = static_cast<int64_t>(group - tiles * per_tile) * args.cluster + cluster_rank;
+    if (list * kLoraListRows < args.rows) list_adapters(args, list);
+    return;
+  }
+  if (role < args.row_groups) {
+    const int64_t end = min(row0 + kUnitRows, args.rows);
+    for (int64_t row = row0 + role * args.cluster + cluster_rank; row < end; row += args.row_groups * args.cluster) quantise_row<kVector>(args, row, block_max_values);
+    return;
+  }
+  // Every warp finds the units of the 32 rows for itself: lane i has row i, and a unit is the set of lanes with one adapter.
+  const int lane = threadIdx.x & 31;
+  const int id = row0 + lane < args.rows ? load_adapter_id(args.adapters, row0 + lane) : -1;
+  const unsigned same = __match_any_sync(0xffffffffu, id);
+  const unsigned leaders = __ballot_sync(0xffffffffu, id >= 0 && (same & ((1u << lane) - 1)) == 0);
+  int chunk_begin, chunk_end;
+  chunk_range(args, cluster_rank, &chunk_begin, &chunk_end);
+  const int rank_blocks = (args.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  const int work = __popc(leaders) * rank_blocks;
+  for (int item = role - args.row_groups; item < work; item += args.unit_groups) {
+    unsigned left = leaders;
+    for (int i = item / rank_blocks; i > 0; --i) left &= left - 1;
+    const int leader = __ffs(left) - 1;
+    const int adapter = __shfl_sync(0xffffffffu, id, leader);
+    const unsigned rows = __shfl_sync(0xffffffffu, same, leader);
+    const int rank0 = item % rank_blocks * kLoraRankBlock;
+    const int count = __popc(rows);
+    const int ranks = min(kLoraRankBlock, args.adapters.rank - rank0);
+    if (threadIdx.x < 32 && (rows >> lane & 1u)) order[__popc(rows & ((1u << lane) - 1))] = lane;
+    __syncthreads();
+    const uint16_t* const x = args.x + row0 * args.k;
+    const uint16_t* const a = args.adapters.a + (static_cast<int64_t>(adapter) * args.adapters.rank + rank0) * args.adapters.a_stride;
+    float* const part = s.part[threadIdx.x >> 5];
+    if (count <= 8) {
+      multiply_unit<kVector, kRankTiles, 1, kRankTiles == 1 ? 4 : kRankTiles == 2 ? 4 : 2>(args, x, order, count, a, ranks, chunk_begin, chunk_end, part);
+      finish_unit<kRankTiles, 1>(args, s, cluster_rank, adapter, row0, order, count, rank0, ranks);
+    } else {
+      multiply_unit<kVector, kRankTiles, 4, kRankTiles == 1 ? 2 : 1>(args, x, order, count, a, ranks, chunk_begin, chunk_end, part);
+      finish_unit<kRankTiles, 4>(args, s, cluster_rank, adapter, row0, order, count, rank0, ranks);
+    }
+  }
+}
+
+// Many rows: a CTA for each row, then the lists.
+template <bool kVector>
+__global__ void __launch_bounds__(kThreads)
+lora_rows_kernel(const __grid_constant__ FrontArgs args) {
+  ptx::launch_dependents();
+  __shared__ float block_max_values[32];
+  if (blockIdx.x == 0 && threadIdx.x < kStatusWords) args.status[threadIdx.x] = 0;
+  if (blockIdx.x >= args.rows) {
+    list_adapters(args, static_cast<int64_t>(blockIdx.x) - args.rows);
+    return;
+  }
+  quantise_row_twice<kVector>(args, blockIdx.x, block_max_values);
+}
+
+// Many rows: the units of 128 rows, shared by unit_groups clusters.  A programmatic dependent of lora_rows_kernel that does not need it: everything is read
+// through L2, and the wait stands at the end.
+template <bool kVector, int kRankTiles>
+__global__ void __launch_bounds__(kThreads, 2)
+lora_units_kernel(const __grid_constant__ FrontArgs args) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  UnitSums<kRankTiles>& sums = *reinterpret_cast<UnitSums<kRankTiles>*>(smem_raw);
+  __shared__ UnitList s;
+  ptx::launch_dependents();
+  const int cluster_rank = static_cast<int>(blockIdx.x) % args.cluster;
+  const int group = static_cast<int>(blockIdx.x) / args.cluster;
+  const int tile = group / args.unit_groups;
+  const int64_t row0 = static_cast<int64_t>(tile) * kTileRows;
+  list_units(s, args, row0);
+  int chunk_begin, chunk_end;
+  chunk_range(args, cluster_rank, &chunk_begin, &chunk_end);
+  const int rank_blocks = (args.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  const int work = s.units * rank_blocks;
+  for (int item = group - tile * args.unit_groups; item < work; item += args.unit_groups) {
+    const int index = item / rank_blocks;
+    const int rank0 = (item - index * rank_blocks) * kLoraRankBlock;
+    const int slot = s.unit_slot[index];
+    const int adapter = s.slot_adapter[slot];
+    const int order0 = s.unit_row[index];
+    const int count = min(kUnitRows, s.slot_first[slot] + s.slot_rows[slot] - order0);
+    const int ranks = min(kLoraRankBlock, args.adapters.rank - rank0);
+    const uint16_t* const a = args.adapters.a + (static_cast<int64_t>(adapter) * args.adapters.rank + rank0) * args.adapters.a_stride;
+    multiply_unit<kVector, kRankTiles, 4, kRankTiles == 1 ? 2 : 1>(args, args.x + row0 * args.k, s.order + order0, count, a, ranks, chunk_begin, chunk_end,
+                                                                   sums.part[threadIdx.x >> 5]);
+    finish_unit<kRankTiles, 4>(args, sums, cluster_rank, adapter, row0, s.order + order0, count, rank0, ranks);
+  }
+  ptx::grid_dependency_wait();  // this kernel's end stands for the end of the one in front too
+}
+
+template <typename Kernel>
+cudaError_t launch_clusters(Kernel kernel, const FrontArgs& args, int64_t blocks, size_t smem_bytes, bool chained, PerDeviceOnce* configured, cudaStream_t stream) {
+  const int device = current_device_ordinal();
+  if (configured->needed(device)) {
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes));
+    if (error != cudaSuccess) return error;
+    configured->mark(device);
+  }
+  if (blocks > (1ll << 31) - 1) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(blocks));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem_bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = static_cast<unsigned>(args.cluster);
+  attributes[0].val.clusterDim.y = 1;
+  attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = chained ? 2 : 1;
+  return cudaLaunchKernelEx(&config, kernel, args);
+}
+
+template <bool kVector, int kRankTiles>
+cudaError_t launch_front(FrontArgs args, cudaStream_t stream) {
+  const bool few = args.rows <= kFewRows;
+  const int tile_rows = few ? kUnitRows : kTileRows;
+  const int64_t tiles = (args.rows + tile_rows - 1) / tile_rows;
+  const int k32 = (args.k + 31) / 32;
+  args.cluster = 1;
+  const int rank_blocks = (args.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  // Units of a tile at most: its rows, and an adapter's groups of 32 rows.
+  const int64_t rows_in_tile = args.rows < tile_rows ? args.rows : tile_rows;
+  const int64_t by_adapter = args.adapters.count + (few ? 0 : rows_in_tile / kUnitRows);
+  const int64_t most = (by_adapter < rows_in_tile ? by_adapter : rows_in_tile) * rank_blocks;
+  // The K range is split over more CTAs the fewer units there are to fill the chip with: of few rows at most `most` a tile (two CTAs fit an SM), of many rows
+  // four a tile where requests follow each other and many more where they are mixed, so that the split ends with 16 clusters' worth of tiles (split for
+  // one unit in 32 rows, 2048 mixed rows of 7168 values with 64 adapters took 144 us instead of 83, for `most`, 1024 rows of 16384 in runs 171 instead of 138).
+  while (args.cluster < kMaxCluster && (few ? tiles * most * args.cluster <= threshold_sms : tiles * args.cluster < 16) && args.cluster * kWarps * 2 <= k32) {
+    args.cluster *= 2;
+  }
+  int64_t groups = 4ll * threshold_sms / (tiles * args.cluster);
+  if (groups < 4) groups = 4;
+  if (groups > most) groups = most;
+  args.unit_groups = static_cast<int>(groups);
+  const int64_t lists = args.lists != nullptr ? (args.rows + kLoraListRows - 1) / kLoraListRows : 0;
+  if (few) {
+    static PerDeviceOnce configured;
+    args.row_groups = static_cast<int>((rows_in_tile + args.cluster - 1) / args.cluster);
+    const int64_t blocks = tiles * (args.row_groups + args.unit_groups) * args.cluster + (lists + args.cluster - 1) / args.cluster * args.cluster;
+    return launch_clusters(lora_front_kernel<kVector, kRankTiles>, args, blocks, sizeof(UnitSums<kRankTiles>), false, &configured, stream);
+  }
+  if (args.rows + lists > (1ll << 31) - 1) return cudaErrorInvalidValue;
+  lora_rows_kernel<kVector><<<static_cast<unsigned>(args.rows + lists), kThreads, 0, stream>>>(args);
+  const cudaError_t error = cudaGetLastError();
+  if (error != cudaSuccess) return error;
+  static PerDeviceOnce configured;
+  return launch_clusters(lora_units_kernel<kVector, kRankTiles>, args, tiles * args.unit_groups * args.cluster, sizeof(UnitSums<kRankTiles>), true, &configured, stream);
+}
+
+template <bool kVector>
+cudaError_t launch_front_ranks(const FrontArgs& args, cudaStream_t stream) {
+  if (args.adapters.rank <= 16) return launch_front<kVector, 1>(args, stream);
+  if (args.adapters.rank <= 32) return launch_front<kVector, 2>(args, stream);
+  return launch_front<kVector, 4>(args, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_lora_front(const LoraGemmArgs& g, const uint16_t* x, int k, int8_t* q, float* scale, uint16_t* t, int* lists, int* row_slots, cudaStream_t stream) {
+  FrontArgs args = {};
+  args.x = x;
+  args.rows = g.rows;
+  args.k = k;
+  args.k_padded = g.k_padded;
+  args.adapters = g.adapters;
+  args.q = q;
+  args.scale = scale;
+  args.t = t;
+  args.planes = g.planes;
+  args.lists = lists;
+  args.row_slots = row_slots;
+  args.status = g.status;
+  const bool vector = k % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  return vector ? launch_front_ranks<true>(args, stream) : launch_front_ranks<false>(args, stream);
+}
+
+}  // namespace fmoe

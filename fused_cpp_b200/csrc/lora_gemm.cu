@@ -1,6 +1,6 @@
 // Dense W8A8 linear with the low-rank adapters of many requests:
 //   out[row, n] = (acc * row scale) * channel scale (+ bias[n]) + sum over r of t[row, r] B[a, n, r],   acc = Xq W^T, a = the row's adapter,
-// with the coefficients t of lora_shrink.cu.  The kernel of dense_gemm.cu (128 output channels of a cluster of `parts` CTAs that split the K
+// with the coefficients t of lora_front.cu.  The kernel of dense_gemm.cu (128 output channels of a cluster of `parts` CTAs that split the K
 // range; their int32 sums meet in distributed shared memory) with the adapters' product beside it, in a second accumulator of tensor memory:
 //   * Rows of a tile may have any adapters in any order.  For each adapter in use by the rows, [t of its rows, zeros for the others] x B[a]^T
 //     is one of bf16 MMAs: a K block of 128-byte rows, as the weights' are, holds 64 ranks of one adapter or two or four adapters of up to 32 or 16

@@ -67,3 +67,22 @@ def test_projection_with_adapters(cuda_device, rows, k, n, count, rank, dtype):
     got = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids, bias=bias, out_dtype=dtype)
     check(got, base, x, a, b, scaling, ids)
     assert torch.equal(got[ids < 0], base[ids < 0].to(dtype))  # a row without an adapter is the base product, bit for bit
+
+
+@pytest.mark.parametrize("rows, k, n, count, rank, none", [
+    (129, 256, 25000, 3, 16, 0.0), (256, 1536, 13000, 200, 33, 0.3), (700, 130, 4504, 2, 8, 0.9), (2000, 400, 1600, 900, 16, 0.1), (3000, 272, 1288, 4, 100, 0.2),
+    (5000, 129, 777, 50, 24, 0.1)])
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_rows(cuda_device, rows, k, n, count, rank, none, order, dtype):
+    """The sizes at which the two-SM kernel takes over, in wide and narrow tiles, aligned output rows and others, up to 200 adapters in 256 rows."""
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, bias = make(rows, k, n, count, rank, seed=rows, none=none)
+    if order == "runs":
+        ids = ids[torch.arange(rows, device=ids.device) // 300]
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    base = base_product(x, w, s, None)
+    got = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids, out_dtype=dtype)
+    check(got, base, x, a, b, scaling, ids)
+    assert torch.equal(got[ids < 0], base[ids < 0].to(dtype))
