@@ -8,8 +8,8 @@ activations, as plain tensors that an optimiser updates.  Both projections, the 
 second; the backward pass is three launches.  Sums are fp32; h = act(..) is rounded to bf16 for the down projection, as in the fused MoE
 operators.  `gated_mlp_forward` and `gated_mlp_backward` are the two passes for programs that keep their own tape.
 
-What a forward pass keeps for the backward pass besides its inputs: h [T, F] and the partial derivatives of h by gate and by up, 2 TF
-fp32 values in an order of the library's own.
+What a forward pass keeps for the backward pass besides its inputs, in one buffer: the partial derivatives of h by gate and by up (fp32, in an
+order of the library's own) and h [T, F].
 """
 from __future__ import annotations
 
@@ -86,22 +86,29 @@ def _whole(tensor: torch.Tensor) -> torch.Tensor:
     return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()
 
 
-def _derivative_count(rows: int, inter: int) -> int:
-    """fmoe_gated_mlp_derivative_count: whole blocks of 32 rows x 32 channels x 2."""
-    return -(-rows // 32) * -(-inter // 32) * 2048
+def _derivative_bytes(rows: int, inter: int) -> int:
+    """4 * fmoe_gated_mlp_derivative_count: whole blocks of 32 rows x 32 channels x 2."""
+    return -(-rows // 32) * -(-inter // 32) * 8192
+
+
+def _kept_bytes(rows: int, inter: int) -> int:
+    """The derivatives, then h."""
+    return _derivative_bytes(rows, inter) + 2 * rows * inter
 
 
 def _forward(index: int, rows, w13, w2, code: int, limit: float, keep: bool, y):
+    """y, and what the backward pass needs (keep) or h alone, in one buffer (the caller's, so that it outlives the kernels on this stream)."""
     count, hidden = rows.shape
     inter = w2.shape[1]
-    h = rows.new_empty((count, inter))
-    derivatives = rows.new_empty(_derivative_count(count, inter), dtype=torch.float32) if keep else None
+    front = _derivative_bytes(count, inter) if keep else 0
+    kept = rows.new_empty(front + 2 * count * inter, dtype=torch.uint8)
+    address = kept.data_ptr()
     _lib.check(_lib.load().fmoe_gated_mlp_forward(rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), count, hidden, inter, code, limit,
-                                                  h.data_ptr(), derivatives.data_ptr() if keep else None, y.data_ptr(), _lib._stream_of(index)))
-    return h, derivatives
+                                                  address + front, address if keep else None, y.data_ptr(), _lib._stream_of(index)))
+    return kept
 
 
-def _backward(index: int, dy, rows, w13, w2, h, derivatives, need_x: bool, need_w13: bool, need_w2: bool):
+def _backward(index: int, dy, rows, w13, w2, kept, need_x: bool, need_w13: bool, need_w2: bool):
     count, hidden = rows.shape
     inter = w2.shape[1]
     if count == 0:
@@ -112,9 +119,10 @@ def _backward(index: int, dy, rows, w13, w2, h, derivatives, need_x: bool, need_
     dw2 = rows.new_empty((hidden, inter)) if need_w2 else None
     scratch = rows.new_empty((count, 2 * inter)) if need_x or need_w13 else None
     pointer = _lib._ptr
-    _lib.check(_lib.load().fmoe_gated_mlp_backward(dy.data_ptr(), _stride(dy), rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), h.data_ptr(),
-                                                   pointer(derivatives), count, hidden, inter, pointer(scratch), pointer(dx), pointer(dw13),
-                                                   pointer(dw2), _lib._stream_of(index)))
+    address = kept.data_ptr()
+    _lib.check(_lib.load().fmoe_gated_mlp_backward(dy.data_ptr(), _stride(dy), rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(),
+                                                   address + _derivative_bytes(count, inter), address, count, hidden, inter, pointer(scratch),
+                                                   pointer(dx), pointer(dw13), pointer(dw2), _lib._stream_of(index)))
     return dx, dw13, dw2
 
 
@@ -127,10 +135,7 @@ class _GatedMLP(torch.autograd.Function):
     def _forward(ctx, input, w13, w2, code, limit, index):
         rows = _rows(input, w2.shape[0])
         y = rows.new_empty(input.shape)
-        need_x, need_w13 = ctx.needs_input_grad[:2]
-        # dW2 needs h alone, dx and dW13 the derivatives.
-        h, derivatives = _forward(index, rows, _whole(w13), _whole(w2), code, limit, need_x or need_w13, y)
-        ctx.save_for_backward(input, w13, w2, h, derivatives)
+        ctx.save_for_backward(input, w13, w2, _forward(index, rows, _whole(w13), _whole(w2), code, limit, True, y))
         ctx.index = index
         return y
 
@@ -142,10 +147,9 @@ class _GatedMLP(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, dy):
-        input, w13, w2, h, derivatives = ctx.saved_tensors
+        input, w13, w2, kept = ctx.saved_tensors
         hidden = w2.shape[0]
-        needs = ctx.needs_input_grad
-        dx, dw13, dw2 = _backward(ctx.index, _rows(dy, hidden), _rows(input, hidden), _whole(w13), _whole(w2), h, derivatives, needs[0], needs[1], needs[2])
+        dx, dw13, dw2 = _backward(ctx.index, _rows(dy, hidden), _rows(input, hidden), _whole(w13), _whole(w2), kept, *ctx.needs_input_grad[:3])
         return dx if dx is None or input.dim() == 2 else dx.view(input.shape), dw13, dw2, None, None, None
 
 
@@ -178,7 +182,7 @@ def _serve(index: int, input, w13, w2, code: int, limit: float, out):
 
 
 def gated_mlp_forward(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float | None = None):
-    """The forward pass without a tape: (y, h, derivatives), the last two for `gated_mlp_backward`."""
+    """The forward pass without a tape: (y, kept), the second for `gated_mlp_backward`."""
     hidden, _, index = _check(input, w13, w2)
     code, limit = _activation(activation, swiglu_limit)
     _require_cuda(index)
@@ -186,30 +190,27 @@ def gated_mlp_forward(input, w13, w2, *, activation: Any = "silu", swiglu_limit:
     def call():
         rows = _rows(input.detach(), hidden)
         y = rows.new_empty(input.shape)
-        return (y, *_forward(index, rows, _whole(w13.detach()), _whole(w2.detach()), code, limit, True, y))
+        return y, _forward(index, rows, _whole(w13.detach()), _whole(w2.detach()), code, limit, True, y)
 
     return _lib.on_device(index, call)
 
 
-def gated_mlp_backward(dy, input, w13, w2, h, derivatives, *, needs: tuple = (True, True, True)):
-    """(dx, dw13, dw2) from dy [..., H] and what `gated_mlp_forward` returned; None where `needs` says so."""
+def gated_mlp_backward(dy, input, w13, w2, kept, *, needs: tuple = (True, True, True)):
+    """(dx, dw13, dw2) from dy [..., H] and what `gated_mlp_forward` kept; None where `needs` says so."""
     hidden, inter, index = _check(input, w13, w2)
     _check_tensor("dy", dy, index)
-    _check_tensor("h", h, index)
-    if not isinstance(derivatives, torch.Tensor) or derivatives.dtype is not torch.float32 or derivatives.get_device() != index:
-        raise TypeError("derivatives must be the float32 tensor that gated_mlp_forward returned")
     if dy.shape != input.shape:
         raise ValueError(f"dy must have the input's shape {tuple(input.shape)}, got {tuple(dy.shape)}")
-    rows = input.numel() // hidden
-    if h.shape != (rows, inter) or derivatives.shape != (_derivative_count(rows, inter),) or not h.is_contiguous() or not derivatives.is_contiguous():
-        raise ValueError("h and derivatives must be what gated_mlp_forward returned for this input")
+    if not isinstance(kept, torch.Tensor) or kept.dtype is not torch.uint8 or kept.get_device() != index or not kept.is_contiguous() \
+            or kept.shape != (_kept_bytes(input.numel() // hidden, inter),):
+        raise ValueError("kept must be what gated_mlp_forward returned for this input")
     if len(needs) != 3:
         raise ValueError("needs must say for dx, dw13 and dw2 whether they are wanted")
     _require_cuda(index)
 
     def call():
-        dx, dw13, dw2 = _backward(index, _rows(dy.detach(), hidden), _rows(input.detach(), hidden), _whole(w13.detach()), _whole(w2.detach()),
-                                  _whole(h.detach()), _whole(derivatives), *(bool(need) for need in needs))
+        dx, dw13, dw2 = _backward(index, _rows(dy.detach(), hidden), _rows(input.detach(), hidden), _whole(w13.detach()), _whole(w2.detach()), kept,
+                                  *(bool(need) for need in needs))
         return None if dx is None else dx.view(input.shape), dw13, dw2
 
     return _lib.on_device(index, call)

@@ -35,21 +35,21 @@ def test_refusals(changes, error, text):
 
 @pytest.mark.parametrize("rows, inter", [(0, 8), (1, 8), (32, 32), (33, 40), (1333, 1024)])
 def test_kept_derivatives_have_the_size_the_library_wants(rows, inter):
-    assert gated._derivative_count(rows, inter) == _lib.load().fmoe_gated_mlp_derivative_count(rows, inter)
+    assert gated._derivative_bytes(rows, inter) == 4 * _lib.load().fmoe_gated_mlp_derivative_count(rows, inter)
+    assert gated._kept_bytes(rows, inter) == gated._derivative_bytes(rows, inter) + 2 * rows * inter
 
 
 def test_backward_refusals():
     x, w13, w2 = (torch.zeros(*shape, dtype=torch.bfloat16) for shape in ((3, 16), (48, 16), (16, 24)))
-    h, derivatives = torch.zeros(3, 24, dtype=torch.bfloat16), torch.zeros(2048)
+    kept = torch.zeros(gated._kept_bytes(3, 24), dtype=torch.uint8)
     with pytest.raises(ValueError, match="input's shape"):
-        moe.gated_mlp_backward(x[:2], x, w13, w2, h, derivatives)
-    with pytest.raises(ValueError, match="what gated_mlp_forward returned"):
-        moe.gated_mlp_backward(x, x, w13, w2, h[:, :16], derivatives)
+        moe.gated_mlp_backward(x[:2], x, w13, w2, kept)
+    for wrong in (kept[:-1], kept.to(torch.int8), None):
+        with pytest.raises(ValueError, match="what gated_mlp_forward returned"):
+            moe.gated_mlp_backward(x, x, w13, w2, wrong)
     with pytest.raises(TypeError, match="dy must be torch.bfloat16"):
-        moe.gated_mlp_backward(x.float(), x, w13, w2, h, derivatives)
-    with pytest.raises(TypeError, match="derivatives must be the float32"):
-        moe.gated_mlp_backward(x, x, w13, w2, h, derivatives.bfloat16())
+        moe.gated_mlp_backward(x.float(), x, w13, w2, kept)
     with pytest.raises(ValueError, match="needs"):
-        moe.gated_mlp_backward(x, x, w13, w2, h, derivatives, needs=(True,))
+        moe.gated_mlp_backward(x, x, w13, w2, kept, needs=(True,))
     with pytest.raises(ValueError, match="CUDA"):
-        moe.gated_mlp_backward(x, x, w13, w2, h, derivatives)
+        moe.gated_mlp_backward(x, x, w13, w2, kept)

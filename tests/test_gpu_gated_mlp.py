@@ -92,3 +92,201 @@ def test_block_and_gradients(cuda_device, tokens, hidden, inter, activation, lim
     with torch.no_grad():
         assert torch.equal(moe.gated_mlp(x, w13, w2, activation=activation, swiglu_limit=limit), got["y"])
     assert _lib.dense_status() == (0, 0)
+
+
+def test_passes_without_a_tape(cuda_device):
+    from fused_cpp_b200 import moe
+
+    for tokens, hidden, inter in ((5, 64, 40), (300, 264, 136)):
+        x, w13, w2, dy = make(tokens, hidden, inter)
+        want = run(moe, x, w13, w2, dy, "silu", 10.0)
+        y, kept = moe.gated_mlp_forward(x, w13, w2, swiglu_limit=10.0)
+        assert torch.equal(y, want["y"])
+        for needs in ((True, True, True), (True, False, False), (False, True, False), (False, False, True), (False, False, False)):
+            got = moe.gated_mlp_backward(dy, x, w13, w2, kept, needs=needs)
+            for name, need, value in zip(("dx", "dw13", "dw2"), needs, got):
+                assert (value is None) if not need else torch.equal(value, want[name]), (needs, name)
+
+
+def test_gradients_of_some_inputs(cuda_device):
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(70, 128, 72)
+    want = run(moe, x, w13, w2, dy)
+    for chosen in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        leaves = [t.detach().requires_grad_(i in chosen) for i, t in enumerate((x, w13, w2))]
+        y = moe.gated_mlp(*leaves)
+        grads = torch.autograd.grad(y, [leaves[i] for i in chosen], dy, retain_graph=True)
+        again = torch.autograd.grad(y, [leaves[i] for i in chosen], dy)
+        for i, grad, second in zip(chosen, grads, again):
+            assert torch.equal(grad, want[("dx", "dw13", "dw2")[i]]) and torch.equal(grad, second)
+
+
+def test_leaves_accumulate_and_shared_weights(cuda_device):
+    """Two uses of the same weights add their gradients; leaves take them in .grad."""
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(40, 64, 48)
+    a = run(moe, x, w13, w2, dy)
+    b = run(moe, x.flip(0), w13, w2, dy)
+    leaves = [t.detach().requires_grad_(True) for t in (w13, w2)]
+    (moe.gated_mlp(x, *leaves) * dy).sum().backward()
+    (moe.gated_mlp(x.flip(0), *leaves) * dy).sum().backward()
+    assert torch.equal(leaves[0].grad, a["dw13"] + b["dw13"]) and torch.equal(leaves[1].grad, a["dw2"] + b["dw2"])
+
+
+def test_second_derivative_is_refused(cuda_device):
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(4, 16, 8)
+    leaves = [t.requires_grad_(True) for t in (x, w13, w2)]
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(moe.gated_mlp(*leaves), leaves, dy, create_graph=True)
+
+
+def test_differences(cuda_device):
+    """The gradient against central differences of the block itself along random directions.  A difference of y over 2e carries two roundings of every y,
+    2 u |y| / 2e at most each weighted by |dy|, of h as many inside, and a third-order term e^2 |f'''| / 6 which a small e leaves below them."""
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(64, 128, 64)
+    got = run(moe, x, w13, w2, dy)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for name, index in (("dx", 0), ("dw13", 1), ("dw2", 2)):
+        tensors = [x, w13, w2]
+        direction = torch.randn(tensors[index].shape, generator=g, device="cuda")
+        step = 0.25 * tensors[index].float().std() * direction
+        low, high = ((tensors[index].float() + sign * step).bfloat16() for sign in (-1, 1))
+        values = []
+        for moved in (low, high):
+            tensors[index] = moved
+            values.append(moe.gated_mlp(*tensors).double())
+        # Along the path from low to high the gradient changes: compare with the mean of the gradients at both ends and in the middle (Simpson).
+        ends = []
+        for moved in (low, high):
+            tensors[index] = moved
+            ends.append(run(moe, *tensors, dy)[name].double())
+        mean = (ends[0] + 4 * got[name].double() + ends[1]) / 6
+        moved = high.double() - low.double()
+        change = ((values[1] - values[0]) * dy.double()).sum()
+        predicted = (mean * moved).sum()
+        # Independent roundings: the sum's standard deviation is u |dy| |y| sqrt(2) at most for y and as much for h; six of them, and 2 % for Simpson's remainder.
+        noise = 6 * 2 * STEP * (2 ** 0.5) * ((values[0].abs() + values[1].abs()) / 2 * dy.double().abs()).norm() + 0.02 * (mean * moved).abs().sum().sqrt() * (mean * moved).norm().sqrt()
+        assert (change - predicted).abs() <= noise, (name, change.item(), predicted.item(), noise.item())
+
+
+def test_no_rows(cuda_device):
+    from fused_cpp_b200 import moe
+
+    _, w13, w2, _ = make(1, 64, 32)
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    got = run(moe, x, w13, w2, x)
+    assert got["y"].shape == (0, 64) and got["dx"].shape == (0, 64)
+    assert not got["dw13"].any() and not got["dw2"].any() and got["dw13"].shape == w13.shape
+
+
+@pytest.mark.parametrize("tokens", [3, 300])
+def test_layouts(cuda_device, tokens):
+    """Rows of a wider matrix, an unaligned view, a transposed matrix, a broadcast dy, three dimensions, weights that are views: the same results."""
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(tokens, 136, 72)
+    want = run(moe, x, w13, w2, dy)
+    wide = torch.randn(tokens, 400, device="cuda").bfloat16()
+    wide[:, 8:144] = x
+    odd = torch.empty(tokens * 136 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(tokens, 136)
+    odd.copy_(x)
+    stacked = torch.randn(3, *w13.shape, device="cuda").bfloat16()
+    stacked[1] = w13
+    for form, weights in ((wide[:, 8:144], (w13, w2)), (odd, (w13, w2)), (x.t().contiguous().t(), (w13, w2)), (x, (stacked[1], w2.t().contiguous().t()))):
+        got = run(moe, form, *weights, dy)
+        for name in want:
+            assert torch.equal(got[name], want[name]), name
+    for form in (wide[:, 8:144].clone(), dy.t().contiguous().t()):
+        assert torch.equal(run(moe, x, w13, w2, form)["dx"], run(moe, x, w13, w2, form.contiguous())["dx"])
+    row = dy[:1].expand(tokens, -1)
+    assert torch.equal(run(moe, x, w13, w2, row)["dw13"], run(moe, x, w13, w2, row.contiguous())["dw13"])
+    cube = run(moe, x.view(1, tokens, 136), w13, w2, dy.view(1, tokens, 136))
+    assert cube["dx"].shape == (1, tokens, 136) and torch.equal(cube["dx"][0], want["dx"]) and torch.equal(cube["dw2"], want["dw2"])
+    vector = run(moe, x[0], w13, w2, dy[0])
+    assert vector["y"].shape == (136,) and torch.equal(vector["y"], run(moe, x[:1], w13, w2, dy[:1])["y"][0])
+    out = torch.empty(tokens * 136 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(tokens, 136)
+    assert moe.gated_mlp(x, w13, w2, out=out) is out and torch.equal(out, want["y"])
+    with pytest.raises(ValueError, match="out must be contiguous"):
+        moe.gated_mlp(x, w13, w2, out=wide[:, 8:144])
+    with pytest.raises(ValueError, match="gradients are asked for"):
+        moe.gated_mlp(x.requires_grad_(True), w13, w2, out=out)
+
+
+@pytest.mark.parametrize("tokens", [2, 260])
+def test_not_finite(cuda_device, tokens):
+    """A NaN or an infinity in one row stays in that row of y and dx; a limit does not hide a NaN."""
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(tokens, 64, 48)
+    want = run(moe, x, w13, w2, dy, "silu", 10.0)
+    for bad in (float("nan"), float("inf")):
+        broken = x.clone()
+        broken[1, 5] = bad
+        got = run(moe, broken, w13, w2, dy, "silu", 10.0)
+        keep = torch.arange(tokens, device="cuda") != 1
+        assert torch.equal(got["y"][keep], want["y"][keep]) and torch.equal(got["dx"][keep], want["dx"][keep])
+        if bad != bad:
+            assert got["y"][1].isnan().all() and got["dw13"].isnan().any()
+
+
+def test_streams_and_graphs(cuda_device):
+    """Calls on two streams at once, and two captured graphs that are replayed in turn on new inputs, each with buffers of its own."""
+    from fused_cpp_b200 import moe
+
+    sets = [make(tokens, 256, 128, seed=tokens) for tokens in (40, 600)]
+    want = [run(moe, *s, "silu", 10.0) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for stream, s in zip(streams, sets):
+            with torch.cuda.stream(stream):
+                got.append(run(moe, *s, "silu", 10.0))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(a[name], b[name]) for name in a)
+    graphs = []
+    for s in sets:
+        leaves = [t.clone() for t in s]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(moe, *leaves, "silu", 10.0)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs = run(moe, *leaves, "silu", 10.0)
+        graphs.append((graph, leaves, outputs))
+    for round_ in range(3):
+        fresh = [make(s[0].shape[0], 256, 128, seed=100 + round_) for s in sets]
+        for (graph, leaves, _), new in zip(graphs, fresh):
+            for to, value in zip(leaves, new):
+                to.copy_(value)
+            graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, outputs), new in zip(graphs, fresh):
+            expected = run(moe, *new, "silu", 10.0)
+            assert all(torch.equal(outputs[name], expected[name]) for name in outputs)
+
+
+def test_first_call_of_a_thread(cuda_device):
+    """A thread whose first call into CUDA is the backward pass (an autograd worker's, or any other)."""
+    import threading
+
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(20, 64, 48)
+    want = run(moe, x, w13, w2, dy)
+    y, kept = moe.gated_mlp_forward(x, w13, w2)
+    torch.cuda.synchronize()
+    found = []
+    thread = threading.Thread(target=lambda: found.append(moe.gated_mlp_backward(dy, x, w13, w2, kept)))
+    thread.start()
+    thread.join()
+    assert len(found) == 1 and torch.equal(found[0][0], want["dx"]) and torch.equal(found[0][1], want["dw13"])

@@ -86,3 +86,156 @@ def test_many_rows(cuda_device, rows, k, n, count, rank, none, order, dtype):
     got = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids, out_dtype=dtype)
     check(got, base, x, a, b, scaling, ids)
     assert torch.equal(got[ids < 0], base[ids < 0].to(dtype))
+
+
+def test_layouts_ids_and_ranks(cuda_device):
+    """Ids of both integer types and out of range, rows in three dimensions, a strided x and strided ids, adapters of unequal ranks, one scaling for all."""
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, bias = make(60, 264, 200, 4, 24)
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    want = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids, bias=bias)
+    assert torch.equal(i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids.int(), bias=bias), want)
+    for outside in (4, 2 ** 31 - 1, -(2 ** 31)):
+        far = torch.where(ids < 0, torch.full_like(ids, outside), ids)
+        assert torch.equal(i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, far, bias=bias), want)
+        assert torch.equal(i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, far.int(), bias=bias), want)
+    assert torch.equal(i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, torch.where(ids < 0, ids + 2 ** 40, ids), bias=bias), want)
+    cube = i8gemm.dynamic_scaled_mm_lora(x.view(3, 20, 264), packed, adapters, ids.view(3, 20), bias=bias)
+    assert cube.shape == (3, 20, 200) and torch.equal(cube.view(60, 200), want)
+    wide = torch.zeros(60, 300, dtype=torch.bfloat16, device="cuda")
+    wide[:, 3:267] = x
+    strided = torch.stack((ids, ids), 1)[:, 0]
+    assert torch.equal(i8gemm.dynamic_scaled_mm_lora(wide[:, 3:267], packed, adapters, strided, bias=bias), want)
+    empty = i8gemm.dynamic_scaled_mm_lora(x[:0], packed, adapters, ids[:0])
+    assert empty.shape == (0, 200) and empty.dtype == torch.bfloat16
+    # Unequal ranks, padded with zeros: the same as whole adapters whose other ranks are zero.
+    ranks = (24, 3, 17, 1)
+    cut = [(a[i, :r], b[i, :, :r]) for i, r in enumerate(ranks)]
+    whole_a, whole_b = a.clone(), b.clone()
+    for i, r in enumerate(ranks):
+        whole_a[i, r:] = 0
+        whole_b[i, :, r:] = 0
+    unequal = lora.prepare_adapters([p[0] for p in cut], [p[1].cpu() for p in cut], 0.5)
+    assert unequal.rank == 24 and unequal.scaling.tolist() == [0.5] * 4
+    equal = lora.prepare_adapters(whole_a, whole_b, [0.5] * 4)
+    assert torch.equal(i8gemm.dynamic_scaled_mm_lora(x, packed, unequal, ids), i8gemm.dynamic_scaled_mm_lora(x, packed, equal, ids))
+
+
+def test_a_slot_is_exchanged_in_place(cuda_device):
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, _ = make(40, 256, 136, 3, 16)
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    before = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids)
+    new_a, new_b = a[1, :9].flip(1).contiguous(), b[1, :, :9].flip(0).contiguous()
+    lora.set_adapter(adapters, 1, new_a, new_b, 0.75)
+    after = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids)
+    assert torch.equal(after[ids != 1], before[ids != 1])
+    a, b, scaling = a.clone(), b.clone(), scaling.clone()
+    a[1], b[1] = 0, 0
+    a[1, :9], b[1, :, :9], scaling[1] = new_a, new_b, 0.75
+    check(after, base_product(x, w, s, None), x, a, b, scaling, ids)
+
+
+@pytest.mark.parametrize("rows", [40, 200, 1000])
+def test_a_row_depends_on_itself_alone(cuda_device, rows):
+    """Neighbours, their adapters, NaN and infinities among them, and the row's place change no bit of it, as long as the same kernel serves the batch."""
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, bias = make(rows, 512, 5000, 6, 16)
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    want = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids, bias=bias)
+    order = torch.randperm(rows, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    assert torch.equal(i8gemm.dynamic_scaled_mm_lora(x[order], packed, adapters, ids[order], bias=bias), want[order])
+    broken, other = x.clone(), ids.clone()
+    broken[::3, 7] = float("nan")
+    broken[1::3, 9] = float("inf")
+    other[::3] = (other[::3] + 1) % 6
+    got = i8gemm.dynamic_scaled_mm_lora(broken, packed, adapters, other, bias=bias)
+    assert torch.equal(got[2::3], want[2::3])
+
+
+@pytest.mark.parametrize("a_value, b_value", [(float("inf"), 1.0), (1.0, float("nan"))])
+def test_adapters_that_are_not_finite_are_refused(cuda_device, a_value, b_value):
+    from fused_cpp_b200 import lora
+
+    a, b = torch.ones(2, 4, 16).bfloat16(), torch.ones(2, 24, 4).bfloat16()
+    a[1, 2, 3], b[1, 2, 3] = a_value, b_value
+    with pytest.raises(ValueError, match="finite"):
+        lora.prepare_adapters(a, b)
+    with pytest.raises(ValueError, match="finite"):
+        lora.prepare_adapters(a[:1], b[:1], float("inf"))
+
+
+def test_refusals_on_the_gpu(cuda_device):
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, bias = make(10, 64, 48, 2, 8)
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    mm = i8gemm.dynamic_scaled_mm_lora
+    for call, error, text in (
+            (lambda: mm(x.float(), packed, adapters, ids), TypeError, "CUDA bfloat16"),
+            (lambda: mm(x[:, :32], packed, adapters, ids), ValueError, "K=64"),
+            (lambda: mm(x, packed, lora.prepare_adapters(a[:, :, :32], b), ids), ValueError, "beside a weight"),
+            (lambda: mm(x, packed, adapters, ids[:4]), ValueError, "one per row"),
+            (lambda: mm(x, packed, adapters, ids.float()), TypeError, "int32 or int64"),
+            (lambda: mm(x, packed, adapters, ids.cpu()), ValueError, "input's device"),
+            (lambda: mm(x, packed, adapters, ids, bias=bias[:4]), ValueError, "bias must be"),
+            (lambda: mm(x, packed, adapters, ids, out_dtype=torch.float16), ValueError, "out_dtype"),
+            (lambda: mm(x, packed, adapters, ids, nthreads=-1), ValueError, "non-negative")):
+        with pytest.raises(error, match=text):
+            call()
+
+
+def test_streams_and_graphs(cuda_device):
+    """Calls on two streams at once, and two captured graphs replayed in turn on new rows and ids, each with a workspace of its own."""
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, bias = make(700, 512, 5000, 6, 16)
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    parts = [(x[:30], ids[:30]), (x[30:], ids[30:])]
+    want = [i8gemm.dynamic_scaled_mm_lora(*p[:1], packed, adapters, p[1], bias=bias) for p in parts]
+    streams = [torch.cuda.Stream() for _ in parts]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for stream, p in zip(streams, parts):
+            with torch.cuda.stream(stream):
+                got.append(i8gemm.dynamic_scaled_mm_lora(p[0], packed, adapters, p[1], bias=bias))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, e) for g, e in zip(got, want))
+    graphs = []
+    for p in parts:
+        inputs = (p[0].clone(), p[1].clone())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = i8gemm.dynamic_scaled_mm_lora(inputs[0], packed, adapters, inputs[1], bias=bias)
+        graphs.append((graph, inputs, out))
+    for round_ in range(3):
+        for graph, inputs, _ in graphs:
+            inputs[0].copy_(inputs[0].flip(0))
+            inputs[1].copy_((inputs[1] + 1 + round_) % 7 - 1)
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, inputs, out in graphs:
+            assert torch.equal(out, i8gemm.dynamic_scaled_mm_lora(inputs[0], packed, adapters, inputs[1], bias=bias))
+
+
+def test_attention_output_then_feed_forward(cuda_device):
+    """The two operators one after the other, as a layer has them: the attention's output projection with the requests' adapters, then the gated block, and the
+    block's weights learning from what comes out."""
+    from fused_cpp_b200 import i8gemm, lora, moe
+
+    x, w, s, a, b, scaling, ids, _ = make(50, 512, 256, 4, 16)
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w13 = (torch.randn(256, 256, generator=g, device="cuda") / 16).bfloat16().requires_grad_(True)
+    w2 = (torch.randn(256, 128, generator=g, device="cuda") / 12).bfloat16().requires_grad_(True)
+    projected = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids)
+    check(projected, base_product(x, w, s, None), x, a, b, scaling, ids)
+    y = moe.gated_mlp(projected, w13, w2, swiglu_limit=10.0)
+    with torch.no_grad():
+        assert torch.equal(y, moe.gated_mlp(projected, w13, w2, swiglu_limit=10.0))
+    y.float().square().mean().backward()
+    assert w13.grad.isfinite().all() and w13.grad.any() and w2.grad.any()
