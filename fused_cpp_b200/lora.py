@@ -9,6 +9,7 @@ Row m of a batch gets scaling[a] * B[a] (A[a] x[m]) added to its projection, a =
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass, field
 from typing import Sequence
 
@@ -110,6 +111,11 @@ def set_adapter(adapters: PreparedAdapters, index: int, a: torch.Tensor, b: torc
         adapters.scaling[index] = float(scaling)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, k: int, rank: int, out_is_bf16: int) -> int:
+    return _lib.load().fmoe_i8gemm_lora_workspace_bytes(rows, k, rank, out_is_bf16)
+
+
 def projection(index: int, x: torch.Tensor, packed, adapters: PreparedAdapters, adapter_ids: torch.Tensor, bias: torch.Tensor | None,
                out: torch.Tensor) -> None:
     """out [..., N] of bf16 rows x [..., K] on CUDA device `index`, checked by the caller; the workspace is the call's own, so that calls on
@@ -121,7 +127,7 @@ def projection(index: int, x: torch.Tensor, packed, adapters: PreparedAdapters, 
     rows, k = x.numel() // packed.k, packed.k
     lib = _lib.load()
     out_is_bf16 = 1 if out.dtype is torch.bfloat16 else 0
-    nbytes = lib.fmoe_i8gemm_lora_workspace_bytes(rows, k, adapters.rank, out_is_bf16)
+    nbytes = _workspace_bytes(rows, k, adapters.rank, out_is_bf16)
     workspace = x.new_empty(nbytes, dtype=torch.uint8)
     _lib.check(lib.fmoe_i8gemm_dynamic_scaled_mm_lora(
         x.data_ptr(), rows, k, packed.packed_weight.data_ptr(), packed.weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), packed.n,

@@ -75,6 +75,11 @@ def _rows(tensor: torch.Tensor, columns: int) -> torch.Tensor:
     return rows if rows.data_ptr() % 16 == 0 else rows.clone()
 
 
+def _like(input: torch.Tensor) -> torch.Tensor:
+    """A contiguous result of the input's shape."""
+    return torch.empty_like(input) if input.is_contiguous() else input.new_empty(input.shape)
+
+
 def _stride(rows: torch.Tensor) -> int:
     """Elements from a row to the next; a single row may carry any stride."""
     return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
@@ -114,9 +119,9 @@ def _backward(index: int, dy, rows, w13, w2, kept, need_x: bool, need_w13: bool,
     if count == 0:
         return (rows.new_zeros((0, hidden)) if need_x else None, w13.new_zeros(w13.shape) if need_w13 else None,
                 w2.new_zeros(w2.shape) if need_w2 else None)
-    dx = rows.new_empty((count, hidden)) if need_x else None
-    dw13 = rows.new_empty((2 * inter, hidden)) if need_w13 else None
-    dw2 = rows.new_empty((hidden, inter)) if need_w2 else None
+    dx = _like(rows) if need_x else None
+    dw13 = torch.empty_like(w13) if need_w13 else None
+    dw2 = torch.empty_like(w2) if need_w2 else None
     scratch = rows.new_empty((count, 2 * inter)) if need_x or need_w13 else None
     pointer = _lib._ptr
     address = kept.data_ptr()
@@ -134,7 +139,7 @@ class _GatedMLP(torch.autograd.Function):
     @staticmethod
     def _forward(ctx, input, w13, w2, code, limit, index):
         rows = _rows(input, w2.shape[0])
-        y = rows.new_empty(input.shape)
+        y = _like(input)
         ctx.save_for_backward(input, w13, w2, _forward(index, rows, _whole(w13), _whole(w2), code, limit, True, y))
         ctx.index = index
         return y
@@ -157,7 +162,10 @@ def gated_mlp(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float |
     """bf16 [..., H] x w13 [2F, H], w2 [H, F] -> bf16 [..., H]; differentiable by input, w13 and w2 (once).
 
     activation: "silu", "gelu" or "swigluoai"; swiglu_limit: None, 0 or 10.0 (with "silu").  H and F are multiples of 8.  With `out`
-    (contiguous, no gradients asked for) the result is written there and `out` returned."""
+    (contiguous, no gradients asked for) the result is written there and `out` returned.
+
+    Both passes can be captured into a CUDA graph.  As with any function of torch, the engine refuses to capture a backward pass while an eager
+    graph of the same leaves lives; `gated_mlp_forward` and `gated_mlp_backward` have no such condition."""
     _, _, index = _check(input, w13, w2)
     code, limit = _activation(activation, swiglu_limit)
     _require_cuda(index)
@@ -171,7 +179,7 @@ def gated_mlp(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float |
 def _serve(index: int, input, w13, w2, code: int, limit: float, out):
     rows = _rows(input, w2.shape[0])
     if out is None:
-        y = out = rows.new_empty(input.shape)
+        y = out = _like(input)
     else:
         _check_tensor("out", out, index)
         if out.shape != input.shape or not out.is_contiguous():
@@ -189,7 +197,7 @@ def gated_mlp_forward(input, w13, w2, *, activation: Any = "silu", swiglu_limit:
 
     def call():
         rows = _rows(input.detach(), hidden)
-        y = rows.new_empty(input.shape)
+        y = _like(rows).view(input.shape)
         return y, _forward(index, rows, _whole(w13.detach()), _whole(w2.detach()), code, limit, True, y)
 
     return _lib.on_device(index, call)

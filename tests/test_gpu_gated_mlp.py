@@ -290,3 +290,20 @@ def test_first_call_of_a_thread(cuda_device):
     thread.start()
     thread.join()
     assert len(found) == 1 and torch.equal(found[0][0], want["dx"]) and torch.equal(found[0][1], want["dw13"])
+
+
+def test_passes_without_a_tape_are_captured_beside_an_eager_graph(cuda_device):
+    """The two passes have no leaves whose accumulators an eager graph could have tied to another stream."""
+    from fused_cpp_b200 import moe
+
+    leaves = [t.requires_grad_(True) for t in make(48, 128, 64)[:3]]
+    dy = make(48, 128, 64)[3]
+    alive = moe.gated_mlp(*leaves)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, kept = moe.gated_mlp_forward(*leaves)
+        grads = moe.gated_mlp_backward(dy, *leaves, kept)
+    graph.replay()
+    assert torch.equal(y, alive.detach())
+    for got, want in zip(grads, torch.autograd.grad(alive, leaves, dy)):
+        assert torch.equal(got, want)
