@@ -23,8 +23,21 @@ __host__ __device__ __forceinline__ int64_t derivative_block(int64_t row0, int c
 template <typename Tag>
 __device__ __forceinline__ void gated_with_derivatives(Tag, float gate, float up, float limit, float* h, float* by_gate, float* by_up) {
   if constexpr (Tag::value == FMOE_ACT_GELU) {
-    const float cdf = normcdff(gate);  // 0.5 (1 + erf) would lose the values of the left tail
-    const float density = 0.39894228040143267794f * __expf(-0.5f * gate * gate);
+    // Phi(-a) = e^(-a^2/2) Q(a) for a >= 0, with Q(a) = erfcx(a / sqrt 2) / 2 fitted here (least squares, reweighted towards the largest relative error) by a polynomial in
+    // t = 1 / (1 + 0.36 a): within 1e-6 of its value on [0, 14.5], behind which e^(-a^2/2) is 0 in 32 bits.  The left tail keeps its relative precision, which
+    // 0.5 (1 + erf) loses, and the one exponential serves the density too (forward and backward of 1333 rows of 2048 x 1024: 97 us with normcdff, 75 like this).
+    const float a = fabsf(gate);
+    const float e = __expf(-0.5f * a * a);
+    const float t = __fdividef(1.0f, fmaf(0.36f, a, 1.0f));
+    float q = fmaf(0.046782233718879906f, t, -0.17882609622498481f);
+    q = fmaf(q, t, 0.1796773446277012f);
+    q = fmaf(q, t, 0.027426644660340928f);
+    q = fmaf(q, t, 0.13940009972259584f);
+    q = fmaf(q, t, 0.14183037149665473f);
+    q = fmaf(q, t, 0.14370896987904766f);
+    const float tail = e * q * t;
+    const float cdf = gate < 0.0f ? tail : 1.0f - tail;
+    const float density = 0.39894228040143267794f * e;
     *h = gate * cdf * up;
     *by_gate = up * (cdf + gate * density);
     *by_up = gate * cdf;

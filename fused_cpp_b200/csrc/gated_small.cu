@@ -408,7 +408,8 @@ cudaError_t launch_tile(Args args, const Operands& o, cudaStream_t stream, bool 
   args.row_tiles = static_cast<int>((args.rows + kRowTile - 1) / kRowTile);
   const int64_t blocks = static_cast<int64_t>((args.n + kChannels - 1) / kChannels) * args.row_tiles;
   if (blocks > (1ll << 27)) return cudaErrorInvalidValue;
-  // As many parts as leave all clusters resident at once, two CTAs per SM if need be, every part at least two K blocks (dense_gemm.cu).
+  // As many parts as leave all clusters resident at once, two CTAs per SM if need be, every part at least two K blocks (dense_gemm.cu): one row of 7168 x 2048,
+  // 2 / 4 / 6 parts of the gated projection: 24.5 / 22.2 / 20.7 us for the block; 256 rows, 4 / 2 parts of the down projection: 44.9 / 38.2 us.
   args.parts = 1;
   for (int parts = kMaxParts; parts > 1; --parts) {
     if (blocks <= 2 * one_per_sm.clusters[parts] && parts * kMinPartBlocks <= args.k_blocks) {
