@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.util
 import os
 from dataclasses import dataclass
 
@@ -36,6 +37,7 @@ W13_INTERLEAVED = 0x100  # or-ed into the activation: gate and up rows of w13 al
 BIAS_BF16 = 0x200        # or-ed into the activation: w13_bias / w2_bias are bf16
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libfused_moe_b200.so")
+HOST_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "fused_moe_b200_host.so")
 DIAG_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libfused_moe_b200_diag.so")
 
 EXPORTS = (
@@ -110,11 +112,6 @@ class Config(ctypes.Structure):
     ]
 
 
-class LoraAdapters(ctypes.Structure):
-    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scaling", ctypes.c_void_p), ("count", ctypes.c_int32), ("rank", ctypes.c_int32),
-                ("a_stride", ctypes.c_int32), ("b_stride", ctypes.c_int32)]
-
-
 class WorkspaceLayout(ctypes.Structure):
     _fields_ = [(name, ctypes.c_size_t) for name in (
         "total_bytes", "status", "counts", "offsets", "sorted_routes", "row_expert", "items", "scratch", "a_rows",
@@ -148,6 +145,24 @@ def load_diag() -> ctypes.CDLL:
         _DIAG_LIB.fmoe_probe_mma_rate.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                                   ctypes.POINTER(ctypes.c_float)]
     return _DIAG_LIB
+
+
+_HOST = None
+
+
+def host():
+    """The native host side of the short calls (csrc/host), bound to the library; raises, never falls back, if it is absent."""
+    global _HOST
+    if _HOST is None:
+        load()
+        if not os.path.exists(HOST_LIB_PATH):
+            raise FusedMoEError(ERR_CUDA, f"{HOST_LIB_PATH} is missing: build it with `python -m fused_cpp_b200.build`")
+        spec = importlib.util.spec_from_file_location("fused_moe_b200_host", HOST_LIB_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(LIB_PATH)
+        _HOST = module
+    return _HOST
 
 
 def _open(path: str) -> ctypes.CDLL:
@@ -187,13 +202,8 @@ def _open(path: str) -> ctypes.CDLL:
     lib.fmoe_route_build_noalloc.argtypes = [p, i64, i32, i32, p, p, p, p, p, p]
     lib.fmoe_i8gemm_dynamic_scaled_mm.argtypes = [p, i32, i64, i32, p, p, p, i32, p, i32, p, ctypes.c_size_t, p]
     lib.fmoe_i8gemm_dynamic_scaled_mm_pair.argtypes = [p, i64, i32, p, p, i32, p, p, p, i32, p, p, ctypes.c_size_t, p]
-    lib.fmoe_i8gemm_lora_workspace_bytes.restype = ctypes.c_size_t
-    lib.fmoe_i8gemm_lora_workspace_bytes.argtypes = [i64, i32, i32, i32]
-    lib.fmoe_i8gemm_dynamic_scaled_mm_lora.argtypes = [p, i64, i32, p, p, p, i32, ctypes.POINTER(LoraAdapters), p, i32, p, i32, p, ctypes.c_size_t, p]
     lib.fmoe_gated_mlp_derivative_count.argtypes = [i64, i32]
     lib.fmoe_gated_mlp_derivative_count.restype = i64
-    lib.fmoe_gated_mlp_forward.argtypes = [p, i64, p, p, i64, i32, i32, i32, ctypes.c_float, p, p, p, p]
-    lib.fmoe_gated_mlp_backward.argtypes = [p, i64, p, i64, p, p, p, p, i64, i32, i32, p, p, p, p, p]
     lib.fmoe_dense_status.argtypes = [p, ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_int32)]
     lib.fmoe_append_shared_route.argtypes = [p, p, i64, i32, i64, ctypes.c_float, p, p, p]
     lib.fmoe_router_topk.argtypes = [p, p, i64, i32, i32, i32, i32, ctypes.c_float, p, p, p]
@@ -238,11 +248,6 @@ def device_supported(device: int | None = None) -> bool:
 # took a fifth of the host time of a forward.)
 def _ptr(tensor: torch.Tensor | None) -> int | None:
     return None if tensor is None else tensor.data_ptr()
-
-
-def _stream_of(index: int) -> int:
-    """Raw handle of the current stream of device `index`."""
-    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _stream() -> int:
@@ -362,14 +367,6 @@ def _require_cuda(name: str, tensor: torch.Tensor, dtype: torch.dtype) -> torch.
     if tensor.dtype is not dtype:
         raise TypeError(f"{name} must have dtype {dtype}, got {tensor.dtype}")
     return tensor if tensor.is_contiguous() else tensor.contiguous()
-
-
-def on_device(index: int, call, *args):
-    """call(*args) with device `index` as the current one, whose current stream and set-up the library then uses."""
-    if torch._C._cuda_getDevice() == index:
-        return call(*args)
-    with torch.cuda.device(index):
-        return call(*args)
 
 
 def dense_status() -> tuple[int, int]:

@@ -17,7 +17,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib, i8gemm
+from . import _lib, i8gemm, lora
 
 _HAS_DEEPSEEK_V4_W8A8 = _lib.device_supported()
 _QUANTISER_COLUMN_QUANTUM = 16  # the row quantiser reads 16-column vectors
@@ -93,15 +93,22 @@ def prepare_deepseek_v4_w8a8_linear_weight(weight: torch.Tensor, *, backend: str
 
 
 def deepseek_v4_w8a8_linear(input: torch.Tensor, weight: PreparedDeepSeekV4W8A8LinearWeight, *, num_threads: int = 0,
-                            out: torch.Tensor | None = None) -> torch.Tensor:
-    """bf16 [*, K] x prepared [N, K]^T -> bf16 [*, N]; with `out`, the result is written there and `out` returned."""
+                            out: torch.Tensor | None = None, adapters: lora.PreparedAdapters | None = None,
+                            adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 [*, K] x prepared [N, K]^T -> bf16 [*, N]; with `out`, the result is written there and `out` returned.  With `adapters`
+    (lora.prepare_adapters) and `adapter_ids` [*], every row has its own low-rank adapter added (i8gemm.dynamic_scaled_mm_lora)."""
     _check_prepared(weight)
     if not _is_cuda_bf16(input):
         raise TypeError("DeepSeek V4 W8A8 input must be a CUDA torch.bfloat16 tensor")
     if input.shape[-1] != weight.k:
         raise ValueError(f"DeepSeek V4 W8A8 input K must be {weight.k}, got {input.shape[-1]}")
     threads = _check_threads(num_threads)
-    product = i8gemm.dynamic_scaled_mm(input, weight.packed, out_dtype=torch.bfloat16, nthreads=threads)
+    if (adapters is None) != (adapter_ids is None):
+        raise ValueError("adapters and adapter_ids are given together")
+    if adapters is not None:
+        product = i8gemm.dynamic_scaled_mm_lora(input, weight.packed, adapters, adapter_ids, out_dtype=torch.bfloat16, nthreads=threads)
+    else:
+        product = i8gemm.dynamic_scaled_mm(input, weight.packed, out_dtype=torch.bfloat16, nthreads=threads)
     if out is None:
         return product
     acceptable = (out.device == product.device and out.dtype == product.dtype and out.shape == product.shape and out.is_contiguous())
@@ -122,9 +129,10 @@ def deepseek_v4_w8a8_linear_pair(input: torch.Tensor, first: PreparedDeepSeekV4W
 
 
 def deepseek_v4_wo_b_w8a8(input: torch.Tensor, weight: PreparedDeepSeekV4W8A8LinearWeight, *, num_threads: int = 0,
-                          out: torch.Tensor | None = None) -> torch.Tensor:
+                          out: torch.Tensor | None = None, adapters: lora.PreparedAdapters | None = None,
+                          adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
     """The tensor-parallel-local `attn.wo_b` projection; the reduction across ranks stays with the caller."""
-    return deepseek_v4_w8a8_linear(input, weight, num_threads=num_threads, out=out)
+    return deepseek_v4_w8a8_linear(input, weight, num_threads=num_threads, out=out, adapters=adapters, adapter_ids=adapter_ids)
 
 
 __all__ = [

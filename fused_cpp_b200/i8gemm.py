@@ -182,11 +182,8 @@ def dynamic_scaled_mm_lora(x: torch.Tensor, packed: PreparedI8GEMMWeight, adapte
             raise ValueError(f"i8gemm.dynamic_scaled_mm_lora: {what} must lie on the input's device")
     if nthreads < 0:
         raise ValueError("nthreads must be non-negative; zero selects the backend default")
-    out = x.new_empty((*shape, n), dtype=out_dtype)
-    if x.numel() == 0:
-        return out
-    _lib.on_device(index, lora.projection, index, x, packed, adapters, adapter_ids, bias, out)
-    return out
+    return _lib.host().lora_mm(x, packed.packed_weight, packed.weight_scale, adapters.a, adapters.b, adapters.scaling, adapter_ids, bias, n,
+                               out_dtype is torch.float32)
 
 
 __all__ = ["PreparedI8GEMMWeight", "_supports_i8gemm", "dynamic_scaled_mm", "dynamic_scaled_mm_lora", "dynamic_scaled_mm_pair", "mm", "prepare"]

@@ -9,8 +9,7 @@ Row m of a batch gets scaling[a] * B[a] (A[a] x[m]) added to its projection, a =
 """
 from __future__ import annotations
 
-import functools
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 from typing import Sequence
 
 import torch
@@ -33,7 +32,6 @@ class PreparedAdapters:
     rank: int
     k: int
     n: int
-    native: _lib.LoraAdapters = field(repr=False, compare=False, default=None)
 
 
 def _check_pair(a, b, where: str) -> None:
@@ -87,8 +85,7 @@ def prepare_adapters(a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor |
             b_rows[i, :, : first.shape[0]] = second
     factors = factors.to(device).expand(count).contiguous()
     _require_finite(where, a_rows, b_rows, factors)
-    native = _lib.LoraAdapters(a_rows.data_ptr(), b_rows.data_ptr(), factors.data_ptr(), count, rank, a_rows.shape[2], b_rows.shape[2])
-    return PreparedAdapters(a_rows, b_rows, factors, count, rank, k, n, native)
+    return PreparedAdapters(a_rows, b_rows, factors, count, rank, k, n)
 
 
 def set_adapter(adapters: PreparedAdapters, index: int, a: torch.Tensor, b: torch.Tensor, scaling: float = 1.0) -> None:
@@ -109,30 +106,6 @@ def set_adapter(adapters: PreparedAdapters, index: int, a: torch.Tensor, b: torc
         adapters.b[index, :, :rank] = b
         adapters.b[index, :, rank:] = 0
         adapters.scaling[index] = float(scaling)
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(rows: int, k: int, rank: int, out_is_bf16: int) -> int:
-    return _lib.load().fmoe_i8gemm_lora_workspace_bytes(rows, k, rank, out_is_bf16)
-
-
-def projection(index: int, x: torch.Tensor, packed, adapters: PreparedAdapters, adapter_ids: torch.Tensor, bias: torch.Tensor | None,
-               out: torch.Tensor) -> None:
-    """out [..., N] of bf16 rows x [..., K] on CUDA device `index`, checked by the caller; the workspace is the call's own, so that calls on
-    several streams and captured ones do not share it."""
-    x = x if x.is_contiguous() else x.contiguous()
-    adapter_ids = adapter_ids if adapter_ids.is_contiguous() else adapter_ids.contiguous()
-    if bias is not None:
-        bias = _lib.as_dtype(bias.to(x.device), torch.float32)
-    rows, k = x.numel() // packed.k, packed.k
-    lib = _lib.load()
-    out_is_bf16 = 1 if out.dtype is torch.bfloat16 else 0
-    nbytes = _workspace_bytes(rows, k, adapters.rank, out_is_bf16)
-    workspace = x.new_empty(nbytes, dtype=torch.uint8)
-    _lib.check(lib.fmoe_i8gemm_dynamic_scaled_mm_lora(
-        x.data_ptr(), rows, k, packed.packed_weight.data_ptr(), packed.weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), packed.n,
-        adapters.native, adapter_ids.data_ptr(), 1 if adapter_ids.dtype is torch.int64 else 0, out.data_ptr(), out_is_bf16, workspace.data_ptr(), nbytes,
-        _lib._stream_of(index)))
 
 
 __all__ = ["MAX_RANK", "PreparedAdapters", "prepare_adapters", "set_adapter"]

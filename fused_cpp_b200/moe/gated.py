@@ -64,33 +64,6 @@ def _require_cuda(index: int) -> None:
         raise ValueError("gated_mlp takes CUDA tensors (this build has no CPU path)")
 
 
-def _rows(tensor: torch.Tensor, columns: int) -> torch.Tensor:
-    """[..., columns] as rows that the kernels can read where they are: unit column stride, every row on a 16-byte boundary."""
-    if tensor.dim() == 2 and tensor.is_contiguous() and tensor.data_ptr() % 16 == 0:
-        return tensor
-    rows = tensor.reshape(-1, columns)
-    if rows.stride(1) == 1 and rows.data_ptr() % 16 == 0 and (rows.shape[0] == 1 or (rows.stride(0) % 8 == 0 and rows.stride(0) >= columns)):
-        return rows
-    rows = rows.contiguous()
-    return rows if rows.data_ptr() % 16 == 0 else rows.clone()
-
-
-def _like(input: torch.Tensor) -> torch.Tensor:
-    """A contiguous result of the input's shape."""
-    return torch.empty_like(input) if input.is_contiguous() else input.new_empty(input.shape)
-
-
-def _stride(rows: torch.Tensor) -> int:
-    """Elements from a row to the next; a single row may carry any stride."""
-    return rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
-
-
-def _whole(tensor: torch.Tensor) -> torch.Tensor:
-    """A weight as contiguous rows on a 16-byte boundary."""
-    tensor = tensor if tensor.is_contiguous() else tensor.contiguous()
-    return tensor if tensor.data_ptr() % 16 == 0 else tensor.clone()
-
-
 def _derivative_bytes(rows: int, inter: int) -> int:
     """4 * fmoe_gated_mlp_derivative_count: whole blocks of 32 rows x 32 channels x 2."""
     return -(-rows // 32) * -(-inter // 32) * 8192
@@ -99,63 +72,6 @@ def _derivative_bytes(rows: int, inter: int) -> int:
 def _kept_bytes(rows: int, inter: int) -> int:
     """The derivatives, then h."""
     return _derivative_bytes(rows, inter) + 2 * rows * inter
-
-
-def _forward(index: int, rows, w13, w2, code: int, limit: float, keep: bool, y):
-    """y, and what the backward pass needs (keep) or h alone, in one buffer (the caller's, so that it outlives the kernels on this stream)."""
-    count, hidden = rows.shape
-    inter = w2.shape[1]
-    front = _derivative_bytes(count, inter) if keep else 0
-    kept = rows.new_empty(front + 2 * count * inter, dtype=torch.uint8)
-    address = kept.data_ptr()
-    _lib.check(_lib.load().fmoe_gated_mlp_forward(rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(), count, hidden, inter, code, limit,
-                                                  address + front, address if keep else None, y.data_ptr(), _lib._stream_of(index)))
-    return kept
-
-
-def _backward(index: int, dy, rows, w13, w2, kept, need_x: bool, need_w13: bool, need_w2: bool):
-    count, hidden = rows.shape
-    inter = w2.shape[1]
-    if count == 0:
-        return (rows.new_zeros((0, hidden)) if need_x else None, w13.new_zeros(w13.shape) if need_w13 else None,
-                w2.new_zeros(w2.shape) if need_w2 else None)
-    dx = _like(rows) if need_x else None
-    dw13 = torch.empty_like(w13) if need_w13 else None
-    dw2 = torch.empty_like(w2) if need_w2 else None
-    scratch = rows.new_empty((count, 2 * inter)) if need_x or need_w13 else None
-    pointer = _lib._ptr
-    address = kept.data_ptr()
-    _lib.check(_lib.load().fmoe_gated_mlp_backward(dy.data_ptr(), _stride(dy), rows.data_ptr(), _stride(rows), w13.data_ptr(), w2.data_ptr(),
-                                                   address + _derivative_bytes(count, inter), address, count, hidden, inter, pointer(scratch),
-                                                   pointer(dx), pointer(dw13), pointer(dw2), _lib._stream_of(index)))
-    return dx, dw13, dw2
-
-
-class _GatedMLP(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, input, w13, w2, code, limit, index):
-        return _lib.on_device(index, _GatedMLP._forward, ctx, input, w13, w2, code, limit, index)
-
-    @staticmethod
-    def _forward(ctx, input, w13, w2, code, limit, index):
-        rows = _rows(input, w2.shape[0])
-        y = _like(input)
-        ctx.save_for_backward(input, w13, w2, _forward(index, rows, _whole(w13), _whole(w2), code, limit, True, y))
-        ctx.index = index
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        if torch.is_grad_enabled():
-            raise RuntimeError("gated_mlp is differentiable once: its backward pass has no gradient (create_graph)")
-        return _lib.on_device(ctx.index, _GatedMLP._backward, ctx, dy)
-
-    @staticmethod
-    def _backward(ctx, dy):
-        input, w13, w2, kept = ctx.saved_tensors
-        hidden = w2.shape[0]
-        dx, dw13, dw2 = _backward(ctx.index, _rows(dy, hidden), _rows(input, hidden), _whole(w13), _whole(w2), kept, *ctx.needs_input_grad[:3])
-        return dx if dx is None or input.dim() == 2 else dx.view(input.shape), dw13, dw2, None, None, None
 
 
 def gated_mlp(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float | None = None, out=None):
@@ -169,38 +85,23 @@ def gated_mlp(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float |
     _, _, index = _check(input, w13, w2)
     code, limit = _activation(activation, swiglu_limit)
     _require_cuda(index)
-    if (input.requires_grad or w13.requires_grad or w2.requires_grad) and torch.is_grad_enabled():
-        if out is not None:
+    if out is not None:
+        if (input.requires_grad or w13.requires_grad or w2.requires_grad) and torch.is_grad_enabled():
             raise ValueError("out cannot be given where gradients are asked for")
-        return _GatedMLP.apply(input, w13, w2, code, limit, index)
-    return _lib.on_device(index, _serve, index, input, w13, w2, code, limit, out)
-
-
-def _serve(index: int, input, w13, w2, code: int, limit: float, out):
-    rows = _rows(input, w2.shape[0])
-    if out is None:
-        y = out = _like(input)
-    else:
         _check_tensor("out", out, index)
         if out.shape != input.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous and match the input shape")
-        y = out if out.data_ptr() % 16 == 0 else rows.new_empty(input.shape)
-    _forward(index, rows, _whole(w13), _whole(w2), code, limit, False, y)
-    return out if y is out else out.copy_(y)
+        _lib.host().gated_mlp(input, w13, w2, code, limit, out)
+        return out
+    return _lib.host().gated_mlp(input, w13, w2, code, limit, None)
 
 
 def gated_mlp_forward(input, w13, w2, *, activation: Any = "silu", swiglu_limit: float | None = None):
     """The forward pass without a tape: (y, kept), the second for `gated_mlp_backward`."""
-    hidden, _, index = _check(input, w13, w2)
+    _, _, index = _check(input, w13, w2)
     code, limit = _activation(activation, swiglu_limit)
     _require_cuda(index)
-
-    def call():
-        rows = _rows(input.detach(), hidden)
-        y = _like(rows).view(input.shape)
-        return y, _forward(index, rows, _whole(w13.detach()), _whole(w2.detach()), code, limit, True, y)
-
-    return _lib.on_device(index, call)
+    return _lib.host().gated_forward(input, w13, w2, code, limit)
 
 
 def gated_mlp_backward(dy, input, w13, w2, kept, *, needs: tuple = (True, True, True)):
@@ -216,9 +117,4 @@ def gated_mlp_backward(dy, input, w13, w2, kept, *, needs: tuple = (True, True, 
         raise ValueError("needs must say for dx, dw13 and dw2 whether they are wanted")
     _require_cuda(index)
 
-    def call():
-        dx, dw13, dw2 = _backward(index, _rows(dy.detach(), hidden), _rows(input.detach(), hidden), _whole(w13.detach()), _whole(w2.detach()), kept,
-                                  *(bool(need) for need in needs))
-        return None if dx is None else dx.view(input.shape), dw13, dw2
-
-    return _lib.on_device(index, call)
+    return _lib.host().gated_backward(dy, input, w13, w2, kept, *(bool(need) for need in needs))

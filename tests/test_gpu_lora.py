@@ -225,15 +225,21 @@ def test_streams_and_graphs(cuda_device):
 def test_attention_output_then_feed_forward(cuda_device):
     """The two operators one after the other, as a layer has them: the attention's output projection with the requests' adapters, then the gated block, and the
     block's weights learning from what comes out."""
-    from fused_cpp_b200 import i8gemm, lora, moe
+    from fused_cpp_b200 import deepseek_v4_w8a8, i8gemm, lora, moe
 
     x, w, s, a, b, scaling, ids, _ = make(50, 512, 256, 4, 16)
     packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
     g = torch.Generator(device="cuda").manual_seed(5)
     w13 = (torch.randn(256, 256, generator=g, device="cuda") / 16).bfloat16().requires_grad_(True)
     w2 = (torch.randn(256, 128, generator=g, device="cuda") / 12).bfloat16().requires_grad_(True)
-    projected = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids)
+    weight = deepseek_v4_w8a8.prepare_deepseek_v4_w8a8_linear_quantized_weight(w, s)
+    projected = deepseek_v4_w8a8.deepseek_v4_wo_b_w8a8(x, weight, adapters=adapters, adapter_ids=ids)
     check(projected, base_product(x, w, s, None), x, a, b, scaling, ids)
+    assert torch.equal(projected, i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids))
+    out = torch.empty_like(projected)
+    assert deepseek_v4_w8a8.deepseek_v4_w8a8_linear(x, weight, out=out, adapters=adapters, adapter_ids=ids) is out and torch.equal(out, projected)
+    with pytest.raises(ValueError, match="given together"):
+        deepseek_v4_w8a8.deepseek_v4_w8a8_linear(x, weight, adapters=adapters)
     y = moe.gated_mlp(projected, w13, w2, swiglu_limit=10.0)
     with torch.no_grad():
         assert torch.equal(y, moe.gated_mlp(projected, w13, w2, swiglu_limit=10.0))
