@@ -38,7 +38,6 @@ constexpr int kTmemColumns = 512;
 constexpr int kStagingBytes = 32 * 128;
 constexpr int kMaxStages = 8;
 constexpr int kTileGroup = 8;  // row tiles that are walked together (gated_gemm.cu)
-constexpr int kWriteAhead = 4; // K blocks of coefficients that a warp writes before it publishes them
 constexpr int kDelay = 4;      // K blocks of the next tile in front of a tile's adapters: what the epilogue takes for step 1
 
 template <int kTileN>
@@ -74,6 +73,7 @@ struct Args {
   int k_blocks, m_tiles, n_tiles, rank_blocks;
   LoraBlock block;
   int tma_store;
+  int pair_store;  // otherwise: whether two bf16 channels are a 4-byte store
 };
 
 struct Tile {
@@ -116,12 +116,7 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t address, const uint32_t* v)
       : "memory");
 }
 
-// Arrival on an mbarrier of either CTA that publishes what this warp wrote (shared memory of its CTA, tensor memory), and the bounded wait that
-// takes it over: writer and reader are in different CTAs.
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_address) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_address) : "memory");
-}
-
+// The bounded wait for arrivals of either CTA.
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -426,8 +421,6 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
       const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
       const uint32_t use = static_cast<uint32_t>(local) >> 1;
       const int warp_row = tile.m * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + quarter * 32;
-      const int64_t row = static_cast<int64_t>(warp_row) + lane;
-      const bool row_ok = row < args.g.rows;
       const int n0 = tile.n * kTileN;
       const uint32_t acc = acc_lane_base + kTileN * buffer;
       // This tile's channel values; the buffer was last read two tiles ago, in front of the barrier of the tile in between.
@@ -470,7 +463,7 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         ptx::tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_release_cluster(converted_leader + 8u * buffer);
+        if (lane == 0) mbar_arrive_cluster(converted_leader + 8u * buffer);
         ptx::mbar_wait(&ctl->all_full[buffer], (all_phase >> buffer) & 1u, abort_flag, status, 79);
         all_phase ^= 1u << buffer;
         ptx::tcgen05_fence_after();
@@ -495,42 +488,51 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
               for (int j = 0; j < 32; ++j) bits[j] = __float_as_uint(__fadd_rn(__uint_as_float(bits[j]), __uint_as_float(delta[j])));
             }
           }
-          const int first = col + 32 * half;
-          if (args.tma_store) {
-            if (!args.g.out_bf16 || half == 0) {
-              if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the block before has been read out of shared memory
-              __syncwarp();
+          // 64 bf16 or 32 fp32 channels of 32 rows in shared memory, a row a lane, 128-byte rows in the 128-byte swizzle.
+          const bool bf16 = args.g.out_bf16 != 0;
+          const bool opens = !bf16 || half == 0, closes = !bf16 || half == 1;
+          const int block_col = bf16 ? col : col + 32 * half;
+          if (opens) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the block before has been read out of shared memory
+            __syncwarp();
+          }
+          auto put = [&](int piece, uint4 value) { *reinterpret_cast<uint4*>(staging + lane * 128 + ((piece ^ (lane & 7)) << 4)) = value; };
+          if (bf16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t words[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) words[j] = pack_bf16(__uint_as_float(bits[8 * q + 2 * j]), __uint_as_float(bits[8 * q + 2 * j + 1]));
+              put(4 * half + q, make_uint4(words[0], words[1], words[2], words[3]));
             }
-            auto put = [&](int piece, uint4 value) { *reinterpret_cast<uint4*>(staging + lane * 128 + ((piece ^ (lane & 7)) << 4)) = value; };
-            if (args.g.out_bf16) {
+          } else {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                uint32_t words[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) words[j] = pack_bf16(__uint_as_float(bits[8 * q + 2 * j]), __uint_as_float(bits[8 * q + 2 * j + 1]));
-                put(4 * half + q, make_uint4(words[0], words[1], words[2], words[3]));
-              }
-            } else {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) put(q, make_uint4(bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]));
+            for (int q = 0; q < 8; ++q) put(q, make_uint4(bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]));
+          }
+          if (closes && args.tma_store) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && block_col < n) {
+              tma_store_2d(&out_map, ptx::smem_u32(staging), block_col, warp_row);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
-            if (!args.g.out_bf16 || half == 1) {
-              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-              __syncwarp();
-              if (lane == 0 && (args.g.out_bf16 || first < n)) {
-                tma_store_2d(&out_map, ptx::smem_u32(staging), args.g.out_bf16 ? col : first, warp_row);
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-              }
-            }
-          } else if (row_ok) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (first + j >= n) break;
-              const float value = __uint_as_float(bits[j]);
-              if (args.g.out_bf16) {
-                static_cast<uint16_t*>(args.g.out)[row * n + first + j] = __bfloat16_as_ushort(__float2bfloat16_rn(value));
+          } else if (closes) {
+            // Rows of the result that start on no 16-byte boundary, which TMA needs: a row at a time, neighbouring lanes neighbouring channels.
+            // (A row a lane, channel by channel: 6846 rows of 143 -> 3253 265 us, XX us like this.)
+            __syncwarp();
+            const int rows_here = static_cast<int>(min(static_cast<int64_t>(32), args.g.rows - warp_row));
+            for (int r = 0; r < rows_here; ++r) {
+              // Word `lane` of row r: two bf16 channels or one fp32 channel.
+              const uint32_t word = *reinterpret_cast<const uint32_t*>(staging + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+              const int64_t index = static_cast<int64_t>(warp_row + r) * n + block_col;
+              if (!bf16) {
+                if (block_col + lane < n) static_cast<float*>(args.g.out)[index + lane] = __uint_as_float(word);
+              } else if (args.pair_store) {
+                if (block_col + 2 * lane < n) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(args.g.out) + index + 2 * lane) = word;
               } else {
-                static_cast<float*>(args.g.out)[row * n + first + j] = value;
+                uint16_t* const to = static_cast<uint16_t*>(args.g.out) + index + 2 * lane;
+                if (block_col + 2 * lane < n) to[0] = static_cast<uint16_t>(word & 0xffffu);
+                if (block_col + 2 * lane + 1 < n) to[1] = static_cast<uint16_t>(word >> 16);
               }
             }
           }
@@ -566,24 +568,20 @@ lora_pair_gemm_kernel(const __grid_constant__ CUtensorMap token_map, const __gri
           value[p] = make_uint4(0, 0, 0, 0);
           if (my_slot >= 0 && p % share < pieces) value[p] = __ldcg(reinterpret_cast<const uint4*>(from) + p % share);
         }
-        // Up to kWriteAhead blocks behind one fence, whose latency and that of the arrival are most of a block's time.  (The stages of all of them fall
-        // vacant without this warp's arrival for any: what they held stands in front of these blocks in every role's order.)
-        for (int slot = 0; slot < slots;) {
-          int blocks = 0;
-          const int first_stage = stage;
-          for (; blocks < kWriteAhead && slot < slots; ++blocks, slot += per_block) {
-            ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 80);
-            used ^= 1u << stage;
-            uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + row_in_cta * 128;
+        for (int slot = 0; slot < slots; slot += per_block) {
+          ptx::mbar_wait(&ctl->vacant[stage], (used >> stage) & 1u, abort_flag, status, 80);
+          used ^= 1u << stage;
+          uint8_t* const to = smem + static_cast<size_t>(stage) * Cfg::kStageBytes + row_in_cta * 128;
 #pragma unroll
-            for (int p = 0; p < 8; ++p) {
-              *reinterpret_cast<uint4*>(to + ((p ^ (row_in_cta & 7)) << 4)) = slot + p / share == my_slot ? value[p] : make_uint4(0, 0, 0, 0);
-            }
-            skip(1);
+          for (int p = 0; p < 8; ++p) {
+            *reinterpret_cast<uint4*>(to + ((p ^ (row_in_cta & 7)) << 4)) = slot + p / share == my_slot ? value[p] : make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane < blocks) mbar_arrive_release_cluster(coefficients_leader + 8u * static_cast<uint32_t>((first_stage + lane) % kStages));
+          // (A cluster-wide release would wait for more than these stores, about half a microsecond a block: 6680 rows of 1733 -> 8181 in fp32 437 us, 379 like this.
+          // What the tensor core reads of the follower's shared memory is what the fence has published.)
+          if (lane == 0) mbar_arrive_cluster(coefficients_leader + 8u * static_cast<uint32_t>(stage));
+          skip(1);
         }
       }
     };
@@ -643,6 +641,7 @@ cudaError_t launch(Args args, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   }
   args.tma_store = static_cast<int64_t>(g.n) * (g.out_bf16 ? 2 : 4) % 16 == 0 && reinterpret_cast<uintptr_t>(g.out) % 16 == 0;
+  args.pair_store = g.n % 2 == 0 && reinterpret_cast<uintptr_t>(g.out) % 4 == 0;
   if (!args.tma_store) {
     maps[3] = maps[0];
   } else if (!make_store_map(&maps[3], g.out, !g.out_bf16, static_cast<uint64_t>(g.n), 1, static_cast<uint64_t>(g.rows))) {
