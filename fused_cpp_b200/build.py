@@ -24,7 +24,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libfused_moe_b200.so")
 DIAG_LIB = os.path.join(OUT_DIR, "libfused_moe_b200_diag.so")
-SOURCES = ["api.cu", "route.cu", "front.cu", "quant.cu", "merge.cu", "umma_gemm.cu", "umma2_gemm.cu", "dense_gemm.cu", "ep.cu", "router.cu", "gated_gemm.cu", "gated_small.cu", "lora_front.cu", "lora_gemm.cu", "lora_pair_gemm.cu"]
+SOURCES = ["api.cu", "route.cu", "front.cu", "quant.cu", "merge.cu", "umma_gemm.cu", "umma2_gemm.cu", "dense_gemm.cu", "ep.cu", "router.cu", "gated_gemm.cu", "gated_small.cu", "lora_front.cu", "lora_units.cu", "lora_gemm.cu", "lora_pair_gemm.cu"]
 HOST_LIB = os.path.join(OUT_DIR, "fused_moe_b200_host.so")
 HOST_SOURCE = os.path.join(CSRC, "host", "host.cpp")
 DIAG_ONLY_SOURCES = ["simt_gemm.cu", "probe.cu"]

@@ -986,6 +986,9 @@ size_t lora_slot_offset(int64_t rows) {
   return align_up(static_cast<size_t>((rows + fmoe::kLoraListRows - 1) / fmoe::kLoraListRows) * fmoe::kLoraListInts * sizeof(int), 256);
 }
 size_t lora_list_bytes(int64_t rows) { return lora_slot_offset(rows) + align_up(static_cast<size_t>(rows) * sizeof(int), 256); }
+size_t lora_copy_bytes(int64_t rows, int k) {
+  return fmoe::lora_wants_copy(rows, k) ? align_up(static_cast<size_t>(rows) * ((static_cast<size_t>(k) + 7) / 8 * 8) * 2, 256) : 0;
+}
 
 // Which kernel: the two-SM one where its tiles of 256 x 256 fill two thirds of the chip, the split one (lora_gemm.cu) before.  Split / two-SM, whole op: 201 rows
 // of 1536 -> 24576 (96 tiles) 38 / 33 us; 384 rows 7168 -> 7168 (56) 47 / 43; 512 rows 16384 -> 7168 (56) 92 / 84; 256 rows of it (28) 64 / 62 to 77; 777 rows 2056 -> 1240
@@ -996,7 +999,8 @@ bool lora_pair_pays(int64_t rows, int n) { return rows > 128 && 3 * ((rows + 255
 size_t fmoe_i8gemm_lora_workspace_bytes(int64_t rows, int32_t k, int32_t rank, int32_t out_is_bf16) {
   if (rows < 0 || k <= 0 || rank <= 0 || rank > fmoe::kLoraMaxRank) return 0;
   const size_t planes = out_is_bf16 ? 1 : fmoe::kLoraPlanes;
-  return align_up(dense_layout(rows, k).total, 256) + lora_list_bytes(rows) + planes * static_cast<size_t>(rows) * fmoe::lora_rank_padded(rank) * 2;
+  return align_up(dense_layout(rows, k).total, 256) + lora_list_bytes(rows) + lora_copy_bytes(rows, k) +
+         planes * static_cast<size_t>(rows) * fmoe::lora_rank_padded(rank) * 2;
 }
 
 int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t k, const int8_t* w, const float* w_scale, const float* bias,
@@ -1031,7 +1035,12 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
                    adapter_ids, ids_are_64, adapters->count, adapters->rank};
   int* const lists = reinterpret_cast<int*>(base + align_up(layout.total, 256));
   int* const row_slots = reinterpret_cast<int*>(reinterpret_cast<char*>(lists) + lora_slot_offset(rows));
-  uint16_t* const t = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(lists) + lora_list_bytes(rows));
+  char* const copy = reinterpret_cast<char*>(lists) + lora_list_bytes(rows);
+  uint16_t* const t = reinterpret_cast<uint16_t*>(copy + lora_copy_bytes(rows, k));
+  const bool wants_copy = fmoe::lora_wants_copy(rows, k);
+  if (rows > fmoe::kLoraFewRows && !wants_copy && reinterpret_cast<uintptr_t>(x_bf16) % 16 != 0) {
+    return fail(FMOE_ERR_INVALID_ARGUMENT, "i8gemm lora: more than %d rows of a multiple of 8 values must start on a 16-byte boundary", fmoe::kLoraFewRows);
+  }
   const bool many = lora_pair_pays(rows, n);
   args.planes = out_is_bf16 ? 1 : fmoe::kLoraPlanes;
   args.xq = reinterpret_cast<const int8_t*>(base + layout.xq);
@@ -1047,7 +1056,8 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
   args.t = t;
   args.status = reinterpret_cast<int*>(base + layout.status);
   cudaError_t error = fmoe::launch_lora_front(args, static_cast<const uint16_t*>(x_bf16), k, reinterpret_cast<int8_t*>(base + layout.xq),
-                                              reinterpret_cast<float*>(base + layout.scale), t, many ? lists : nullptr, row_slots, stream);
+                                              reinterpret_cast<float*>(base + layout.scale), t, many ? lists : nullptr, row_slots,
+                                              wants_copy ? reinterpret_cast<uint16_t*>(copy) : nullptr, stream);
   if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora rows and coefficients");
   args.lists = lists;
   args.row_slots = row_slots;

@@ -188,7 +188,7 @@ at::Tensor lora_mm(const at::Tensor& x, const at::Tensor& weight, const at::Tens
   shape.back() = n;
   const at::Tensor out = at::empty(shape, x.options().dtype(out_is_f32 ? at::kFloat : at::kBFloat16));
   if (x.numel() == 0) return out;
-  const at::Tensor rows = x.contiguous(), row_ids = ids.contiguous();
+  const at::Tensor rows = whole(x), row_ids = ids.contiguous();
   at::Tensor bias_f32;
   if (bias.has_value()) bias_f32 = bias->to(x.options().dtype(at::kFloat)).contiguous();
   const int64_t count = rows.numel() / k;

@@ -74,8 +74,14 @@ struct LoraGemmArgs {
 // Rows of x [rows, k] as int8 q [rows, k_padded] with a scale each, zeros behind k; t[plane][row][rank] = scaling[id] * (A[id] x[row]) for the rows that
 // have an adapter (the others' are left as they are), as `planes` bf16 terms; with lists, the adapters in use by every kLoraListRows rows and
 // each row's place among them.  Clears the status block.  What it writes is what the GEMM of the same arguments reads.
+// x_copy (nullable): room for rows of k padded to 8 values, wanted where lora_wants_copy.
 cudaError_t launch_lora_front(const LoraGemmArgs& args, const uint16_t* x, int k, int8_t* q, float* scale, uint16_t* t, int* lists, int* row_slots,
-                              cudaStream_t stream);
+                              uint16_t* x_copy, cudaStream_t stream);
+constexpr int kLoraFewRows = 256;  // up to so many rows one launch makes rows and coefficients
+inline bool lora_wants_copy(int64_t rows, int k) { return rows > kLoraFewRows && k % 8 != 0; }
+// The coefficients of many rows x, which lie on 16-byte boundaries, k padded to 8 values from a row to the next (lora_units.cu).  A programmatic dependent of the kernel in
+// front, which writes x if `behind`.
+cudaError_t launch_lora_units(const LoraGemmArgs& args, const uint16_t* x, int k, bool behind, uint16_t* t, cudaStream_t stream);
 cudaError_t launch_lora_gemm(const LoraGemmArgs& args, cudaStream_t stream);
 // The same over many rows, by lists.
 cudaError_t launch_lora_pair_gemm(const LoraGemmArgs& args, cudaStream_t stream);

@@ -26,11 +26,9 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTileRows = 128;            // rows of a list of units, where there are many
 constexpr int kUnitRows = 32;
 constexpr int kMaxCluster = 8;
 constexpr int kHeld = 8;                  // 16-byte vectors of a row that a thread holds
-constexpr int kFewRows = 256;
 
 struct FrontArgs {
   const uint16_t* x;
@@ -42,7 +40,8 @@ struct FrontArgs {
   uint16_t* t;
   int planes;
   int* lists;      // nullable
-  int* row_slots;  // [rows], with lists
+  int* row_slots;    // [rows], with lists
+  uint16_t* x_copy;  // many rows on no 16-byte boundaries: where they are written on such, for lora_units.cu
   int* status;
   int cluster;       // CTAs that share a unit's K range
   int unit_groups;   // clusters that share a tile's units
@@ -55,15 +54,6 @@ struct UnitSums {
   static constexpr int kValues = 16 * kRankTiles * kUnitRows;
   alignas(16) float total[kValues];
   alignas(16) float part[kWarps][kValues];  // stored in pairs
-};
-
-struct UnitList {
-  alignas(16) int id[kTileRows];
-  int slot_adapter[kTileRows], slot_rows[kTileRows], slot_first[kTileRows];
-  int unit_slot[kTileRows], unit_row[kTileRows];  // unit -> slot, first row of it in `order`
-  int order[kTileRows];                           // rows of the tile, slot by slot
-  int warp_count[4];
-  int units;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -106,74 +96,6 @@ __device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int columns
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
   }
-}
-
-// The tile's units, in an order that the ids alone decide.
-__device__ __forceinline__ void list_units(UnitList& s, const FrontArgs& args, int64_t row0) {
-  const int i = threadIdx.x;
-  const int lane = i & 31;
-  const int tile_rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), args.rows - row0));
-  int before = 0, total = 0, first = kTileRows;
-  if (i < kTileRows) s.id[i] = i < tile_rows ? load_adapter_id(args.adapters, row0 + i) : -1;
-  __syncthreads();
-  const int mine = i < kTileRows ? s.id[i] : -1;
-  if (mine >= 0) {
-    for (int j = 0; j < tile_rows; j += 4) {
-      const int4 others = *reinterpret_cast<const int4*>(&s.id[j]);
-      const int four[4] = {others.x, others.y, others.z, others.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool same = four[k] == mine;
-        if (same && first == kTileRows) first = j + k;
-        before += same && j + k < i;
-        total += same;
-      }
-    }
-  }
-  const bool owner = mine >= 0 && first == i;
-  const unsigned owners = __ballot_sync(0xffffffffu, owner);
-  if (i < kTileRows && lane == 0) s.warp_count[i >> 5] = __popc(owners);
-  __syncthreads();
-  int slot = __popc(owners & ((1u << lane) - 1));
-  int slots = 0;
-  for (int w = 0; w < 4; ++w) {
-    if (w < (i >> 5)) slot += s.warp_count[w];
-    slots += s.warp_count[w];
-  }
-  if (owner) {
-    s.slot_adapter[slot] = mine;
-    s.slot_rows[slot] = total;
-    s.unit_row[i] = slot;  // for a moment: the slot of the adapter's first row
-  }
-  __syncthreads();
-  const int my_slot = mine >= 0 ? s.unit_row[first] : 0;
-  // Rows (low half) and units (high half) of the slots in front of slot i.
-  const int rows = i < slots ? s.slot_rows[i] : 0;
-  const int packed = rows | ((rows + kUnitRows - 1) / kUnitRows) << 16;
-  int scan = packed;
-#pragma unroll
-  for (int offset = 1; offset < 32; offset <<= 1) {
-    const int other = __shfl_up_sync(0xffffffffu, scan, offset);
-    if (lane >= offset) scan += other;
-  }
-  __syncthreads();  // unit_row and warp_count are read
-  if (i < kTileRows && lane == 31) s.warp_count[i >> 5] = scan;
-  __syncthreads();
-  int front = scan - packed;
-  for (int w = 0; w < 4 && w < (i >> 5); ++w) front += s.warp_count[w];
-  if (i < slots) {
-    const int row_first = front & 0xffff, unit_first = front >> 16;
-    s.slot_first[i] = row_first;
-    for (int u = 0; u < packed >> 16; ++u) {
-      s.unit_slot[unit_first + u] = i;
-      s.unit_row[unit_first + u] = row_first + u * kUnitRows;
-    }
-    if (i == slots - 1) s.units = unit_first + (packed >> 16);
-  }
-  if (slots == 0 && i == 0) s.units = 0;
-  __syncthreads();
-  if (mine >= 0) s.order[s.slot_first[my_slot] + before] = i;
-  __syncthreads();
 }
 
 // The warps' partial sums of a unit: the rows order[0 .. count) of x from `x` on, times the first `ranks` rows of `a`.
@@ -284,8 +206,10 @@ __device__ __forceinline__ void quantise_row_twice(const FrontArgs& args, int64_
   const float inverse = __fdiv_rn(1.0f, scale);
   uint2* const dst = reinterpret_cast<uint2*>(args.q + row * args.k_padded);
   for (int v = threadIdx.x; v < vectors; v += kThreads) {
+    const uint4 eight = load_x8<kVector>(src, 8 * v, args.k);
+    if (!kVector && 8 * v < args.k) reinterpret_cast<uint4*>(args.x_copy + row * ((args.k + 7) / 8 * 8))[v] = eight;
     float values[8];
-    unpack8(load_x8<kVector>(src, 8 * v, args.k), values);
+    unpack8(eight, values);
     dst[v] = make_uint2(quantize4_torchref_fast<false>(values, scale, inverse, -128.0f), quantize4_torchref_fast<false>(values + 4, scale, inverse, -128.0f));
   }
 }
@@ -464,113 +388,57 @@ lora_rows_kernel(const __grid_constant__ FrontArgs args) {
   quantise_row_twice<kVector>(args, blockIdx.x, block_max_values);
 }
 
-// Many rows: the units of 128 rows, shared by unit_groups clusters.  A programmatic dependent of lora_rows_kernel that does not need it: everything is read
-// through L2, and the wait stands at the end.
 template <bool kVector, int kRankTiles>
-__global__ void __launch_bounds__(kThreads, 2)
-lora_units_kernel(const __grid_constant__ FrontArgs args) {
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  UnitSums<kRankTiles>& sums = *reinterpret_cast<UnitSums<kRankTiles>*>(smem_raw);
-  __shared__ UnitList s;
-  ptx::launch_dependents();
-  const int cluster_rank = static_cast<int>(blockIdx.x) % args.cluster;
-  const int group = static_cast<int>(blockIdx.x) / args.cluster;
-  const int tile = group / args.unit_groups;
-  const int64_t row0 = static_cast<int64_t>(tile) * kTileRows;
-  list_units(s, args, row0);
-  int chunk_begin, chunk_end;
-  chunk_range(args, cluster_rank, &chunk_begin, &chunk_end);
-  const int rank_blocks = (args.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
-  const int work = s.units * rank_blocks;
-  for (int item = group - tile * args.unit_groups; item < work; item += args.unit_groups) {
-    const int index = item / rank_blocks;
-    const int rank0 = (item - index * rank_blocks) * kLoraRankBlock;
-    const int slot = s.unit_slot[index];
-    const int adapter = s.slot_adapter[slot];
-    const int order0 = s.unit_row[index];
-    const int count = min(kUnitRows, s.slot_first[slot] + s.slot_rows[slot] - order0);
-    const int ranks = min(kLoraRankBlock, args.adapters.rank - rank0);
-    const uint16_t* const a = args.adapters.a + (static_cast<int64_t>(adapter) * args.adapters.rank + rank0) * args.adapters.a_stride;
-    multiply_unit<kVector, kRankTiles, 4, kRankTiles == 1 ? 2 : 1>(args, args.x + row0 * args.k, s.order + order0, count, a, ranks, chunk_begin, chunk_end,
-                                                                   sums.part[threadIdx.x >> 5]);
-    finish_unit<kRankTiles, 4>(args, sums, cluster_rank, adapter, row0, s.order + order0, count, rank0, ranks);
-  }
-  ptx::grid_dependency_wait();  // this kernel's end stands for the end of the one in front too
-}
-
-template <typename Kernel>
-cudaError_t launch_clusters(Kernel kernel, const FrontArgs& args, int64_t blocks, size_t smem_bytes, bool chained, PerDeviceOnce* configured, cudaStream_t stream) {
+cudaError_t launch_few(FrontArgs args, cudaStream_t stream) {
+  auto kernel = lora_front_kernel<kVector, kRankTiles>;
+  static PerDeviceOnce configured;
   const int device = current_device_ordinal();
-  if (configured->needed(device)) {
-    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes));
+  if (configured.needed(device)) {
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(UnitSums<kRankTiles>)));
     if (error != cudaSuccess) return error;
-    configured->mark(device);
+    configured.mark(device);
   }
-  if (blocks > (1ll << 31) - 1) return cudaErrorInvalidValue;
+  const int rank_blocks = (args.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  const int tiles = static_cast<int>((args.rows + kUnitRows - 1) / kUnitRows);
+  const int rows_in_tile = static_cast<int>(args.rows < kUnitRows ? args.rows : kUnitRows);
+  const int most = (args.adapters.count < rows_in_tile ? args.adapters.count : rows_in_tile) * rank_blocks;  // units of a tile
+  // The K range is split over more CTAs the fewer units there can be (two CTAs fit an SM).
+  const int k32 = (args.k + 31) / 32;
+  args.cluster = 1;
+  while (args.cluster < kMaxCluster && tiles * most * args.cluster <= threshold_sms && args.cluster * kWarps * 2 <= k32) args.cluster *= 2;
+  int groups = 4 * threshold_sms / (tiles * args.cluster);
+  if (groups < 4) groups = 4;
+  if (groups > most) groups = most;
+  args.unit_groups = groups;
+  args.row_groups = (rows_in_tile + args.cluster - 1) / args.cluster;
+  const int lists = args.lists != nullptr ? static_cast<int>((args.rows + kLoraListRows - 1) / kLoraListRows) : 0;
+  const int blocks = tiles * (args.row_groups + args.unit_groups) * args.cluster + (lists + args.cluster - 1) / args.cluster * args.cluster;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(blocks));
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = smem_bytes;
+  config.dynamicSmemBytes = sizeof(UnitSums<kRankTiles>);
   config.stream = stream;
-  cudaLaunchAttribute attributes[2];
-  attributes[0].id = cudaLaunchAttributeClusterDimension;
-  attributes[0].val.clusterDim.x = static_cast<unsigned>(args.cluster);
-  attributes[0].val.clusterDim.y = 1;
-  attributes[0].val.clusterDim.z = 1;
-  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attributes[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attributes;
-  config.numAttrs = chained ? 2 : 1;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(args.cluster);
+  attribute.val.clusterDim.y = 1;
+  attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, kernel, args);
 }
 
-template <bool kVector, int kRankTiles>
-cudaError_t launch_front(FrontArgs args, cudaStream_t stream) {
-  const bool few = args.rows <= kFewRows;
-  const int tile_rows = few ? kUnitRows : kTileRows;
-  const int64_t tiles = (args.rows + tile_rows - 1) / tile_rows;
-  const int k32 = (args.k + 31) / 32;
-  args.cluster = 1;
-  const int rank_blocks = (args.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
-  // Units of a tile at most: its rows, and an adapter's groups of 32 rows.
-  const int64_t rows_in_tile = args.rows < tile_rows ? args.rows : tile_rows;
-  const int64_t by_adapter = args.adapters.count + (few ? 0 : rows_in_tile / kUnitRows);
-  const int64_t most = (by_adapter < rows_in_tile ? by_adapter : rows_in_tile) * rank_blocks;
-  // The K range is split over more CTAs the fewer units there are to fill the chip with: of few rows at most `most` a tile (two CTAs fit an SM), of many rows
-  // four a tile where requests follow each other and many more where they are mixed, so that the split ends with 16 clusters' worth of tiles (split for
-  // one unit in 32 rows, 2048 mixed rows of 7168 values with 64 adapters took 144 us instead of 83, for `most`, 1024 rows of 16384 in runs 171 instead of 138).
-  while (args.cluster < kMaxCluster && (few ? tiles * most * args.cluster <= threshold_sms : tiles * args.cluster < 16) && args.cluster * kWarps * 2 <= k32) {
-    args.cluster *= 2;
-  }
-  int64_t groups = 4ll * threshold_sms / (tiles * args.cluster);
-  if (groups < 4) groups = 4;
-  if (groups > most) groups = most;
-  args.unit_groups = static_cast<int>(groups);
-  const int64_t lists = args.lists != nullptr ? (args.rows + kLoraListRows - 1) / kLoraListRows : 0;
-  if (few) {
-    static PerDeviceOnce configured;
-    args.row_groups = static_cast<int>((rows_in_tile + args.cluster - 1) / args.cluster);
-    const int64_t blocks = tiles * (args.row_groups + args.unit_groups) * args.cluster + (lists + args.cluster - 1) / args.cluster * args.cluster;
-    return launch_clusters(lora_front_kernel<kVector, kRankTiles>, args, blocks, sizeof(UnitSums<kRankTiles>), false, &configured, stream);
-  }
-  if (args.rows + lists > (1ll << 31) - 1) return cudaErrorInvalidValue;
-  lora_rows_kernel<kVector><<<static_cast<unsigned>(args.rows + lists), kThreads, 0, stream>>>(args);
-  const cudaError_t error = cudaGetLastError();
-  if (error != cudaSuccess) return error;
-  static PerDeviceOnce configured;
-  return launch_clusters(lora_units_kernel<kVector, kRankTiles>, args, tiles * args.unit_groups * args.cluster, sizeof(UnitSums<kRankTiles>), true, &configured, stream);
-}
-
 template <bool kVector>
-cudaError_t launch_front_ranks(const FrontArgs& args, cudaStream_t stream) {
-  if (args.adapters.rank <= 16) return launch_front<kVector, 1>(args, stream);
-  if (args.adapters.rank <= 32) return launch_front<kVector, 2>(args, stream);
-  return launch_front<kVector, 4>(args, stream);
+cudaError_t launch_few_ranks(const FrontArgs& args, cudaStream_t stream) {
+  if (args.adapters.rank <= 16) return launch_few<kVector, 1>(args, stream);
+  if (args.adapters.rank <= 32) return launch_few<kVector, 2>(args, stream);
+  return launch_few<kVector, 4>(args, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_lora_front(const LoraGemmArgs& g, const uint16_t* x, int k, int8_t* q, float* scale, uint16_t* t, int* lists, int* row_slots, cudaStream_t stream) {
+cudaError_t launch_lora_front(const LoraGemmArgs& g, const uint16_t* x, int k, int8_t* q, float* scale, uint16_t* t, int* lists, int* row_slots,
+                              uint16_t* x_copy, cudaStream_t stream) {
   FrontArgs args = {};
   args.x = x;
   args.rows = g.rows;
@@ -585,7 +453,18 @@ cudaError_t launch_lora_front(const LoraGemmArgs& g, const uint16_t* x, int k, i
   args.row_slots = row_slots;
   args.status = g.status;
   const bool vector = k % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  return vector ? launch_front_ranks<true>(args, stream) : launch_front_ranks<false>(args, stream);
+  if (g.rows <= kLoraFewRows) return vector ? launch_few_ranks<true>(args, stream) : launch_few_ranks<false>(args, stream);
+  if (!vector && x_copy == nullptr) return cudaErrorInvalidValue;
+  args.x_copy = vector ? nullptr : x_copy;
+  const int64_t blocks = g.rows + (lists != nullptr ? (g.rows + kLoraListRows - 1) / kLoraListRows : 0);
+  if (blocks > (1ll << 31) - 1) return cudaErrorInvalidValue;
+  if (vector) {
+    lora_rows_kernel<true><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(args);
+  } else {
+    lora_rows_kernel<false><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(args);
+  }
+  const cudaError_t error = cudaGetLastError();
+  return error != cudaSuccess ? error : launch_lora_units(g, vector ? x : x_copy, k, !vector, t, stream);
 }
 
 }  // namespace fmoe

@@ -1,0 +1,373 @@
+// Coefficients of low-rank adapters for many rows: t[row] = scaling[a] * (A[a] x[row]) with a = the row's adapter, rows in any order.
+//
+// A tile of 128 rows is multiplied with every adapter that any of them uses (tcgen05.mma: rows are the lanes of tensor memory, the adapters' ranks side
+// by side its columns), and a row keeps the columns of its own: x is read once for all adapters of the tile, an adapter once for all rows, and the products
+// that nobody asked for cost the tensor core little next to the reading of x.  More adapters than 256 columns hold, or ranks above 64, are passes over x, the later ones
+// from L2.  Where there are few tiles, CTAs share a tile's passes, and a cluster splits the K range; the parts' sums meet in distributed shared memory in the order of the parts.
+// By mma.sync, with fragments straight from global memory as for few rows (lora_front.cu): 6680 rows of 1733 values, 4 adapters of rank 94: 62 us, 28 us like this; 8192 rows
+// of 16384, 16 adapters of rank 32: 79, 50 to 58 (42 is the reading of x).
+#include <cuda.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "lora.h"
+#include "ptx.cuh"
+
+namespace fmoe {
+
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kBlockK = 64;  // elements of K per pipeline stage: 128 bytes
+constexpr int kUmmaK = 16;
+constexpr int kThreads = 192;  // warp 0: TMA, warp 1: tensor memory and MMA, warps 2..5: a row each
+constexpr int kXBytes = kTileRows * kBlockK * 2;
+constexpr int kMaxColumns = 256;  // of a pass
+constexpr int kMaxStages = 12;
+constexpr int kMaxCluster = 8;
+constexpr int kMinPartBlocks = 2;  // K blocks of a part, at least
+constexpr int kRowFloats = kLoraRankBlock + 4;  // of a row in the exchange: no two of eight lanes in one bank group
+static_assert(sizeof(float) * kTileRows * kRowFloats <= 64 * 1024, "the exchange lies where the stages do");
+
+struct UnitsArgs {
+  int64_t rows;
+  int k_blocks, cluster;
+  int groups;  // clusters that share a tile's passes
+  LoraAdapters adapters;
+  uint16_t* t;
+  int planes;
+  int behind;       // x is written by the kernel in front
+  int stage_bytes;  // shared memory for stages
+  int* status;
+};
+
+struct Control {
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
+  uint64_t acc_full;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+  int slots;
+  int warp_count[4];
+  alignas(16) int id[kTileRows];
+  int slot_at[kTileRows];       // of a row that is the first of its adapter
+  int slot_adapter[kTileRows];
+  int slot[kTileRows];          // of a row, -1 = no adapter
+  float scaling[kTileRows];     // of a slot's adapter
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float4 load_cluster_float4(uint32_t smem_address, int cta) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_address), "r"(cta));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      :
+      : "r"(ptx::smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__global__ void __launch_bounds__(kThreads)
+lora_units_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap a_map, const __grid_constant__ UnitsArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // [128 rows][64 ranks] over the stages: it is written when all products of a pass are there, and read before the next pass loads.
+  float* const exchange = reinterpret_cast<float*>(smem);
+  Control* ctl = reinterpret_cast<Control*>(smem + args.stage_bytes);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  int* status = args.status;
+  const int parts = args.cluster;
+  const int part = static_cast<int>(blockIdx.x) % parts;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x) / parts / args.groups;
+  const int group = static_cast<int>(blockIdx.x) / parts % args.groups;
+  const int64_t row0 = tile * kTileRows;
+  const int tile_rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), args.rows - row0));
+  const int kb_begin = part * args.k_blocks / parts;
+  const int count = (part + 1) * args.k_blocks / parts - kb_begin;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kMaxStages; ++s) {
+      ptx::mbar_init(&ctl->full[s], 1);
+      ptx::mbar_init(&ctl->empty[s], 1);
+    }
+    ptx::mbar_init(&ctl->acc_full, 1);
+    ctl->abort_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(&ctl->tmem_base, kMaxColumns);
+    ptx::tmem_relinquish();
+  }
+  ptx::launch_dependents();  // behind the allocation: a kernel that starts early takes what is left
+  // The adapters of the tile, each once in the order of its first row: warps 2..5 hold a row a thread.
+  const int i = static_cast<int>(threadIdx.x) - 64;
+  int mine = -1;
+  if (i >= 0) {
+    mine = i < tile_rows ? load_adapter_id(args.adapters, row0 + i) : -1;
+    ctl->id[i] = mine;
+  }
+  __syncthreads();
+  int first = i;
+  bool owner = false;
+  unsigned owners = 0;
+  if (i >= 0) {
+    if (mine >= 0) {
+      for (int j = 0; j < i; j += 4) {
+        const int4 others = *reinterpret_cast<const int4*>(&ctl->id[j]);
+        const int four[4] = {others.x, others.y, others.z, others.w};
+#pragma unroll
+        for (int c = 3; c >= 0; --c) {
+          if (four[c] == mine && j + c < first) first = j + c;
+        }
+      }
+    }
+    owner = mine >= 0 && first == i;
+    __syncwarp();
+    owners = __ballot_sync(0xffffffffu, owner);
+    if (lane == 0) ctl->warp_count[warp - 2] = __popc(owners);
+  }
+  __syncthreads();
+  if (i >= 0) {
+    int slot = __popc(owners & ((1u << lane) - 1)), slots = 0;
+    for (int w = 0; w < 4; ++w) {
+      if (w < warp - 2) slot += ctl->warp_count[w];
+      slots += ctl->warp_count[w];
+    }
+    if (owner) {
+      ctl->slot_adapter[slot] = mine;
+      ctl->scaling[slot] = __ldcg(args.adapters.scaling + mine);
+      ctl->slot_at[i] = slot;
+    }
+    if (i == 0) ctl->slots = slots;
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::tcgen05_fence_after();
+  if (i >= 0) ctl->slot[i] = mine >= 0 ? ctl->slot_at[first] : -1;
+  __syncthreads();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, ctl->tmem_base, 0);
+  const int slots = __shfl_sync(0xffffffffu, ctl->slots, 0);
+  volatile int* abort_flag = &ctl->abort_flag;
+
+  const int rank = args.adapters.rank;
+  const int rank_padded = lora_rank_padded(rank);
+  const int rank_blocks = (rank + kLoraRankBlock - 1) / kLoraRankBlock;
+  const int columns = min(kLoraRankBlock, rank_padded);  // of an adapter
+  const int per_pass = kMaxColumns / columns;            // adapters of a pass
+  const int slot_groups = (slots + per_pass - 1) / per_pass;
+  const int passes = slot_groups * rank_blocks;
+  const uint32_t adapter_bytes = static_cast<uint32_t>(columns) * 128;
+  // Stages are as large as the widest pass needs.
+  const uint32_t stage_size = kXBytes + min(per_pass, slots) * adapter_bytes;
+  const int stages = min(kMaxStages, args.stage_bytes / static_cast<int>(stage_size));  // at least two (launch_lora_units)
+  int stage = 0;
+  uint32_t phase = 0;
+  auto advance = [&]() {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  };
+  const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id % 4
+  const int my_row = quarter * 32 + lane;
+  if (args.behind) ptx::grid_dependency_wait();
+  int done = 0;  // passes of this CTA
+  for (int pass = group; pass < passes; pass += args.groups, ++done) {
+    const int rank0 = pass / slot_groups * kLoraRankBlock;
+    const int slot0 = pass % slot_groups * per_pass;
+    const int here = min(per_pass, slots - slot0);
+    if (warp == 0) {
+      // ---------------- TMA producer (the whole warp walks the loop, one elected lane issues) ----------------
+      const bool issuer = ptx::elect_one();
+      for (int b = 0; b < count; ++b) {
+        ptx::mbar_wait(&ctl->empty[stage], phase ^ 1u, abort_flag, status, 91);
+        if (issuer) {
+          uint8_t* const to = smem + static_cast<size_t>(stage) * stage_size;
+          const int k0 = (kb_begin + b) * kBlockK;
+          ptx::mbar_arrive_expect_tx(&ctl->full[stage], kXBytes + here * adapter_bytes);
+          ptx::tma_load_2d(to, &x_map, &ctl->full[stage], k0, static_cast<int>(row0));
+          for (int g = 0; g < here; ++g) tma_load_3d(to + kXBytes + g * adapter_bytes, &a_map, &ctl->full[stage], k0, rank0, ctl->slot_adapter[slot0 + g]);
+        }
+        advance();
+      }
+    } else if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      const bool issuer = ptx::elect_one();
+      const uint32_t idesc = ptx::make_instr_desc(false, kTileRows, here * columns);
+      for (int b = 0; b < count; ++b) {
+        ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 92);
+        ptx::tcgen05_fence_after();
+        const uint32_t stage_addr = ptx::smem_u32(smem + static_cast<size_t>(stage) * stage_size);
+        if (issuer) {
+#pragma unroll
+          for (int ks = 0; ks < kBlockK / kUmmaK; ++ks) {
+            ptx::umma_ss<false>(tmem_base, ptx::make_smem_desc_sw128(stage_addr + ks * kUmmaK * 2),
+                                ptx::make_smem_desc_sw128(stage_addr + kXBytes + ks * kUmmaK * 2), idesc, (b > 0 || ks > 0) ? 1u : 0u);
+          }
+          ptx::tcgen05_commit(&ctl->empty[stage]);
+        }
+        advance();
+      }
+      if (issuer) ptx::tcgen05_commit(&ctl->acc_full);
+    } else {
+      // ---------------- a row keeps the columns of its adapter ----------------
+      const int my_slot = ctl->slot[my_row];
+      const uint32_t acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+      ptx::mbar_wait(&ctl->acc_full, static_cast<uint32_t>(done) & 1u, abort_flag, status, 93);
+      ptx::tcgen05_fence_after();
+      for (int g = 0; g < here; ++g) {
+        const bool keep = my_slot == slot0 + g;
+        if (__ballot_sync(0xffffffffu, keep) == 0) continue;
+        for (int c = 0; c < columns; c += 16) {
+          uint32_t bits[16];
+          ptx::tmem_ld_x8(acc + g * columns + c, bits);
+          ptx::tmem_ld_x8(acc + g * columns + c + 8, bits + 8);
+          ptx::tmem_ld_wait();
+          if (keep) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              *reinterpret_cast<uint4*>(exchange + my_row * kRowFloats + c + 4 * q) = make_uint4(bits[4 * q], bits[4 * q + 1], bits[4 * q + 2], bits[4 * q + 3]);
+            }
+          }
+          __syncwarp();
+        }
+      }
+      ptx::tcgen05_fence_before();
+    }
+    __syncwarp();
+    cluster_sync();  // every part's sums lie in its shared memory, and tensor memory may be written again
+    ptx::tcgen05_fence_after();
+    // A thread finishes four ranks of a row; every parts-th row is this CTA's.
+    const int own = (tile_rows - part + parts - 1) / parts, quads = columns / 4;
+    for (int e = threadIdx.x; e < own * quads; e += kThreads) {
+      const int index = e / quads, r = 4 * (e - index * quads);
+      const int row = part + parts * index;
+      const int slot = ctl->slot[row];
+      if (slot < slot0 || slot >= slot0 + here || rank0 + r >= rank_padded) continue;
+      const uint32_t at = ptx::smem_u32(exchange + row * kRowFloats + r);
+      float4 values[kMaxCluster];
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) values[c] = c < parts ? load_cluster_float4(at, c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float rest[4] = {values[0].x, values[0].y, values[0].z, values[0].w};
+#pragma unroll
+      for (int c = 1; c < kMaxCluster; ++c) {
+        rest[0] += values[c].x;
+        rest[1] += values[c].y;
+        rest[2] += values[c].z;
+        rest[3] += values[c].w;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) rest[q] = rank0 + r + q < rank ? __fmul_rn(rest[q], ctl->scaling[slot]) : 0.0f;
+      uint16_t* to = args.t + (row0 + row) * rank_padded + rank0 + r;
+      for (int plane = 0; plane < args.planes; ++plane) {
+        uint32_t bits[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          bits[q] = __bfloat16_as_ushort(__float2bfloat16_rn(rest[q]));
+          rest[q] = __fsub_rn(rest[q], bf16_bits_to_f32(static_cast<uint16_t>(bits[q])));  // exact; what is left of an infinity (NaN) is not wanted
+          if (!isfinite(rest[q])) rest[q] = 0.0f;
+        }
+        *reinterpret_cast<uint2*>(to) = make_uint2(bits[0] | bits[1] << 16, bits[2] | bits[3] << 16);
+        to += args.rows * rank_padded;
+      }
+    }
+    asm volatile("fence.proxy.async;" ::: "memory");  // the next loads overwrite the exchange
+    __syncwarp();
+    cluster_sync();  // nobody still reads these sums
+  }
+  // Drain: every load must have landed before the CTA may exit (the MMA warp has consumed them unless it gave up).
+  if (warp == 0) {
+    const int pending = min(stages, done * count);
+    for (int back = 0; back < pending; ++back) {
+      int s = stage - 1 - back;
+      uint32_t p = phase;
+      if (s < 0) {
+        s += stages;
+        p ^= 1u;
+      }
+      const unsigned long long start = ptx::global_timer_ns();
+      while (!ptx::mbar_try_wait(&ctl->full[s], p)) {
+        if (ptx::global_timer_ns() - start > ptx::kWaitLimitNs) break;
+      }
+    }
+  }
+  ptx::grid_dependency_wait();  // this kernel's end stands for the end of the one in front too
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tcgen05_fence_after();
+    ptx::tmem_dealloc(tmem_base, kMaxColumns);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_lora_units(const LoraGemmArgs& g, const uint16_t* x, int k, bool behind, uint16_t* t, cudaStream_t stream) {
+  UnitsArgs args = {};
+  args.rows = g.rows;
+  args.k_blocks = (k + kBlockK - 1) / kBlockK;
+  args.adapters = g.adapters;
+  args.t = t;
+  args.planes = g.planes;
+  args.behind = behind ? 1 : 0;
+  args.status = g.status;
+  const int columns = lora_rank_padded(g.adapters.rank) < kLoraRankBlock ? lora_rank_padded(g.adapters.rank) : kLoraRankBlock;
+  const int most = g.adapters.count < kTileRows ? g.adapters.count : kTileRows;
+  const int widest = most * columns < kMaxColumns ? most * columns : kMaxColumns / columns * columns;
+  // Two stages of the widest pass at least, and two CTAs on an SM; a tile of requests that follow each other uses one or two adapters, and has more stages.
+  args.stage_bytes = 2 * (kXBytes + widest * 128);
+  if (args.stage_bytes < 64 * 1024) args.stage_bytes = 64 * 1024;
+  const size_t smem_bytes = 1024 + args.stage_bytes + sizeof(Control);
+  CUtensorMap maps[2];
+  const uint64_t stride = (static_cast<uint64_t>(k) + 7) / 8 * 8;
+  if (!make_sw128_map(&maps[0], x, false, static_cast<uint64_t>(g.rows), static_cast<uint64_t>(k), kTileRows, stride) ||
+      !make_adapter_map(&maps[1], g.adapters.a, static_cast<uint64_t>(k), static_cast<uint64_t>(g.adapters.rank), static_cast<uint64_t>(g.adapters.count),
+                        static_cast<uint64_t>(g.adapters.a_stride), kBlockK, static_cast<uint32_t>(columns))) {
+    return cudaErrorInvalidValue;
+  }
+  static PerDeviceOnce configured;
+  const int device = current_device_ordinal();
+  if (configured.needed(device)) {
+    const cudaError_t error = cudaFuncSetAttribute(lora_units_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(1024 + 2 * (kXBytes + kMaxColumns * 128) + sizeof(Control)));
+    if (error != cudaSuccess) return error;
+    configured.mark(device);
+  }
+  const int64_t tiles = (g.rows + kTileRows - 1) / kTileRows;
+  // The K range is split where there are too few tiles to fill the chip.
+  args.cluster = 1;
+  while (args.cluster < kMaxCluster && args.cluster * 2 * kMinPartBlocks <= args.k_blocks && tiles * args.cluster < threshold_sms) args.cluster *= 2;
+  // So are the passes, as many as a tile may need.
+  const int64_t most_passes = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock * static_cast<int64_t>((most * columns + kMaxColumns - 1) / kMaxColumns);
+  args.groups = static_cast<int>(2 * threshold_sms / (tiles * args.cluster));
+  if (args.groups > most_passes) args.groups = static_cast<int>(most_passes);
+  if (args.groups < 1) args.groups = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(tiles * args.groups * args.cluster));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem_bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = static_cast<unsigned>(args.cluster);
+  attributes[0].val.clusterDim.y = 1;
+  attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
+  return cudaLaunchKernelEx(&config, lora_units_kernel, maps[0], maps[1], args);
+}
+
+}  // namespace fmoe
