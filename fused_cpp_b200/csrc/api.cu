@@ -1126,8 +1126,8 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
                                           swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(derivatives), words, stream, false);
   }
   if (error == cudaSuccess) {
-    const fmoe::DenseProductArgs down = {{static_cast<const uint16_t*>(h), inter}, {static_cast<const uint16_t*>(w2), inter}, static_cast<uint16_t*>(y), rows, hidden, inter};
-    error = fmoe::launch_dense_products(fmoe::DenseForm::kRowsRows, &down, 1, words, stream, true);
+    const fmoe::DenseProductArgs down = {{static_cast<const uint16_t*>(h), inter}, {static_cast<const uint16_t*>(w2), inter}, static_cast<uint16_t*>(y), rows, hidden, inter, false};
+    error = fmoe::launch_dense_rows(down, words, stream, true);
   }
   return error == cudaSuccess ? FMOE_OK : cuda_fail(error, what);
 }
@@ -1163,25 +1163,30 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
                    static_cast<uint16_t*>(d_gate_up), words, stream, chained);
     chained = true;
   }
-  if (error == cudaSuccess && dx != nullptr) {
-    const fmoe::DenseProductArgs product = {{static_cast<const uint16_t*>(d_gate_up), 2 * static_cast<int64_t>(inter)},
-                                            {static_cast<const uint16_t*>(w13), hidden}, static_cast<uint16_t*>(dx), rows, hidden, 2 * static_cast<int64_t>(inter)};
-    error = small ? fmoe::launch_dense_small(static_cast<const uint16_t*>(d_gate_up), rows, 2 * inter, static_cast<const uint16_t*>(w13), hidden, true,
-                                             static_cast<uint16_t*>(dx), words, stream, chained)
-                  : fmoe::launch_dense_products(fmoe::DenseForm::kRowsByK, &product, 1, words, stream, chained);
-    chained = true;
-  }
-  // Both weight gradients in one launch: apart, each ends with a wave of tiles that does not fill the chip.
-  fmoe::DenseProductArgs products[2];
+  // What is left does not depend on each other.  One launch: apart, each product ends with a round of tiles that does not fill the chip.
+  fmoe::DenseProductArgs products[3];
   int count = 0;
+  if (dx != nullptr) {
+    if (small) {  // few tiles of a long K, which is split
+      if (error == cudaSuccess) {
+        error = fmoe::launch_dense_small(static_cast<const uint16_t*>(d_gate_up), rows, 2 * inter, static_cast<const uint16_t*>(w13), hidden, true,
+                                         static_cast<uint16_t*>(dx), words, stream, chained);
+      }
+      chained = true;
+    } else {
+      products[count++] = {{static_cast<const uint16_t*>(d_gate_up), 2 * static_cast<int64_t>(inter)}, {static_cast<const uint16_t*>(w13), hidden},
+                           static_cast<uint16_t*>(dx), rows, hidden, 2 * static_cast<int64_t>(inter), false};
+    }
+  }
   if (dw13 != nullptr) {
     products[count++] = {{static_cast<const uint16_t*>(d_gate_up), 2 * static_cast<int64_t>(inter)}, {static_cast<const uint16_t*>(x), x_stride},
-                         static_cast<uint16_t*>(dw13), 2 * static_cast<int64_t>(inter), hidden, rows};
+                         static_cast<uint16_t*>(dw13), 2 * static_cast<int64_t>(inter), hidden, rows, true};
   }
   if (dw2 != nullptr) {
-    products[count++] = {{static_cast<const uint16_t*>(dy), dy_stride}, {static_cast<const uint16_t*>(h), inter}, static_cast<uint16_t*>(dw2), hidden, inter, rows};
+    products[count++] = {{static_cast<const uint16_t*>(dy), dy_stride}, {static_cast<const uint16_t*>(h), inter}, static_cast<uint16_t*>(dw2), hidden, inter,
+                         rows, true};
   }
-  if (error == cudaSuccess && count > 0) error = fmoe::launch_dense_products(fmoe::DenseForm::kByKByK, products, count, words, stream, chained);
+  if (error == cudaSuccess && count > 0) error = fmoe::launch_dense_gradients(products, count, words, stream, chained);
   return error == cudaSuccess ? FMOE_OK : cuda_fail(error, what);
 }
 

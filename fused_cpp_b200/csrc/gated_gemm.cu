@@ -55,6 +55,8 @@ struct TileConfig {
   static_assert(kSmemBytes <= 227 * 1024, "a CTA has 227 KB of shared memory");
 };
 
+constexpr int kMaxProblems = 3;
+
 struct Control {
   uint64_t full[kMaxStages];
   uint64_t empty[kMaxStages];
@@ -70,11 +72,41 @@ struct Problem {
   int n;         // output channels
   int k_blocks;
   int m_tiles, n_tiles;
+  int a_by_k;
+};
+
+struct Maps {
+  CUtensorMap a[kMaxProblems], b[kMaxProblems], out[kMaxProblems];
+};
+
+// Which tiles a pair works on.  Tiles come in one or two classes, the first with the longer K range: pair j takes the tiles j, j + pairs, ... of it, so
+// that pairs from `left_out` on have one less if the last round is not full.  These take `ahead` rounds of the second class first, then all pairs
+// together the rest, the pairs from `turn` on in front.
+struct Schedule {
+  int first, total;  // tiles of the first class, and of both
+  int pairs, rounds, left_out, ahead, turn;  // rounds = first / pairs
+
+  // The tile of pair `pair` in its round `round`; -1 behind its last one.
+  __host__ __device__ __forceinline__ int tile(int pair, int round) const {
+    const int own = rounds + (pair < left_out ? 1 : 0);
+    if (round < own) return round * pairs + pair;
+    round -= own;
+    int index = first;
+    if (pair >= left_out && round < ahead) {
+      index += round * (pairs - left_out) + pair - left_out;
+    } else {
+      if (pair >= left_out) round -= ahead;
+      const int place = pair >= turn ? pair - turn : pair - turn + pairs;
+      index += ahead * (pairs - left_out) + round * pairs + place;
+    }
+    return index < total ? index : -1;
+  }
 };
 
 struct Args {
-  Problem problem[2];
-  int64_t tiles[2];  // tiles of the first problem, and of both
+  Problem problem[kMaxProblems];
+  int tiles[kMaxProblems];  // tiles up to and with each problem
+  Schedule schedule;
   int keep;             // the forward pass stores the derivatives
   float4* derivatives;  // see derivative_block
   int activation;
@@ -88,11 +120,11 @@ struct Tile {
 
 // Tiles in the order of their numbers: groups of kTileGroup row tiles, inside a group all row tiles of a column tile before the next one, so that the
 // tiles in flight (74 pairs) share both their A rows and their B rows in L2.
-__device__ __forceinline__ Tile tile_at(const Args& args, int64_t index) {
+__device__ __forceinline__ Tile tile_at(const Args& args, int index) {
   Tile t;
-  t.problem = index >= args.tiles[0] ? 1 : 0;
+  t.problem = index < args.tiles[0] ? 0 : index < args.tiles[1] ? 1 : 2;
   const Problem& p = args.problem[t.problem];
-  const int local = static_cast<int>(index - (t.problem ? args.tiles[0] : 0));
+  const int local = index - (t.problem > 0 ? args.tiles[t.problem - 1] : 0);
   const int per_group = kTileGroup * p.n_tiles;
   const int group = local / per_group;
   const int rest = local - group * per_group;
@@ -141,11 +173,10 @@ struct Staging {
   }
 };
 
+// kAByK: how A lies in memory is the problem's to say (otherwise all rows run along k).
 template <Epilogue kEpilogue, bool kAByK, bool kBByK, int kTileN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_constant__ CUtensorMap b_map0,
-                       const __grid_constant__ CUtensorMap a_map1, const __grid_constant__ CUtensorMap b_map1,
-                       const __grid_constant__ CUtensorMap out_map0, const __grid_constant__ CUtensorMap out_map1, const __grid_constant__ Args args) {
+gated_pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args args) {
   using Cfg = TileConfig<kTileN>;
   constexpr int kStages = Cfg::kStages;
   constexpr int kColumns = kEpilogue == Epilogue::kGated ? kTileN / 2 : kTileN;  // output channels of a tile
@@ -159,9 +190,7 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
   const uint32_t cta = cluster_cta_rank();
   const bool leader = cta == 0;
   int* status = args.status;
-  const int64_t tiles = args.tiles[1];
-  const int64_t first_tile = blockIdx.x >> 1;
-  const int64_t tile_stride = gridDim.x >> 1;
+  const int pair = static_cast<int>(blockIdx.x >> 1);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -196,11 +225,12 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
     int stage = 0;
     uint32_t phase = 0;
     int issued = 0;
-    for (int64_t index = first_tile; index < tiles; index += tile_stride) {
+    for (int round = 0, index; (index = args.schedule.tile(pair, round)) >= 0; ++round) {
       const Tile tile = tile_at(args, index);
-      const CUtensorMap* const a_map = tile.problem ? &a_map1 : &a_map0;
-      const CUtensorMap* const b_map = tile.problem ? &b_map1 : &b_map0;
+      const CUtensorMap* const a_map = &maps.a[tile.problem];
+      const CUtensorMap* const b_map = &maps.b[tile.problem];
       const int k_blocks = args.problem[tile.problem].k_blocks;
+      const bool a_by_k = kAByK && args.problem[tile.problem].a_by_k;
       const int a_row = tile.m * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta);
       const int b_row = kEpilogue == Epilogue::kGated ? tile.n * kColumns + static_cast<int>(cta) * args.problem[0].n
                                                       : tile.n * kTileN + Cfg::kBRows * static_cast<int>(cta);
@@ -211,7 +241,7 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
           const uint32_t bar = full_leader0 + 8u * static_cast<uint32_t>(stage);
           if (leader) ptx::mbar_arrive_expect_tx(&ctl->full[stage], 2 * Cfg::kStageBytes);
           const int k0 = kb * kBlockK;
-          if constexpr (kAByK) {
+          if (a_by_k) {
             tma_load_2d_pair(dst, a_map, bar, a_row, k0);
             tma_load_2d_pair(dst + kChunkBytes, a_map, bar, a_row + 64, k0);
           } else {
@@ -255,11 +285,9 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
       // operand lie kChunkBytes apart (leading offset), groups of eight K rows 1024 bytes (stride offset), and the next 16
       // K elements are two such groups on.
       constexpr uint32_t kByKLead = static_cast<uint32_t>(kChunkBytes >> 4) << 16;
-      constexpr uint32_t kALead = kAByK ? kByKLead : (1u << 16);
       constexpr uint32_t kBLead = kBByK ? kByKLead : (1u << 16);
-      constexpr uint32_t kAStep = kAByK ? 2048 >> 4 : 32 >> 4;
       constexpr uint32_t kBStep = kBByK ? 2048 >> 4 : 32 >> 4;
-      constexpr uint32_t kIdesc = ptx::make_instr_desc(false, 2 * kRowsPerCta, kTileN) | (kAByK ? 1u << 15 : 0u) | (kBByK ? 1u << 16 : 0u);
+      constexpr uint32_t kIdesc = ptx::make_instr_desc(false, 2 * kRowsPerCta, kTileN) | (kBByK ? 1u << 16 : 0u);
       const uint32_t desc_hi = static_cast<uint32_t>(1024 >> 4) | (1u << 14) | (2u << 29);
       const uint32_t stage0 = (smem_base & 0x3ffffu) >> 4;
       const uint32_t empty_c0 = map_to_cta(ptx::smem_u32(&ctl->empty[0]), 0);
@@ -269,11 +297,15 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
       int stage = 0;
       uint32_t phase = 0;
       uint32_t stage_lo = stage0;
-      int local = 0;
-      for (int64_t index = first_tile; index < tiles; index += tile_stride, ++local) {
-        const int k_blocks = args.problem[index >= args.tiles[0] ? 1 : 0].k_blocks;
-        const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
-        const uint32_t use = static_cast<uint32_t>(local) >> 1;
+      for (int round = 0, index; (index = args.schedule.tile(pair, round)) >= 0; ++round) {
+        const Problem& p = args.problem[index < args.tiles[0] ? 0 : index < args.tiles[1] ? 1 : 2];
+        const int k_blocks = p.k_blocks;
+        const bool a_by_k = kAByK && p.a_by_k;
+        const uint32_t a_lead = a_by_k ? kByKLead : (1u << 16);
+        const uint32_t a_step = a_by_k ? 2048 >> 4 : 32 >> 4;
+        const uint32_t idesc = kIdesc | (a_by_k ? 1u << 15 : 0u);
+        const uint32_t buffer = static_cast<uint32_t>(round) & 1u;
+        const uint32_t use = static_cast<uint32_t>(round) >> 1;
         const uint32_t acc = tmem_base + kTileN * buffer;
         ptx::mbar_wait(&ctl->acc_empty[buffer], (use & 1u) ^ 1u, abort_flag, status, 42);
         ptx::tcgen05_fence_after();
@@ -282,11 +314,11 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
           ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 43);
           ptx::tcgen05_fence_after();
           if (issuer) {
-            const uint32_t a_lo = stage_lo | kALead;
+            const uint32_t a_lo = stage_lo | a_lead;
             const uint32_t b_lo = (stage_lo + (Cfg::kABytes >> 4)) | kBLead;
 #pragma unroll
             for (uint32_t ks = 0; ks < kBlockK / kUmmaK; ++ks) {
-              umma_pair<false>(acc, a_lo + kAStep * ks, b_lo + kBStep * ks, desc_hi, kIdesc, ks == 0 ? accumulate : 1u);
+              umma_pair<false>(acc, a_lo + a_step * ks, b_lo + kBStep * ks, desc_hi, idesc, ks == 0 ? accumulate : 1u);
             }
             tcgen05_commit_pair(empty_c0 + 8u * static_cast<uint32_t>(stage));
             tcgen05_commit_pair(empty_c1 + 8u * static_cast<uint32_t>(stage));
@@ -315,13 +347,12 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
     const Staging staging = {staging_base + (warp - 2) * kStagingBytes, lane};
     const uint32_t acc_lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t acc_empty_leader = map_to_cta(ptx::smem_u32(&ctl->acc_empty[0]), 0);
-    int local = 0;
-    for (int64_t index = first_tile; index < tiles; index += tile_stride, ++local) {
+    for (int round = 0, index; (index = args.schedule.tile(pair, round)) >= 0; ++round) {
       const Tile tile = tile_at(args, index);
       const Problem& p = args.problem[tile.problem];
-      const CUtensorMap* const out_map = tile.problem ? &out_map1 : &out_map0;
-      const uint32_t buffer = static_cast<uint32_t>(local) & 1u;
-      const uint32_t use = static_cast<uint32_t>(local) >> 1;
+      const CUtensorMap* const out_map = &maps.out[tile.problem];
+      const uint32_t buffer = static_cast<uint32_t>(round) & 1u;
+      const uint32_t use = static_cast<uint32_t>(round) >> 1;
       const int warp_row = tile.m * 2 * kRowsPerCta + kRowsPerCta * static_cast<int>(cta) + quarter * 32;  // below 2^31 (check_gated_shape)
       const int n0 = tile.n * kColumns;
       const uint32_t acc = acc_lane_base + kTileN * buffer;
@@ -359,7 +390,7 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
               }
             });
           }
-          staging.end([&](uint32_t block) { tma_store_2d(&out_map0, block, col, warp_row); });
+          staging.end([&](uint32_t block) { tma_store_2d(out_map, block, col, warp_row); });
         } else if constexpr (kEpilogue == Epilogue::kGatedBack) {
           uint32_t d_up[32];  // 64 channels, kept while those of d_gate are on their way out
           staging.begin();
@@ -385,11 +416,11 @@ gated_pair_gemm_kernel(const __grid_constant__ CUtensorMap a_map0, const __grid_
 #pragma unroll
             for (int q = 0; q < 4; ++q) staging.put(4 * half + q, make_uint4(d_gate[4 * q], d_gate[4 * q + 1], d_gate[4 * q + 2], d_gate[4 * q + 3]));
           }
-          staging.end([&](uint32_t block) { tma_store_3d(&out_map0, block, col, 0, warp_row); });
+          staging.end([&](uint32_t block) { tma_store_3d(out_map, block, col, 0, warp_row); });
           staging.begin();
 #pragma unroll
           for (int q = 0; q < 8; ++q) staging.put(q, make_uint4(d_up[4 * q], d_up[4 * q + 1], d_up[4 * q + 2], d_up[4 * q + 3]));
-          staging.end([&](uint32_t block) { tma_store_3d(&out_map0, block, col, 1, warp_row); });
+          staging.end([&](uint32_t block) { tma_store_3d(out_map, block, col, 1, warp_row); });
         } else {
           uint32_t bits[64];
           tmem_ld_x32(from, bits);
@@ -428,10 +459,65 @@ struct Operands {
   DenseOperand a, b;
   int64_t b_rows;  // rows of B along its n axis in memory (2 * inter for the gated projection)
   uint16_t* out;   // [m, n], or [m, 2, n] for the gated backward product
+  int64_t k;
+  bool a_by_k;
 };
 
+// The schedule of tiles of at most two lengths, with what the longest pair takes, in K blocks.
+struct Plan {
+  Schedule schedule;
+  int64_t blocks;
+};
+
+Plan plan_tiles(int64_t first, int64_t first_blocks, int64_t second, int64_t second_blocks, int64_t pairs) {
+  Plan best = {{}, INT64_MAX};
+  const int64_t left_out = first % pairs, others = pairs - left_out;
+  const int64_t most = left_out > 0 && second_blocks > 0 ? first_blocks / second_blocks + 1 : 0;
+  for (int64_t ahead = most > 0 ? most - 1 : 0; ahead <= most; ++ahead) {
+    const int64_t rest = second - ahead * others > 0 ? second - ahead * others : 0;
+    int64_t load[2] = {first / pairs * first_blocks + rest / pairs * second_blocks, 0};  // of the pairs below left_out, and of the others
+    load[1] = load[0] + (second < ahead * others ? (second + others - 1) / others : ahead) * second_blocks;
+    if (left_out > 0) load[0] += first_blocks;
+    const int lighter = load[1] <= load[0] || left_out == 0 ? 1 : 0;
+    const int64_t width = lighter ? others : left_out;
+    if (rest % pairs > 0) load[lighter] += second_blocks;
+    if (rest % pairs > width) load[1 - lighter] += second_blocks;
+    const int64_t blocks = load[0] > load[1] ? load[0] : load[1];
+    if (blocks < best.blocks) {
+      best = {{static_cast<int>(first), static_cast<int>(first + second), static_cast<int>(pairs), static_cast<int>(first / pairs), static_cast<int>(left_out), static_cast<int>(ahead),
+               static_cast<int>(lighter ? left_out : 0)},
+              blocks};
+    }
+  }
+  return best;
+}
+
+constexpr int64_t kStoreBlocks = 6;  // a tile takes no less than its store, as long as this many K blocks
+
+int64_t tile_blocks(int64_t k) {
+  const int64_t blocks = (k + kBlockK - 1) / kBlockK;
+  return blocks > kStoreBlocks ? blocks : kStoreBlocks;
+}
+
+// Tiles of the problems with the longest K range, which lead the list, and of the others.
+template <Epilogue kEpilogue, int kTileN>
+Plan plan_form(const Args& args, const Operands* operands, int count) {
+  constexpr int kColumns = kEpilogue == Epilogue::kGated ? kTileN / 2 : kTileN;
+  int64_t tiles[2] = {0, 0}, blocks[2] = {tile_blocks(operands[0].k), 0};
+  for (int i = 0; i < count; ++i) {
+    const Problem& p = args.problem[i];
+    const int other = operands[i].k != operands[0].k ? 1 : 0;
+    tiles[other] += (p.m + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta) * ((p.n + kColumns - 1) / kColumns);
+    blocks[other] = tile_blocks(operands[i].k);
+  }
+  if (tiles[0] + tiles[1] > (1ll << 30)) return {{}, -1};
+  int64_t pairs = sm_count_of_current_device() / 2;
+  if (pairs > tiles[0] + tiles[1]) pairs = tiles[0] + tiles[1];
+  return plan_tiles(tiles[0], blocks[0], tiles[1], blocks[1], pairs);
+}
+
 template <Epilogue kEpilogue, bool kAByK, bool kBByK, int kTileN>
-cudaError_t launch_tiles(Args args, const Operands* operands, int count, const int64_t* depth, cudaStream_t stream, bool chained) {
+cudaError_t launch_tiles(Args& args, const Operands* operands, int count, const Schedule& schedule, cudaStream_t stream, bool chained) {
   using Cfg = TileConfig<kTileN>;
   auto kernel = gated_pair_gemm_kernel<kEpilogue, kAByK, kBByK, kTileN>;
   static PerDeviceOnce configured;
@@ -442,56 +528,45 @@ cudaError_t launch_tiles(Args args, const Operands* operands, int count, const i
     configured.mark(device);
   }
   constexpr int kColumns = kEpilogue == Epilogue::kGated ? kTileN / 2 : kTileN;
-  CUtensorMap maps[6];
+  Maps maps;
   int64_t total = 0;
-  for (int i = 0; i < 2; ++i) {
-    const int from = i < count ? i : 0;
-    Problem& p = args.problem[i];
-    if (i >= count) p = args.problem[0];
-    const Operands& o = operands[from];
-    const uint64_t m = static_cast<uint64_t>(p.m), n = static_cast<uint64_t>(o.b_rows), k = static_cast<uint64_t>(depth[from]);
-    const bool ok = make_sw128_map(&maps[2 * i], o.a.data, false, kAByK ? k : m, kAByK ? m : k, kAByK ? kBlockK : kRowsPerCta, o.a.stride) &&
-                    make_sw128_map(&maps[2 * i + 1], o.b.data, false, kBByK ? k : n, kBByK ? n : k, kBByK ? kBlockK : Cfg::kBRows, o.b.stride);
-    if (!ok) return cudaErrorInvalidValue;
-    bool out_ok;
-    if (kEpilogue == Epilogue::kGatedBack) {
-      out_ok = make_store_map(&maps[4 + i], o.out, false, static_cast<uint64_t>(p.n), 2, m);
-    } else {
-      out_ok = make_store_map(&maps[4 + i], o.out, false, static_cast<uint64_t>(p.n), 1, m);
+  for (int i = 0; i < kMaxProblems; ++i) {
+    if (i >= count) {  // not reached by any tile
+      args.problem[i] = args.problem[0];
+      args.tiles[i] = static_cast<int>(total);
+      maps.a[i] = maps.a[0];
+      maps.b[i] = maps.b[0];
+      maps.out[i] = maps.out[0];
+      continue;
     }
-    if (!out_ok) return cudaErrorInvalidValue;
+    Problem& p = args.problem[i];
+    const Operands& o = operands[i];
+    const uint64_t m = static_cast<uint64_t>(p.m), n = static_cast<uint64_t>(o.b_rows), k = static_cast<uint64_t>(o.k);
+    const bool ok = make_sw128_map(&maps.a[i], o.a.data, false, o.a_by_k ? k : m, o.a_by_k ? m : k, o.a_by_k ? kBlockK : kRowsPerCta, o.a.stride) &&
+                    make_sw128_map(&maps.b[i], o.b.data, false, kBByK ? k : n, kBByK ? n : k, kBByK ? kBlockK : Cfg::kBRows, o.b.stride) &&
+                    make_store_map(&maps.out[i], o.out, false, static_cast<uint64_t>(p.n), kEpilogue == Epilogue::kGatedBack ? 2 : 1, m);
+    if (!ok) return cudaErrorInvalidValue;
     p.k_blocks = static_cast<int>((k + kBlockK - 1) / kBlockK);
     p.m_tiles = static_cast<int>((p.m + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta));
     p.n_tiles = (p.n + kColumns - 1) / kColumns;
-    if (i < count) total += static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-    if (i == 0) args.tiles[0] = total;
+    p.a_by_k = o.a_by_k ? 1 : 0;
+    total += static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+    args.tiles[i] = static_cast<int>(total);
   }
-  args.tiles[1] = total;
-  if (total > (1ll << 30)) return cudaErrorInvalidValue;
-  int64_t pairs = sm_count_of_current_device() / 2;
-  if (pairs > total) pairs = total;
-  return launch_chained(kernel, dim3(static_cast<unsigned>(2 * pairs)), kThreads, Cfg::kSmemBytes, stream, chained, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], args);
+  args.schedule = schedule;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(2 * schedule.pairs)), kThreads, Cfg::kSmemBytes, stream, chained, maps, args);
 }
 
 template <Epilogue kEpilogue, bool kAByK, bool kBByK>
-cudaError_t launch_form(const Args& args, const Operands* operands, int count, const int64_t* depth, cudaStream_t stream, bool chained) {
+cudaError_t launch_form(Args& args, const Operands* operands, int count, cudaStream_t stream, bool chained) {
   // Tiles of 256 columns, or of 128 where those end sooner: they take 0.55 of the time each (one pair brings 48 KB instead of 64 KB a K
   // block, for half the products), and few or unlucky numbers of the wide ones leave pairs without work.  512 rows of 7168 x 2048
   // (32 and 56 wide tiles): forward 58.0 -> 45.0 us; 1111 rows of 2880 x 1416: backward 66.8 -> 58.8; 2048 rows of 7168 x 2048 (128 and 224) stay
   // wide: 131.9 us, 141.2 in narrow tiles.
-  constexpr int kWide = kEpilogue == Epilogue::kGated ? 128 : 256;  // output channels
-  int64_t wide = 0, narrow = 0;
-  for (int i = 0; i < count; ++i) {
-    const Problem& p = args.problem[i];
-    const int64_t m_tiles = (p.m + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta);
-    wide += m_tiles * ((p.n + kWide - 1) / kWide);
-    narrow += m_tiles * ((p.n + kWide / 2 - 1) / (kWide / 2));
-  }
-  const int64_t pairs = sm_count_of_current_device() / 2;
-  if ((narrow + pairs - 1) / pairs * 11 < (wide + pairs - 1) / pairs * 20) {
-    return launch_tiles<kEpilogue, kAByK, kBByK, 128>(args, operands, count, depth, stream, chained);
-  }
-  return launch_tiles<kEpilogue, kAByK, kBByK, 256>(args, operands, count, depth, stream, chained);
+  const Plan wide = plan_form<kEpilogue, 256>(args, operands, count), narrow = plan_form<kEpilogue, 128>(args, operands, count);
+  if (wide.blocks < 0 || narrow.blocks < 0) return cudaErrorInvalidValue;
+  if (narrow.blocks * 11 < wide.blocks * 20) return launch_tiles<kEpilogue, kAByK, kBByK, 128>(args, operands, count, narrow.schedule, stream, chained);
+  return launch_tiles<kEpilogue, kAByK, kBByK, 256>(args, operands, count, wide.schedule, stream, chained);
 }
 
 // Where the kernels of the operators without a workspace of their own report a wait that gave up.
@@ -524,9 +599,8 @@ cudaError_t launch_gated_projection(const uint16_t* x, int64_t x_stride, const u
   args.activation = activation;
   args.limit = limit;
   args.status = status;
-  const Operands operands = {{x, x_stride}, {w13, hidden}, 2 * static_cast<int64_t>(inter), h};
-  const int64_t depth = hidden;
-  return launch_form<Epilogue::kGated, false, false>(args, &operands, 1, &depth, stream, chained);
+  const Operands operands = {{x, x_stride}, {w13, hidden}, 2 * static_cast<int64_t>(inter), h, hidden, false};
+  return launch_form<Epilogue::kGated, false, false>(args, &operands, 1, stream, chained);
 }
 
 cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const uint16_t* w2, const float* derivatives, int64_t rows, int hidden,
@@ -536,30 +610,38 @@ cudaError_t launch_gated_backward(const uint16_t* dy, int64_t dy_stride, const u
   args.problem[0].n = inter;
   args.derivatives = reinterpret_cast<float4*>(const_cast<float*>(derivatives));
   args.status = status;
-  const Operands operands = {{dy, dy_stride}, {w2, inter}, inter, d_gate_up};
-  const int64_t depth = hidden;
-  return launch_form<Epilogue::kGatedBack, false, true>(args, &operands, 1, &depth, stream, chained);
+  const Operands operands = {{dy, dy_stride}, {w2, inter}, inter, d_gate_up, hidden, false};
+  return launch_form<Epilogue::kGatedBack, false, true>(args, &operands, 1, stream, chained);
 }
 
-cudaError_t launch_dense_products(DenseForm form, const DenseProductArgs* products, int count, int* status, cudaStream_t stream, bool chained) {
-  if (count < 1 || count > 2) return cudaErrorInvalidValue;
+cudaError_t launch_dense_rows(const DenseProductArgs& product, int* status, cudaStream_t stream, bool chained) {
   Args args = {};
-  Operands operands[2];
-  int64_t depth[2];
-  for (int i = 0; i < count; ++i) {
-    const DenseProductArgs& p = products[i];
-    args.problem[i].m = p.m;
-    args.problem[i].n = p.n;
-    operands[i] = {p.a, p.b, p.n, p.out};
-    depth[i] = p.k;
-  }
+  args.problem[0].m = product.m;
+  args.problem[0].n = product.n;
   args.status = status;
-  switch (form) {
-    case DenseForm::kRowsRows: return launch_form<Epilogue::kPlain, false, false>(args, operands, count, depth, stream, chained);
-    case DenseForm::kRowsByK: return launch_form<Epilogue::kPlain, false, true>(args, operands, count, depth, stream, chained);
-    case DenseForm::kByKByK: return launch_form<Epilogue::kPlain, true, true>(args, operands, count, depth, stream, chained);
+  const Operands operands = {product.a, product.b, product.n, product.out, product.k, false};
+  return launch_form<Epilogue::kPlain, false, false>(args, &operands, 1, stream, chained);
+}
+
+cudaError_t launch_dense_gradients(const DenseProductArgs* products, int count, int* status, cudaStream_t stream, bool chained) {
+  if (count < 1 || count > kMaxProblems) return cudaErrorInvalidValue;
+  int64_t longest = 0;
+  for (int i = 0; i < count; ++i) longest = products[i].k > longest ? products[i].k : longest;
+  Args args = {};
+  args.status = status;
+  Operands operands[kMaxProblems];
+  int filled = 0;
+  for (int turn = 0; turn < 2; ++turn) {  // the longest K ranges in front
+    for (int i = 0; i < count; ++i) {
+      const DenseProductArgs& p = products[i];
+      if ((p.k == longest) != (turn == 0)) continue;
+      if (turn == 1 && filled > 0 && operands[filled - 1].k != longest && operands[filled - 1].k != p.k) return cudaErrorInvalidValue;
+      args.problem[filled].m = p.m;
+      args.problem[filled].n = p.n;
+      operands[filled++] = {p.a, p.b, p.n, p.out, p.k, p.a_by_k};
+    }
   }
-  return cudaErrorInvalidValue;
+  return launch_form<Epilogue::kPlain, true, true>(args, operands, count, stream, chained);
 }
 
 }  // namespace fmoe

@@ -312,6 +312,7 @@ struct DenseProductArgs {
   int64_t m;
   int n;
   int64_t k;
+  bool a_by_k;
 };
 // h = act(x Wg^T, x Wu^T) for rows x [rows, hidden] and w13 [2 * inter, hidden]; derivatives (nullable): the partial derivatives of h by gate
 // and up, fp32 in the blocks of gated.cuh.
@@ -330,9 +331,10 @@ cudaError_t launch_gated_backward_small(const uint16_t* dy, int64_t dy_stride, c
                                         int inter, uint16_t* d_gate_up, int* status, cudaStream_t stream, bool chained);
 cudaError_t launch_dense_small(const uint16_t* tokens, int64_t rows, int k, const uint16_t* weight, int n, bool weight_by_k, uint16_t* out, int* status,
                                cudaStream_t stream, bool chained);
-// One or two products of one form in a launch.
-enum class DenseForm { kRowsRows, kRowsByK, kByKByK };  // how A and B lie: [m, k] and [n, k]; [m, k] and [k, n]; [k, m] and [k, n]
-cudaError_t launch_dense_products(DenseForm form, const DenseProductArgs* products, int count, int* status, cudaStream_t stream, bool chained);
+// A and B with rows along k.
+cudaError_t launch_dense_rows(const DenseProductArgs& product, int* status, cudaStream_t stream, bool chained);
+// Up to three products with B by k, of at most two lengths of K, in one launch.
+cudaError_t launch_dense_gradients(const DenseProductArgs* products, int count, int* status, cudaStream_t stream, bool chained);
 
 // ---- dense_gemm.cu: dense W8A8 linear over tiles of kDenseMaxRows rows, one or two weight matrices in one launch.
 // Programmatic dependent of the kernel in front of it in the stream (the row quantiser that writes a_rows / a_scale).
