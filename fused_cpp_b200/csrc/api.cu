@@ -1075,9 +1075,11 @@ int check_gated_shape(const char* what, int64_t rows, int hidden, int inter) {
   }
   return FMOE_OK;
 }
-// Up to so many rows the products of the gated block go to the kernel that splits the K range (gated_small.cu).  7168 x 2048, forward, split / whole
-// K range: 64 rows 25.8 / 53 us (wide tiles), 256 rows 37.7 / 38.4, 512 rows 56.9 / 45.0; 4096 x 512: 256 rows 19.9 / 22.4, 512 rows 24.0 / 23.2.
-constexpr int64_t kGatedSmallRows = 256;
+// Up to 256 rows the products of the gated block go to the kernel that splits the K range (gated_small.cu).  7168 x 2048, forward, split / whole
+// K range: 64 rows 25.8 / 53 us (wide tiles), 256 rows 37.7 / 38.4, 512 rows 56.9 / 45.0; 4096 x 512: 256 rows 19.9 / 22.4, 512 rows 24.0 / 23.2.  Not where there is
+// little to split: 131 rows of 192 x 312, forward and backward 49.9 / 28.2; forward 110 rows of 504 x 288 14.7 / 12.1, 88 rows of 352 x 1752 12.8 / 14.5; 50 rows of 328 x 136,
+// forward and backward 21.7 / 25.8.
+bool gated_splits(int64_t rows, int64_t k) { return rows <= 256 && (rows <= 64 || k > 384); }
 bool vector_aligned(const void* pointer) { return reinterpret_cast<uintptr_t>(pointer) % 16 == 0; }
 int check_rows(const char* what, const char* name, const void* data, int64_t stride, int columns) {
   if (data == nullptr || !vector_aligned(data) || stride % 8 != 0 || stride < columns) {
@@ -1112,20 +1114,15 @@ int fmoe_gated_mlp_forward(const void* x, int64_t x_stride, const void* w13, con
   if (!vector_aligned(derivatives)) return fail(FMOE_ERR_INVALID_ARGUMENT, "%s: derivatives must be 16-byte aligned", what);
   int* words = nullptr;
   cudaError_t error = fmoe::dense_status_words(&words);
-  if (error == cudaSuccess && rows <= kGatedSmallRows) {
-    error = fmoe::launch_gated_projection_small(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
-                                                swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(derivatives), words, stream, false);
-    if (error == cudaSuccess) {
-      error = fmoe::launch_dense_small(static_cast<const uint16_t*>(h), rows, inter, static_cast<const uint16_t*>(w2), hidden, false, static_cast<uint16_t*>(y), words,
-                                       stream, true);
-    }
-    return error == cudaSuccess ? FMOE_OK : cuda_fail(error, what);
-  }
   if (error == cudaSuccess) {
-    error = fmoe::launch_gated_projection(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation,
-                                          swiglu_limit, static_cast<uint16_t*>(h), static_cast<float*>(derivatives), words, stream, false);
+    auto launch = gated_splits(rows, hidden) ? fmoe::launch_gated_projection_small : fmoe::launch_gated_projection;
+    error = launch(static_cast<const uint16_t*>(x), x_stride, static_cast<const uint16_t*>(w13), rows, hidden, inter, activation, swiglu_limit,
+                   static_cast<uint16_t*>(h), static_cast<float*>(derivatives), words, stream, false);
   }
-  if (error == cudaSuccess) {
+  if (error == cudaSuccess && gated_splits(rows, inter)) {
+    error = fmoe::launch_dense_small(static_cast<const uint16_t*>(h), rows, inter, static_cast<const uint16_t*>(w2), hidden, false, static_cast<uint16_t*>(y), words,
+                                     stream, true);
+  } else if (error == cudaSuccess) {
     const fmoe::DenseProductArgs down = {{static_cast<const uint16_t*>(h), inter}, {static_cast<const uint16_t*>(w2), inter}, static_cast<uint16_t*>(y), rows, hidden, inter, false};
     error = fmoe::launch_dense_rows(down, words, stream, true);
   }
@@ -1156,9 +1153,8 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
   int* words = nullptr;
   cudaError_t error = fmoe::dense_status_words(&words);
   bool chained = false;
-  const bool small = rows <= kGatedSmallRows;
   if (error == cudaSuccess && needs_gate_up) {
-    auto launch = small ? fmoe::launch_gated_backward_small : fmoe::launch_gated_backward;
+    auto launch = gated_splits(rows, hidden) ? fmoe::launch_gated_backward_small : fmoe::launch_gated_backward;
     error = launch(static_cast<const uint16_t*>(dy), dy_stride, static_cast<const uint16_t*>(w2), static_cast<const float*>(derivatives), rows, hidden, inter,
                    static_cast<uint16_t*>(d_gate_up), words, stream, chained);
     chained = true;
@@ -1167,7 +1163,9 @@ int fmoe_gated_mlp_backward(const void* dy, int64_t dy_stride, const void* x, in
   fmoe::DenseProductArgs products[3];
   int count = 0;
   if (dx != nullptr) {
-    if (small) {  // few tiles of a long K, which is split
+    // Few rows: few tiles of a long K, which is split, in a launch of its own.  Up to 1792 of K one launch of all three takes 0.80 to 0.97 of the time (157 rows of 1048 x 152: 37.0 ->
+    // 29.7 us), 17 rows of 592 x 1872 27.1 us instead of 25.0.
+    if (rows <= 256 && 2 * inter > 1792) {
       if (error == cudaSuccess) {
         error = fmoe::launch_dense_small(static_cast<const uint16_t*>(d_gate_up), rows, 2 * inter, static_cast<const uint16_t*>(w13), hidden, true,
                                          static_cast<uint16_t*>(dx), words, stream, chained);
