@@ -1037,8 +1037,8 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
   int* const row_slots = reinterpret_cast<int*>(reinterpret_cast<char*>(lists) + lora_slot_offset(rows));
   char* const copy = reinterpret_cast<char*>(lists) + lora_list_bytes(rows);
   uint16_t* const t = reinterpret_cast<uint16_t*>(copy + lora_copy_bytes(rows, k));
-  const bool wants_copy = fmoe::lora_wants_copy(rows, k);
-  if (rows > fmoe::kLoraFewRows && !wants_copy && reinterpret_cast<uintptr_t>(x_bf16) % 16 != 0) {
+  const bool units = fmoe::lora_units_pay(rows, k, adapters->count, adapters->rank);
+  if (rows > fmoe::kLoraFewRows && k % 8 == 0 && reinterpret_cast<uintptr_t>(x_bf16) % 16 != 0) {
     return fail(FMOE_ERR_INVALID_ARGUMENT, "i8gemm lora: more than %d rows of a multiple of 8 values must start on a 16-byte boundary", fmoe::kLoraFewRows);
   }
   const bool many = lora_pair_pays(rows, n);
@@ -1057,7 +1057,8 @@ int fmoe_i8gemm_dynamic_scaled_mm_lora(const void* x_bf16, int64_t rows, int32_t
   args.status = reinterpret_cast<int*>(base + layout.status);
   cudaError_t error = fmoe::launch_lora_front(args, static_cast<const uint16_t*>(x_bf16), k, reinterpret_cast<int8_t*>(base + layout.xq),
                                               reinterpret_cast<float*>(base + layout.scale), t, many ? lists : nullptr, row_slots,
-                                              wants_copy ? reinterpret_cast<uint16_t*>(copy) : nullptr, stream);
+                                              units && fmoe::lora_wants_copy(rows, k) ? reinterpret_cast<uint16_t*>(copy) : nullptr, units,
+                                              stream);
   if (error != cudaSuccess) return cuda_fail(error, "i8gemm lora rows and coefficients");
   args.lists = lists;
   args.row_slots = row_slots;

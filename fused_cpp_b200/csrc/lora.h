@@ -74,10 +74,16 @@ struct LoraGemmArgs {
 // Rows of x [rows, k] as int8 q [rows, k_padded] with a scale each, zeros behind k; t[plane][row][rank] = scaling[id] * (A[id] x[row]) for the rows that
 // have an adapter (the others' are left as they are), as `planes` bf16 terms; with lists, the adapters in use by every kLoraListRows rows and
 // each row's place among them.  Clears the status block.  What it writes is what the GEMM of the same arguments reads.
-// x_copy (nullable): room for rows of k padded to 8 values, wanted where lora_wants_copy.
+// x_copy (nullable): room for rows of k padded to 8 values, wanted where lora_wants_copy.  `units`: see lora_units_pay.
 cudaError_t launch_lora_front(const LoraGemmArgs& args, const uint16_t* x, int k, int8_t* q, float* scale, uint16_t* t, int* lists, int* row_slots,
-                              uint16_t* x_copy, cudaStream_t stream);
-constexpr int kLoraFewRows = 256;  // up to so many rows one launch makes rows and coefficients
+                              uint16_t* x_copy, bool units, cudaStream_t stream);
+// Whether the coefficients have a launch of their own (lora_units.cu) behind that of the rows, or one launch makes both (lora_front.cu).  One launch / two,
+// whole op: 64 rows of 3882 values, 63 adapters of rank 60 (0.9 in the rule's unit) 20.6 / 23.6 us; 80 rows of 9644, 23 of rank 60 (1.0) 42.9 / 50.7; 101 rows of 15909, 25 of 37
+// (1.4) 40.0 / 43.6; 122 rows of 5061, 26 of 128 (1.9) 48.4 / 38.2; 210 rows of 8158, 54 of 29 (2.5) 79.9 / 76.6; 179 rows of 14210, 20 of 74 (3.5) 99.4 / 63.6.
+constexpr int kLoraFewRows = 64, kLoraManyRows = 256;
+inline bool lora_units_pay(int64_t rows, int k, int adapters, int rank) {
+  return rows > kLoraManyRows || (rows > kLoraFewRows && rows * (rows < adapters ? rows : adapters) * rank * static_cast<int64_t>(k) > (3ll << 29));
+}
 inline bool lora_wants_copy(int64_t rows, int k) { return rows > kLoraFewRows && k % 8 != 0; }
 // The coefficients of many rows x, which lie on 16-byte boundaries, k padded to 8 values from a row to the next (lora_units.cu).  A programmatic dependent of the kernel in
 // front, which writes x if `behind`.

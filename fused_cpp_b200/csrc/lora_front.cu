@@ -438,7 +438,7 @@ cudaError_t launch_few_ranks(const FrontArgs& args, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_lora_front(const LoraGemmArgs& g, const uint16_t* x, int k, int8_t* q, float* scale, uint16_t* t, int* lists, int* row_slots,
-                              uint16_t* x_copy, cudaStream_t stream) {
+                              uint16_t* x_copy, bool units, cudaStream_t stream) {
   FrontArgs args = {};
   args.x = x;
   args.rows = g.rows;
@@ -453,7 +453,7 @@ cudaError_t launch_lora_front(const LoraGemmArgs& g, const uint16_t* x, int k, i
   args.row_slots = row_slots;
   args.status = g.status;
   const bool vector = k % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  if (g.rows <= kLoraFewRows) return vector ? launch_few_ranks<true>(args, stream) : launch_few_ranks<false>(args, stream);
+  if (!units) return vector ? launch_few_ranks<true>(args, stream) : launch_few_ranks<false>(args, stream);
   if (!vector && x_copy == nullptr) return cudaErrorInvalidValue;
   args.x_copy = vector ? nullptr : x_copy;
   const int64_t blocks = g.rows + (lists != nullptr ? (g.rows + kLoraListRows - 1) / kLoraListRows : 0);
