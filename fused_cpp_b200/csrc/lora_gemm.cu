@@ -30,6 +30,7 @@ constexpr int kThreads = 192;       // warp 0: TMA, warp 1: tensor memory and MM
 constexpr int kWeightBytes = kBlockM * kBlockKBytes;
 constexpr int kMaxStages = 10;
 constexpr int kMaxParts = 8;
+constexpr int kLeastTile = 16;
 constexpr int kMinPartBlocks = 2;
 constexpr int kTileRows = 128;
 constexpr int kWriters = 4;         // warps that write masked coefficients
@@ -534,8 +535,34 @@ cudaError_t launch_kernel(const KernelArgs& args, int64_t blocks, const CUtensor
   return cudaLaunchKernelEx(&config, lora_gemm_kernel<kRowTile, kDeep>, maps[0], maps[1], maps[2], args);
 }
 
+// How a call is cut: as many parts as leave all clusters resident at once, two CTAs per SM if need be, every part at least two K blocks (dense_gemm.cu).
+struct Cut {
+  int64_t blocks;
+  int row_tiles, parts;
+  bool deep;  // one CTA per SM
+};
+
 template <int kRowTile>
-cudaError_t launch_tile(KernelArgs args, cudaStream_t stream) {
+cudaError_t cut_rows(const KernelArgs& args, Cut* out) {
+  Residency one_per_sm;
+  const cudaError_t error = residency<kRowTile>(&one_per_sm);
+  if (error != cudaSuccess) return error;
+  out->row_tiles = static_cast<int>((args.g.rows + kRowTile - 1) / kRowTile);
+  out->blocks = static_cast<int64_t>((args.g.n + kBlockM - 1) / kBlockM) * out->row_tiles;
+  if (out->blocks > (1ll << 27)) return cudaErrorInvalidValue;
+  out->parts = 1;
+  for (int parts = kMaxParts; parts > 1; --parts) {
+    if (out->blocks <= 2 * one_per_sm.clusters[parts] && parts * kMinPartBlocks <= args.k_blocks) {
+      out->parts = parts;
+      break;
+    }
+  }
+  out->deep = out->blocks <= one_per_sm.clusters[out->parts];
+  return cudaSuccess;
+}
+
+template <int kRowTile>
+cudaError_t launch_tile(KernelArgs args, const Cut& cut, cudaStream_t stream) {
   const LoraGemmArgs& g = args.g;
   const uint64_t k = static_cast<uint64_t>(g.k_padded);
   CUtensorMap maps[3];
@@ -543,22 +570,28 @@ cudaError_t launch_tile(KernelArgs args, cudaStream_t stream) {
       !make_adapter_map(&maps[2], g.adapters.b, g.adapters.rank, g.n, g.adapters.count, g.adapters.b_stride, args.block.ranks, kBlockM)) {
     return cudaErrorInvalidValue;
   }
-  Residency one_per_sm;
-  const cudaError_t error = residency<kRowTile>(&one_per_sm);
-  if (error != cudaSuccess) return error;
-  args.row_tiles = static_cast<int>((g.rows + kRowTile - 1) / kRowTile);
-  const int64_t blocks = static_cast<int64_t>((g.n + kBlockM - 1) / kBlockM) * args.row_tiles;
-  if (blocks > (1ll << 27)) return cudaErrorInvalidValue;
-  // As many parts as leave all clusters resident at once, two CTAs per SM if need be, every part at least two K blocks (dense_gemm.cu).
-  args.parts = 1;
-  for (int parts = kMaxParts; parts > 1; --parts) {
-    if (blocks <= 2 * one_per_sm.clusters[parts] && parts * kMinPartBlocks <= args.k_blocks) {
-      args.parts = parts;
-      break;
-    }
+  args.row_tiles = cut.row_tiles;
+  args.parts = cut.parts;
+  return cut.deep ? launch_kernel<kRowTile, true>(args, cut.blocks, maps, stream) : launch_kernel<kRowTile, false>(args, cut.blocks, maps, stream);
+}
+
+// Tiles of kRowTile rows, or of half as many where the chip has room for them: a CTA then has fewer adapters to go through.
+template <int kRowTile>
+cudaError_t launch_rows(const KernelArgs& args, const Cut& cut, cudaStream_t stream) {
+  if constexpr (kRowTile > kLeastTile) {
+    Cut half;
+    const cudaError_t error = cut_rows<kRowTile / 2>(args, &half);
+    if (error != cudaSuccess) return error;
+    if (half.deep && half.parts >= cut.parts) return launch_rows<kRowTile / 2>(args, half, stream);
   }
-  if (blocks <= one_per_sm.clusters[args.parts]) return launch_kernel<kRowTile, true>(args, blocks, maps, stream);
-  return launch_kernel<kRowTile, false>(args, blocks, maps, stream);
+  return launch_tile<kRowTile>(args, cut, stream);
+}
+
+template <int kRowTile>
+cudaError_t launch_up_to(const KernelArgs& args, cudaStream_t stream) {
+  Cut cut;
+  const cudaError_t error = cut_rows<kRowTile>(args, &cut);
+  return error != cudaSuccess ? error : launch_rows<kRowTile>(args, cut, stream);
 }
 
 }  // namespace
@@ -570,10 +603,10 @@ cudaError_t launch_lora_gemm(const LoraGemmArgs& g, cudaStream_t stream) {
   args.rank_blocks = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
   args.block = lora_block(g.adapters.rank);
   args.vector_store = dense_vector_store(g.out, g.n, g.out_bf16 != 0) ? 1 : 0;
-  if (g.rows <= 16) return launch_tile<16>(args, stream);
-  if (g.rows <= 32) return launch_tile<32>(args, stream);
-  if (g.rows <= 64) return launch_tile<64>(args, stream);
-  return launch_tile<128>(args, stream);
+  if (g.rows <= 16) return launch_up_to<16>(args, stream);
+  if (g.rows <= 32) return launch_up_to<32>(args, stream);
+  if (g.rows <= 64) return launch_up_to<64>(args, stream);
+  return launch_up_to<128>(args, stream);
 }
 
 }  // namespace fmoe
