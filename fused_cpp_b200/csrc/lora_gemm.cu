@@ -35,11 +35,13 @@ constexpr int kMinPartBlocks = 2;
 constexpr int kTileRows = 128;
 constexpr int kWriters = 4;         // warps that write masked coefficients
 
-template <int kRowTile, bool kDeep>
+template <int kRowTile, bool kDeep, int kTerms>
 struct LoraConfig {
-  static constexpr int kTokenBytes = kRowTile * kBlockKBytes;
-  static constexpr int kStageBytes = kWeightBytes + kTokenBytes;
+  static constexpr int kLoadBytes = kWeightBytes + kRowTile * kBlockKBytes;
   static constexpr int kBudget = kDeep ? 200 * 1024 : 98 * 1024;
+  // Rows of a stage's token tile.  The terms of fp32 results' coefficients lie one under the other in it where they fit, so that a tile of B serves them all.
+  static constexpr int kHeldRows = kTerms > 1 && kRowTile < 16 * kTerms ? 16 * kTerms : kRowTile;
+  static constexpr int kStageBytes = kWeightBytes + kHeldRows * kBlockKBytes;
   static constexpr int kStages = kBudget / kStageBytes < kMaxStages ? kBudget / kStageBytes : kMaxStages;
   static constexpr int kTmemColumns = 2 * kRowTile;  // the int32 and the fp32 accumulator
   static constexpr size_t kSmemBytes = 1024 /*alignment slack*/ + static_cast<size_t>(kStages) * kStageBytes + 4096 /*control block*/;
@@ -104,11 +106,11 @@ __device__ __forceinline__ void store_value(const LoraGemmArgs& g, int64_t index
   }
 }
 
-template <int kRowTile, bool kDeep>
+template <int kRowTile, bool kDeep, int kTerms>
 __global__ void __launch_bounds__(kThreads)
 lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap token_map, const __grid_constant__ CUtensorMap b_map,
                  const __grid_constant__ KernelArgs args) {
-  using Cfg = LoraConfig<kRowTile, kDeep>;
+  using Cfg = LoraConfig<kRowTile, kDeep, kTerms>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   LoraControl* ctl = reinterpret_cast<LoraControl*>(smem + static_cast<size_t>(Cfg::kStages) * Cfg::kStageBytes);
@@ -176,10 +178,10 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
       ptx::mbar_arrive(&ctl->listed);
     }
   } else if (warp == 0) {
-    // Weights of the first stages: they depend neither on the ids nor on the kernels that may still be running.
+    // Weights of the first Cfg::kStages: they depend neither on the ids nor on the kernels that may still be running.
     if (ptx::elect_one()) {
       for (int i = 0; i < (count < Cfg::kStages ? count : Cfg::kStages); ++i) {
-        ptx::mbar_arrive_expect_tx(&ctl->full[i], Cfg::kStageBytes);
+        ptx::mbar_arrive_expect_tx(&ctl->full[i], Cfg::kLoadBytes);
         ptx::tma_load_2d(smem + static_cast<size_t>(i) * Cfg::kStageBytes, &weight_map, &ctl->full[i], (kb_begin + i) * kBlockKBytes, n0);
       }
     }
@@ -191,7 +193,10 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
   const int per_block = args.block.adapters;
   const int slot_blocks = (slots + per_block - 1) / per_block;
   const uint32_t adapter_bytes = static_cast<uint32_t>(kBlockM) * args.block.ranks * 2;  // of one adapter's tile
-  const int extra = slot_blocks * args.rank_blocks * args.g.planes;
+  const int own16 = (own + 15) & ~15;
+  const int together = kTerms * own16 <= Cfg::kHeldRows ? kTerms : 1;  // terms of the coefficients in a block
+  const int rounds = kTerms / together;
+  const int extra = slot_blocks * args.rank_blocks * rounds;
   const int all = count + extra;
 
   if (warp == 0) {
@@ -212,12 +217,12 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
       if (issuer) {
         uint8_t* stage_base = smem + static_cast<size_t>(stage) * Cfg::kStageBytes;
         if (i < count) {
-          ptx::mbar_arrive_expect_tx(&ctl->full[stage], Cfg::kStageBytes);
+          ptx::mbar_arrive_expect_tx(&ctl->full[stage], Cfg::kLoadBytes);
           ptx::tma_load_2d(stage_base, &weight_map, &ctl->full[stage], (kb_begin + i) * kBlockKBytes, n0);
           ptx::tma_load_2d(stage_base + kWeightBytes, &token_map, &ctl->full[stage], (kb_begin + i) * kBlockKBytes, static_cast<int>(row0));
         } else {
           const int u = i - count;
-          const int rank_block = u / slot_blocks / args.g.planes;
+          const int rank_block = u / slot_blocks / rounds;
           const int slot = u % slot_blocks * per_block;
           const int here = min(per_block, slots - slot);
           ptx::mbar_arrive(&ctl->vacant[stage]);
@@ -254,7 +259,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
     const uint32_t idesc_extra = ptx::make_instr_desc(false, kBlockM, (own + 15) & ~15);
     int stage = 0;
     uint32_t phase = 0;
-    uint32_t used = 0;  // stages, one bit each, whose coefficients barrier is in its odd phase
+    uint32_t used = 0;  // Cfg::kStages, one bit each, whose coefficients barrier is in its odd phase
     for (int i = 0; i < all; ++i) {
       ptx::mbar_wait(&ctl->full[stage], phase, abort_flag, status, 52);
       if (i >= count) {
@@ -271,16 +276,18 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
                                ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + ks * kUmmaKBytes), idesc, (i > 0 || ks > 0) ? 1u : 0u);
           }
         } else {
-          const int rank_block = (i - count) / slot_blocks / args.g.planes;
+          const int rank_block = (i - count) / slot_blocks / rounds;
           const int here = min(per_block, slots - (i - count) % slot_blocks * per_block);
           const int steps = (min(args.block.ranks, args.g.adapters.rank - rank_block * kLoraRankBlock) + 15) >> 4;  // of an adapter
           for (int g = 0; g < here; ++g) {
             const uint32_t b_lo = (((stage_addr + g * adapter_bytes) & 0x3ffffu) >> 4) | (1u << 16);
             for (int ks = 0; ks < steps; ++ks) {
               // (B is this MMA's A operand: channels are the lanes.)
-              ptx::umma_ss<false>(tmem_base + kRowTile, static_cast<uint64_t>(b_desc_hi) << 32 | (b_lo + 2u * ks),
-                                  ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + (g * steps + ks) * kUmmaKBytes), idesc_extra,
-                                  (i > count || g > 0 || ks > 0) ? 1u : 0u);
+              for (int plane = 0; plane < together; ++plane) {
+                ptx::umma_ss<false>(tmem_base + kRowTile, static_cast<uint64_t>(b_desc_hi) << 32 | (b_lo + 2u * ks),
+                                    ptx::make_smem_desc_sw128(stage_addr + kWeightBytes + plane * own16 * kBlockKBytes + (g * steps + ks) * kUmmaKBytes), idesc_extra,
+                                    (i > count || g > 0 || ks > 0 || plane > 0) ? 1u : 0u);
+              }
             }
           }
         }
@@ -294,34 +301,33 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
     if (issuer) ptx::tcgen05_commit(&ctl->acc_full);
   } else if (extra > 0) {
     // ---------------- masked coefficients (warps 2..5) ----------------
-    // A thread holds up to eight 16-byte pieces of the own rows' coefficients, and for each adapter in turn writes those of its rows and zeros
+    // A thread holds up to eight 16-byte pieces of the own rows' coefficients (all terms of them, or one after the other), and for each adapter in turn writes those of its rows and zeros
     // for the others.  (Loaded again for every adapter, by one warp: 201 rows of 1536 -> 24576 with four adapters of rank 64 97.6 us.)
     ptx::grid_dependency_wait();
     const int thread = static_cast<int>(threadIdx.x) - 64;
     const int rank_padded = lora_rank_padded(args.g.adapters.rank);
-    const int own16 = (own + 15) & ~15;
     const uint16_t* const t_rows = args.g.t + (row0 + own_first) * rank_padded;
-    constexpr int kPieces = kRowTile * 8 / 128;  // of a thread
+    constexpr int kPieces = Cfg::kHeldRows * 8 / 128;  // of a thread
     const int share = args.block.ranks / 8;       // 16-byte pieces of an adapter in a row of 128 bytes: 2, 4 or 8
     int stage = count % Cfg::kStages;
-    uint32_t used = 0;  // stages, one bit each, whose vacant barrier is in its odd phase
-    for (int outer = 0; outer < args.rank_blocks * args.g.planes; ++outer) {
-      const int rank0 = outer / args.g.planes * kLoraRankBlock;
-      const int plane = outer % args.g.planes;
+    uint32_t used = 0;  // Cfg::kStages, one bit each, whose vacant barrier is in its odd phase
+    for (int outer = 0; outer < args.rank_blocks * rounds; ++outer) {
+      const int rank0 = outer / rounds * kLoraRankBlock;
+      const int plane0 = outer % rounds;  // together == 1, or the first of all
       const int pieces = 2 * ((min(args.block.ranks, args.g.adapters.rank - rank0) + 15) >> 4);  // of 16 bytes with ranks, in an adapter's share of a row
-      const uint16_t* const from = t_rows + static_cast<int64_t>(plane) * args.g.rows * rank_padded + rank0;
+      const uint16_t* const from = t_rows + rank0;
       uint4 value[kPieces];
       int block[kPieces];  // the row's adapter is in this block, at this piece (or in none)
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) {
         const int e = thread + 128 * p;
-        const int row = e / 8, piece = e % 8;
+        const int plane = kTerms > 1 ? (e / 8 >= own16) + (e / 8 >= 2 * own16) : 0, row = e / 8 - plane * own16, piece = e % 8;
         value[p] = make_uint4(0, 0, 0, 0);
         block[p] = -1;
-        const int slot = row < own ? ctl->slot[row] : -1;
+        const int slot = plane < together && row < own ? ctl->slot[row] : -1;  // (a row from 3 * own16 on is none of its own)
         if (slot >= 0 && slot % per_block == piece / share) {
           block[p] = slot / per_block;
-          if (piece % share < pieces) value[p] = __ldcg(reinterpret_cast<const uint4*>(from + static_cast<int64_t>(row) * rank_padded) + piece % share);
+          if (piece % share < pieces) value[p] = __ldcg(reinterpret_cast<const uint4*>(from + ((plane0 + plane) * args.g.rows + row) * rank_padded) + piece % share);
         }
       }
       for (int b = 0; b < slot_blocks; ++b) {
@@ -334,7 +340,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
           const int e = thread + 128 * p;
           const int row = e / 8, piece = e % 8;
           // The 128-byte swizzle that the operand tiles have: the 16-byte piece's number is xor-ed with the row's in its group of eight.
-          if (row < own16) *reinterpret_cast<uint4*>(to + row * kBlockKBytes + ((piece ^ (row & 7)) << 4)) = block[p] == b ? value[p] : make_uint4(0, 0, 0, 0);
+          if (row < together * own16) *reinterpret_cast<uint4*>(to + row * kBlockKBytes + ((piece ^ (row & 7)) << 4)) = block[p] == b ? value[p] : make_uint4(0, 0, 0, 0);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -350,7 +356,7 @@ lora_gemm_kernel(const __grid_constant__ CUtensorMap weight_map, const __grid_co
   const bool channel_ok = n0 + channel < n;
   const bool epilogue = warp >= 2;
   float channel_scale = 1.0f, bias = 0.0f;
-  int* exchange = reinterpret_cast<int*>(smem);                          // [rows][128 channels], once the stages are done with
+  int* exchange = reinterpret_cast<int*>(smem);                          // [rows][128 channels], once the Cfg::kStages are done with
   float* deltas = reinterpret_cast<float*>(smem) + kRowTile * kBlockM;  // [own rows][128 channels]: the adapters' sums
   const uint32_t acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
   if (epilogue) {
@@ -475,15 +481,15 @@ struct Residency {
   int clusters[kMaxParts + 1] = {};
 };
 
-template <int kRowTile, bool kDeep>
+template <int kRowTile, bool kDeep, int kTerms>
 cudaError_t configure() {
-  auto kernel = lora_gemm_kernel<kRowTile, kDeep>;
+  auto kernel = lora_gemm_kernel<kRowTile, kDeep, kTerms>;
   const cudaError_t error =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(LoraConfig<kRowTile, kDeep>::kSmemBytes));
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(LoraConfig<kRowTile, kDeep, kTerms>::kSmemBytes));
   return error != cudaSuccess ? error : cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
 }
 
-template <int kRowTile>
+template <int kRowTile, int kTerms>
 cudaError_t residency(Residency* out) {
   static std::mutex guard;  // a thread that finds the flag set has to find the table too
   static PerDeviceOnce configured;
@@ -494,13 +500,13 @@ cudaError_t residency(Residency* out) {
     *out = known[device];
     return cudaSuccess;
   }
-  cudaError_t error = configure<kRowTile, true>();
-  if (error == cudaSuccess) error = configure<kRowTile, false>();
+  cudaError_t error = configure<kRowTile, true, kTerms>();
+  if (error == cudaSuccess) error = configure<kRowTile, false, kTerms>();
   for (int parts = 1; parts <= kMaxParts && error == cudaSuccess; ++parts) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(static_cast<unsigned>(parts));
     config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = LoraConfig<kRowTile, true>::kSmemBytes;
+    config.dynamicSmemBytes = LoraConfig<kRowTile, true, kTerms>::kSmemBytes;
     cudaLaunchAttribute attribute;
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = static_cast<unsigned>(parts);
@@ -508,7 +514,7 @@ cudaError_t residency(Residency* out) {
     attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    error = cudaOccupancyMaxActiveClusters(&out->clusters[parts], lora_gemm_kernel<kRowTile, true>, &config);
+    error = cudaOccupancyMaxActiveClusters(&out->clusters[parts], lora_gemm_kernel<kRowTile, true, kTerms>, &config);
   }
   if (error != cudaSuccess) return error;
   if (device >= 0 && device < kMaxDevices) known[device] = *out;
@@ -516,12 +522,12 @@ cudaError_t residency(Residency* out) {
   return cudaSuccess;
 }
 
-template <int kRowTile, bool kDeep>
+template <int kRowTile, bool kDeep, int kTerms>
 cudaError_t launch_kernel(const KernelArgs& args, int64_t blocks, const CUtensorMap* maps, cudaStream_t stream) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(blocks * args.parts));
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = LoraConfig<kRowTile, kDeep>::kSmemBytes;
+  config.dynamicSmemBytes = LoraConfig<kRowTile, kDeep, kTerms>::kSmemBytes;
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeClusterDimension;
@@ -532,7 +538,7 @@ cudaError_t launch_kernel(const KernelArgs& args, int64_t blocks, const CUtensor
   attributes[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attributes;
   config.numAttrs = 2;
-  return cudaLaunchKernelEx(&config, lora_gemm_kernel<kRowTile, kDeep>, maps[0], maps[1], maps[2], args);
+  return cudaLaunchKernelEx(&config, lora_gemm_kernel<kRowTile, kDeep, kTerms>, maps[0], maps[1], maps[2], args);
 }
 
 // How a call is cut: as many parts as leave all clusters resident at once, two CTAs per SM if need be, every part at least two K blocks (dense_gemm.cu).
@@ -542,10 +548,10 @@ struct Cut {
   bool deep;  // one CTA per SM
 };
 
-template <int kRowTile>
+template <int kRowTile, int kTerms>
 cudaError_t cut_rows(const KernelArgs& args, Cut* out) {
   Residency one_per_sm;
-  const cudaError_t error = residency<kRowTile>(&one_per_sm);
+  const cudaError_t error = residency<kRowTile, kTerms>(&one_per_sm);
   if (error != cudaSuccess) return error;
   out->row_tiles = static_cast<int>((args.g.rows + kRowTile - 1) / kRowTile);
   out->blocks = static_cast<int64_t>((args.g.n + kBlockM - 1) / kBlockM) * out->row_tiles;
@@ -561,7 +567,7 @@ cudaError_t cut_rows(const KernelArgs& args, Cut* out) {
   return cudaSuccess;
 }
 
-template <int kRowTile>
+template <int kRowTile, int kTerms>
 cudaError_t launch_tile(KernelArgs args, const Cut& cut, cudaStream_t stream) {
   const LoraGemmArgs& g = args.g;
   const uint64_t k = static_cast<uint64_t>(g.k_padded);
@@ -572,26 +578,34 @@ cudaError_t launch_tile(KernelArgs args, const Cut& cut, cudaStream_t stream) {
   }
   args.row_tiles = cut.row_tiles;
   args.parts = cut.parts;
-  return cut.deep ? launch_kernel<kRowTile, true>(args, cut.blocks, maps, stream) : launch_kernel<kRowTile, false>(args, cut.blocks, maps, stream);
+  return cut.deep ? launch_kernel<kRowTile, true, kTerms>(args, cut.blocks, maps, stream) : launch_kernel<kRowTile, false, kTerms>(args, cut.blocks, maps, stream);
 }
 
 // Tiles of kRowTile rows, or of half as many where the chip has room for them: a CTA then has fewer adapters to go through.
-template <int kRowTile>
+template <int kRowTile, int kTerms>
 cudaError_t launch_rows(const KernelArgs& args, const Cut& cut, cudaStream_t stream) {
   if constexpr (kRowTile > kLeastTile) {
     Cut half;
-    const cudaError_t error = cut_rows<kRowTile / 2>(args, &half);
+    const cudaError_t error = cut_rows<kRowTile / 2, kTerms>(args, &half);
     if (error != cudaSuccess) return error;
-    if (half.deep && half.parts >= cut.parts) return launch_rows<kRowTile / 2>(args, half, stream);
+    if (half.deep && half.parts >= cut.parts) return launch_rows<kRowTile / 2, kTerms>(args, half, stream);
   }
-  return launch_tile<kRowTile>(args, cut, stream);
+  return launch_tile<kRowTile, kTerms>(args, cut, stream);
 }
 
-template <int kRowTile>
+template <int kRowTile, int kTerms>
 cudaError_t launch_up_to(const KernelArgs& args, cudaStream_t stream) {
   Cut cut;
-  const cudaError_t error = cut_rows<kRowTile>(args, &cut);
-  return error != cudaSuccess ? error : launch_rows<kRowTile>(args, cut, stream);
+  const cudaError_t error = cut_rows<kRowTile, kTerms>(args, &cut);
+  return error != cudaSuccess ? error : launch_rows<kRowTile, kTerms>(args, cut, stream);
+}
+
+template <int kTerms>
+cudaError_t launch_terms(const KernelArgs& args, cudaStream_t stream) {
+  if (args.g.rows <= 16) return launch_up_to<16, kTerms>(args, stream);
+  if (args.g.rows <= 32) return launch_up_to<32, kTerms>(args, stream);
+  if (args.g.rows <= 64) return launch_up_to<64, kTerms>(args, stream);
+  return launch_up_to<128, kTerms>(args, stream);
 }
 
 }  // namespace
@@ -603,10 +617,7 @@ cudaError_t launch_lora_gemm(const LoraGemmArgs& g, cudaStream_t stream) {
   args.rank_blocks = (g.adapters.rank + kLoraRankBlock - 1) / kLoraRankBlock;
   args.block = lora_block(g.adapters.rank);
   args.vector_store = dense_vector_store(g.out, g.n, g.out_bf16 != 0) ? 1 : 0;
-  if (g.rows <= 16) return launch_up_to<16>(args, stream);
-  if (g.rows <= 32) return launch_up_to<32>(args, stream);
-  if (g.rows <= 64) return launch_up_to<64>(args, stream);
-  return launch_up_to<128>(args, stream);
+  return g.planes > 1 ? launch_terms<kLoraPlanes>(args, stream) : launch_terms<1>(args, stream);
 }
 
 }  // namespace fmoe
