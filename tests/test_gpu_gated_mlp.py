@@ -307,3 +307,22 @@ def test_passes_without_a_tape_are_captured_beside_an_eager_graph(cuda_device):
     assert torch.equal(y, alive.detach())
     for got, want in zip(grads, torch.autograd.grad(alive, leaves, dy)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("tokens, hidden, inter", [
+    (65, 384, 384), (65, 392, 384), (66, 384, 392), (131, 192, 312), (200, 152, 904), (256, 896, 896), (80, 264, 1000), (257, 384, 384), (600, 4104, 256),
+    (1333, 2048, 1024), (520, 5000, 1304), (2100, 136, 2000)])
+def test_sizes_about_the_rules(cuda_device, tokens, hidden, inter):
+    """Between the forms for few and for many rows, one launch or two for the gradients, and gradients whose tiles the pairs share out unevenly."""
+    from fused_cpp_b200 import _lib, moe
+
+    x, w13, w2, dy = make(tokens, hidden, inter, seed=tokens)
+    want = run(moe, x, w13, w2, dy, "silu", 10.0)
+    check_all(want, x, w13, w2, dy, "silu", 10.0)
+    y, kept = moe.gated_mlp_forward(x, w13, w2, swiglu_limit=10.0)
+    assert torch.equal(y, want["y"])
+    for needs in ((True, False, False), (False, True, False), (False, False, True), (True, False, True), (False, True, True)):
+        got = moe.gated_mlp_backward(dy, x, w13, w2, kept, needs=needs)
+        for name, need, value in zip(("dx", "dw13", "dw2"), needs, got):
+            assert (value is None) if not need else torch.equal(value, want[name]), (needs, name)
+    assert _lib.dense_status() == (0, 0)

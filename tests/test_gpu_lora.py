@@ -245,3 +245,22 @@ def test_attention_output_then_feed_forward(cuda_device):
         assert torch.equal(y, moe.gated_mlp(projected, w13, w2, swiglu_limit=10.0))
     y.float().square().mean().backward()
     assert w13.grad.isfinite().all() and w13.grad.any() and w2.grad.any()
+
+
+@pytest.mark.parametrize("rows, k, n, count, rank", [
+    (65, 8192, 200, 65, 64), (200, 4100, 300, 40, 64), (256, 8192, 136, 16, 70), (130, 3001, 520, 130, 33), (64, 8192, 200, 65, 64), (300, 8, 40, 5, 3),
+    (270, 64, 64, 270, 17), (1500, 120, 72, 60, 130), (40, 130, 8200, 40, 7), (127, 2048, 128, 20, 200)])
+@pytest.mark.parametrize("none", [0.0, 0.6])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_sizes_about_the_rules(cuda_device, rows, k, n, count, rank, none, dtype):
+    """Between the forms of the coefficients' kernel, many adapters in a tile, K ranges of one block, and row tiles of every size; x on no boundary too."""
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, bias = make(rows, k, n, count, rank, seed=rows, none=none)
+    packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+    base = base_product(x, w, s, bias)
+    got = i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids, bias=bias, out_dtype=dtype)
+    check(got, base, x, a, b, scaling, ids)
+    assert torch.equal(got[ids < 0], base[ids < 0].to(dtype))
+    shifted = torch.empty(rows * k + 1, dtype=x.dtype, device="cuda")[1:].view(rows, k).copy_(x)
+    assert torch.equal(i8gemm.dynamic_scaled_mm_lora(shifted, packed, adapters, ids, bias=bias, out_dtype=dtype), got)
