@@ -64,7 +64,7 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 
 // Eight values of a row of x from element k on; k is a multiple of 8, what lies behind the row's end is zero.  Without kVector the row may start at any
 // element: the two 16-byte groups that hold the values are loaded and shifted into place.  A group is loaded only if a value of the row lies in it, so that nothing outside the
-// allocation's own 16-byte groups is touched.  (Element by element, 1733 values a row and 6680 rows took XX us of front.)
+// allocation's own 16-byte groups is touched.  (Element by element, and results stored so, 6680 rows of 1733 -> 8181 took 762 us, 428 like this.)
 template <bool kVector>
 __device__ __forceinline__ uint4 load_x8(const uint16_t* row, int k, int columns) {
   if (k >= columns) return make_uint4(0, 0, 0, 0);

@@ -108,7 +108,6 @@ lora_units_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     ptx::tmem_alloc(&ctl->tmem_base, kMaxColumns);
     ptx::tmem_relinquish();
   }
-  ptx::launch_dependents();  // behind the allocation: a kernel that starts early takes what is left
   // The adapters of the tile, each once in the order of its first row: warps 2..5 hold a row a thread.
   const int i = static_cast<int>(threadIdx.x) - 64;
   int mine = -1;
@@ -117,6 +116,7 @@ lora_units_kernel(const __grid_constant__ CUtensorMap x_map, const __grid_consta
     ctl->id[i] = mine;
   }
   __syncthreads();
+  ptx::launch_dependents();  // behind the allocation: a kernel that starts early takes what is left
   int first = i;
   bool owner = false;
   unsigned owners = 0;

@@ -55,7 +55,8 @@ def _require_finite(where: str, *tensors) -> None:
 def prepare_adapters(a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor | Sequence[torch.Tensor],
                      scaling: float | Sequence[float] | torch.Tensor = 1.0) -> PreparedAdapters:
     """Adapters of one projection [N, K], on the current CUDA device: bf16 a [L, R, K] and b [L, N, R], or sequences of [R_i, K] and
-    [N, R_i] of unequal ranks (R is the largest, the others are padded with zeros).  scaling: one number, or one per adapter."""
+    [N, R_i] of unequal ranks (R is the largest, the others are padded with zeros).  scaling: one number, or one per adapter.  Tensors are
+    copied, without a gradient."""
     where = "prepare_adapters"
     firsts, seconds = list(a), list(b)
     if not firsts or len(firsts) != len(seconds):
@@ -76,13 +77,14 @@ def prepare_adapters(a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor |
     device = torch.device("cuda", torch.cuda.current_device())
     a_rows = torch.zeros((count, rank, -(-k // _QUANTUM) * _QUANTUM), dtype=torch.bfloat16, device=device)
     b_rows = torch.zeros((count, n, -(-rank // _QUANTUM) * _QUANTUM), dtype=torch.bfloat16, device=device)
-    if all(first.shape[0] == rank for first in firsts) and isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor):
-        a_rows[:, :, :k] = a
-        b_rows[:, :, :rank] = b
-    else:
-        for i, (first, second) in enumerate(zip(firsts, seconds)):
-            a_rows[i, : first.shape[0], :k] = first
-            b_rows[i, :, : first.shape[0]] = second
+    with torch.no_grad():
+        if all(first.shape[0] == rank for first in firsts) and isinstance(a, torch.Tensor) and isinstance(b, torch.Tensor):
+            a_rows[:, :, :k] = a
+            b_rows[:, :, :rank] = b
+        else:
+            for i, (first, second) in enumerate(zip(firsts, seconds)):
+                a_rows[i, : first.shape[0], :k] = first
+                b_rows[i, :, : first.shape[0]] = second
     factors = factors.to(device).expand(count).contiguous()
     _require_finite(where, a_rows, b_rows, factors)
     return PreparedAdapters(a_rows, b_rows, factors, count, rank, k, n)

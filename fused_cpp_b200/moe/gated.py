@@ -5,7 +5,7 @@
 
 The trainable companion of `shared_mlp_bf16_tiled`: the same weights ([2F, H] gate rows then up rows, and [H, F]) and the same
 activations, as plain tensors that an optimiser updates.  Both projections, the activation and the product are one kernel, the down projection a
-second; the backward pass is three launches.  Sums are fp32; h = act(..) is rounded to bf16 for the down projection, as in the fused MoE
+second; the backward pass is two or three launches.  Sums are fp32; h = act(..) is rounded to bf16 for the down projection, as in the fused MoE
 operators.  `gated_mlp_forward` and `gated_mlp_backward` are the two passes for programs that keep their own tape.
 
 What a forward pass keeps for the backward pass besides its inputs, in one buffer: the partial derivatives of h by gate and by up (fp32, in an

@@ -326,3 +326,16 @@ def test_sizes_about_the_rules(cuda_device, tokens, hidden, inter):
         for name, need, value in zip(("dx", "dw13", "dw2"), needs, got):
             assert (value is None) if not need else torch.equal(value, want[name]), (needs, name)
     assert _lib.dense_status() == (0, 0)
+
+
+def test_refusals_of_the_library(cuda_device):
+    """What only the library can see is refused as the same kind of error: a kept buffer on no boundary."""
+    from fused_cpp_b200 import moe
+
+    x, w13, w2, dy = make(5, 64, 40)
+    _, kept = moe.gated_mlp_forward(x, w13, w2)
+    shifted = torch.empty(kept.numel() + 2, dtype=torch.uint8, device="cuda")[2:].copy_(kept)
+    with pytest.raises(ValueError, match="aligned"):
+        moe.gated_mlp_backward(dy, x, w13, w2, shifted)
+    with pytest.raises(ValueError, match="kept"):
+        moe.gated_mlp_backward(dy, x, w13, w2, kept[:-1])

@@ -264,3 +264,42 @@ def test_sizes_about_the_rules(cuda_device, rows, k, n, count, rank, none, dtype
     assert torch.equal(got[ids < 0], base[ids < 0].to(dtype))
     shifted = torch.empty(rows * k + 1, dtype=x.dtype, device="cuda")[1:].view(rows, k).copy_(x)
     assert torch.equal(i8gemm.dynamic_scaled_mm_lora(shifted, packed, adapters, ids, bias=bias, out_dtype=dtype), got)
+
+
+def test_adapters_in_training(cuda_device):
+    """Adapters that are leaves of a graph are copied without it, and serve under and without recorded gradients."""
+    from fused_cpp_b200 import i8gemm, lora
+
+    x, w, s, a, b, scaling, ids, _ = make(20, 64, 40, 3, 8)
+    packed = i8gemm.prepare(w, s)
+    want = i8gemm.dynamic_scaled_mm_lora(x, packed, lora.prepare_adapters(a, b, scaling), ids)
+    for first, second in ((a.clone().requires_grad_(True), b.clone().requires_grad_(True)), ([t.clone().requires_grad_(True) for t in a], list(b))):
+        adapters = lora.prepare_adapters(first, second, scaling.clone().requires_grad_(True))
+        assert not (adapters.a.requires_grad or adapters.b.requires_grad or adapters.scaling.requires_grad)
+        assert torch.equal(i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids), want)
+
+
+def test_streams_at_once(cuda_device):
+    """Calls of all forms on four streams at the same time, with the gated block's, give what they give alone."""
+    from fused_cpp_b200 import i8gemm, lora, moe
+
+    jobs = []
+    for rows, k, n, count, rank in ((300, 1000, 520, 9, 40), (200, 4104, 304, 40, 64), (40, 512, 2000, 5, 16), (2000, 400, 3200, 30, 24)):
+        x, w, s, a, b, scaling, ids, _ = make(rows, k, n, count, rank, seed=rows)
+        packed, adapters = i8gemm.prepare(w, s), lora.prepare_adapters(a, b, scaling)
+        w13, w2 = (torch.randn(shape, device="cuda").bfloat16() / 16 for shape in ((512, 256), (256, 256)))
+        rows_in = torch.randn(rows, 256, device="cuda").bfloat16()
+
+        def job(x=x, packed=packed, adapters=adapters, ids=ids, w13=w13, w2=w2, rows_in=rows_in):
+            y, kept = moe.gated_mlp_forward(rows_in, w13, w2)
+            return (i8gemm.dynamic_scaled_mm_lora(x, packed, adapters, ids), y, *moe.gated_mlp_backward(rows_in, rows_in, w13, w2, kept))
+        jobs.append((job, job(), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(20):
+        for job, want, stream in jobs:
+            with torch.cuda.stream(stream):
+                results.append((job(), want))
+    torch.cuda.synchronize()
+    for got, want in results:
+        assert all(torch.equal(g, v) for g, v in zip(got, want))
