@@ -9,8 +9,9 @@
 //
 // Two CTAs of a cluster drive one 256 x 256 tile (cta_group::2): each stages its 128 A rows and its half of the B rows (64 KB a K block of
 // 64 for the pair), which is what an SM can take from L2 while the tensor pipe works (umma2_gemm.cu has the figures).  D rows are token or weight rows and lie in
-// the lanes of tensor memory; its columns are output channels.  An epilogue warp turns 64 of them at a time into 128-byte rows of its 4 KB of shared
-// memory, and TMA stores the 32 x 64 block (and clips what lies behind the matrix).  Stored by the lanes, 16 bytes of a row each, the weight gradients of 40 rows
+// the lanes of tensor memory; its columns are output channels.  One of sixteen epilogue warps turns 32 of them at a time into 64-byte rows of its 2 KB of
+// shared memory, and TMA stores the 32 x 32 block (and clips what lies behind the matrix); eight warps with 4 KB leave their latencies open (gate_up of 8192 rows of
+// 128 x 2048: 37.1 us, 27.4 like this).  Stored by the lanes, 16 bytes of a row each, the weight gradients of 40 rows
 // of 7168 x 2048, which write 88 MB behind one K block a tile, took 42 us.  For the gated projection CTA 0 stages 128 gate rows and CTA 1 the 128 up rows of the same channels: gate and up of
 // a channel are columns c and 128 + c of the same lane.  Two accumulators of 256 columns take turns: the epilogue of a tile runs under the products of the
 // next.
@@ -34,10 +35,10 @@ constexpr int kRowsPerCta = 128;                  // A rows staged by one CTA
 constexpr int kBlockK = 64;                       // K elements of a pipeline stage: 128 bytes
 constexpr int kChunkBytes = 64 * kBlockK * 2;     // a 64 x 64 block
 constexpr int kUmmaK = 16;
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 16;
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kTmemColumns = 512;
-constexpr int kStagingBytes = 32 * 128;           // of an epilogue warp: 32 rows of 128 bytes
+constexpr int kStagingBytes = 32 * 64;            // of an epilogue warp: 32 rows of 64 bytes
 constexpr int kMaxStages = 8;
 constexpr int kTileGroup = 8;  // row tiles that are walked together (see tile_at)
 
@@ -148,7 +149,7 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t sm
                : "memory");
 }
 
-// A warp's 4 KB of shared memory on the way to a block of 32 rows of 128 bytes, in the 128-byte swizzle: lane r fills row r.
+// A warp's 2 KB of shared memory on the way to a block of 32 rows of 64 bytes, in the 64-byte swizzle: lane r fills row r.
 struct Staging {
   uint8_t* base;
   int lane;
@@ -159,7 +160,7 @@ struct Staging {
     __syncwarp();
   }
   __device__ __forceinline__ void put(int piece, uint4 value) const {
-    *reinterpret_cast<uint4*>(base + lane * 128 + ((piece ^ (lane & 7)) << 4)) = value;
+    *reinterpret_cast<uint4*>(base + lane * 64 + ((piece ^ ((lane >> 1) & 3)) << 4)) = value;
   }
   // All rows are written: store(shared-memory address) issues the copy.
   template <typename Store>
@@ -343,7 +344,7 @@ gated_pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant_
     const int quarter = warp & 3;  // the TMEM lanes a warp may read are fixed by warp id % 4
     const int chunk_first = (warp - 2) >> 2;
     constexpr int kChunkStep = kEpilogueWarps / 4;
-    constexpr int kChunks = kColumns / 64;
+    constexpr int kChunks = kColumns / 32;
     const Staging staging = {staging_base + (warp - 2) * kStagingBytes, lane};
     const uint32_t acc_lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t acc_empty_leader = map_to_cta(ptx::smem_u32(&ctl->acc_empty[0]), 0);
@@ -360,75 +361,78 @@ gated_pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant_
       ptx::mbar_wait(&ctl->acc_full[buffer], use & 1u, abort_flag, status, 44);
       ptx::tcgen05_fence_after();
       for (int chunk = chunk_first; chunk < kChunks; chunk += kChunkStep) {
-        const int col = n0 + 64 * chunk;
+        const int col = n0 + 32 * chunk;
         if (!rows_exist || col >= p.n) break;
-        const uint32_t from = acc + 64u * static_cast<uint32_t>(chunk);
+        const uint32_t from = acc + 32u * static_cast<uint32_t>(chunk);
         if constexpr (kEpilogue == Epilogue::kGated) {
           staging.begin();
+          float4* const by = args.keep && warp_row + lane < p.m ? args.derivatives + derivative_block(warp_row, col, p.n) + lane : nullptr;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            uint32_t bits[32], up_bits[32];
-            tmem_ld_x32(from + 32u * half, bits);
-            tmem_ld_x32(from + static_cast<uint32_t>(kTileN / 2) + 32u * half, up_bits);
+            uint32_t bits[16], up_bits[16];
+            tmem_ld_x16(from + 16u * half, bits);
+            tmem_ld_x16(from + static_cast<uint32_t>(kTileN / 2) + 16u * half, up_bits);
             ptx::tmem_ld_wait();
-            float4* const by = args.keep && warp_row + lane < p.m && col + 32 * half < p.n ? args.derivatives + derivative_block(warp_row, col + 32 * half, p.n) + lane : nullptr;
             with_activation<false>(args.activation, [&](auto act) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
+              for (int q = 0; q < 2; ++q) {
                 float h[8], by_gate[8], by_up[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                   gated_with_derivatives(act, __uint_as_float(bits[8 * q + j]), __uint_as_float(up_bits[8 * q + j]), args.limit, &h[j], &by_gate[j], &by_up[j]);
                 }
-                staging.put(4 * half + q, make_uint4(pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3]), pack_bf16(h[4], h[5]), pack_bf16(h[6], h[7])));
+                staging.put(2 * half + q, make_uint4(pack_bf16(h[0], h[1]), pack_bf16(h[2], h[3]), pack_bf16(h[4], h[5]), pack_bf16(h[6], h[7])));
                 if (by != nullptr) {
-                  by[64 * q] = make_float4(by_gate[0], by_gate[1], by_gate[2], by_gate[3]);
-                  by[64 * q + 32] = make_float4(by_gate[4], by_gate[5], by_gate[6], by_gate[7]);
-                  by[256 + 64 * q] = make_float4(by_up[0], by_up[1], by_up[2], by_up[3]);
-                  by[256 + 64 * q + 32] = make_float4(by_up[4], by_up[5], by_up[6], by_up[7]);
+                  float4* const at = by + 128 * half + 64 * q;
+                  at[0] = make_float4(by_gate[0], by_gate[1], by_gate[2], by_gate[3]);
+                  at[32] = make_float4(by_gate[4], by_gate[5], by_gate[6], by_gate[7]);
+                  at[256] = make_float4(by_up[0], by_up[1], by_up[2], by_up[3]);
+                  at[288] = make_float4(by_up[4], by_up[5], by_up[6], by_up[7]);
                 }
               }
             });
           }
           staging.end([&](uint32_t block) { tma_store_2d(out_map, block, col, warp_row); });
         } else if constexpr (kEpilogue == Epilogue::kGatedBack) {
-          uint32_t d_up[32];  // 64 channels, kept while those of d_gate are on their way out
+          uint32_t d_up[16];  // kept while those of d_gate are on their way out
           staging.begin();
+          const bool exists = warp_row + lane < p.m;
+          const float4* const by = args.derivatives + derivative_block(warp_row, col, p.n) + lane;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const bool exists = warp_row + lane < p.m && col + 32 * half < p.n;
-            const float4* const by = args.derivatives + derivative_block(warp_row, col + 32 * half, p.n) + lane;
-            float4 factors[16];
+            float4 factors[8];  // by gate, by up
 #pragma unroll
-            for (int q = 0; q < 16; ++q) factors[q] = exists ? __ldcs(by + 32 * q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            uint32_t bits[32];
-            tmem_ld_x32(from + 32u * half, bits);
+            for (int q = 0; q < 4; ++q) {
+              factors[q] = exists ? __ldcs(by + 128 * half + 32 * q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              factors[4 + q] = exists ? __ldcs(by + 256 + 128 * half + 32 * q) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            uint32_t bits[16];
+            tmem_ld_x16(from + 16u * half, bits);
             ptx::tmem_ld_wait();
-            uint32_t d_gate[16];
+            uint32_t d_gate[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
+            for (int q = 0; q < 4; ++q) {
               const float v[4] = {__uint_as_float(bits[4 * q]), __uint_as_float(bits[4 * q + 1]), __uint_as_float(bits[4 * q + 2]), __uint_as_float(bits[4 * q + 3])};
               d_gate[2 * q] = pack_bf16(v[0] * factors[q].x, v[1] * factors[q].y);
               d_gate[2 * q + 1] = pack_bf16(v[2] * factors[q].z, v[3] * factors[q].w);
-              d_up[16 * half + 2 * q] = pack_bf16(v[0] * factors[8 + q].x, v[1] * factors[8 + q].y);
-              d_up[16 * half + 2 * q + 1] = pack_bf16(v[2] * factors[8 + q].z, v[3] * factors[8 + q].w);
+              d_up[8 * half + 2 * q] = pack_bf16(v[0] * factors[4 + q].x, v[1] * factors[4 + q].y);
+              d_up[8 * half + 2 * q + 1] = pack_bf16(v[2] * factors[4 + q].z, v[3] * factors[4 + q].w);
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q) staging.put(4 * half + q, make_uint4(d_gate[4 * q], d_gate[4 * q + 1], d_gate[4 * q + 2], d_gate[4 * q + 3]));
+            for (int q = 0; q < 2; ++q) staging.put(2 * half + q, make_uint4(d_gate[4 * q], d_gate[4 * q + 1], d_gate[4 * q + 2], d_gate[4 * q + 3]));
           }
           staging.end([&](uint32_t block) { tma_store_3d(out_map, block, col, 0, warp_row); });
           staging.begin();
 #pragma unroll
-          for (int q = 0; q < 8; ++q) staging.put(q, make_uint4(d_up[4 * q], d_up[4 * q + 1], d_up[4 * q + 2], d_up[4 * q + 3]));
+          for (int q = 0; q < 4; ++q) staging.put(q, make_uint4(d_up[4 * q], d_up[4 * q + 1], d_up[4 * q + 2], d_up[4 * q + 3]));
           staging.end([&](uint32_t block) { tma_store_3d(out_map, block, col, 1, warp_row); });
         } else {
-          uint32_t bits[64];
+          uint32_t bits[32];
           tmem_ld_x32(from, bits);
-          tmem_ld_x32(from + 32u, bits + 32);
           ptx::tmem_ld_wait();
           staging.begin();
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
+          for (int q = 0; q < 4; ++q) {
             uint32_t words[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) words[j] = pack_bf16(__uint_as_float(bits[8 * q + 2 * j]), __uint_as_float(bits[8 * q + 2 * j + 1]));
@@ -544,7 +548,7 @@ cudaError_t launch_tiles(Args& args, const Operands* operands, int count, const 
     const uint64_t m = static_cast<uint64_t>(p.m), n = static_cast<uint64_t>(o.b_rows), k = static_cast<uint64_t>(o.k);
     const bool ok = make_sw128_map(&maps.a[i], o.a.data, false, o.a_by_k ? k : m, o.a_by_k ? m : k, o.a_by_k ? kBlockK : kRowsPerCta, o.a.stride) &&
                     make_sw128_map(&maps.b[i], o.b.data, false, kBByK ? k : n, kBByK ? n : k, kBByK ? kBlockK : Cfg::kBRows, o.b.stride) &&
-                    make_store_map(&maps.out[i], o.out, false, static_cast<uint64_t>(p.n), kEpilogue == Epilogue::kGatedBack ? 2 : 1, m);
+                    make_store_map(&maps.out[i], o.out, false, static_cast<uint64_t>(p.n), kEpilogue == Epilogue::kGatedBack ? 2 : 1, m, 64);
     if (!ok) return cudaErrorInvalidValue;
     p.k_blocks = static_cast<int>((k + kBlockK - 1) / kBlockK);
     p.m_tiles = static_cast<int>((p.m + 2 * kRowsPerCta - 1) / (2 * kRowsPerCta));

@@ -297,8 +297,9 @@ bool make_sw128_map(CUtensorMap* map, const void* base, bool int8, uint64_t rows
 bool make_adapter_map(CUtensorMap* map, const void* base, uint64_t columns, uint64_t rows, uint64_t planes, uint64_t row_stride, uint32_t box_columns,
                       uint32_t box_rows);
 
-// Result rows [rows, columns] (sides = 1) or [rows, sides, columns] of bf16 or fp32, for stores of swizzled boxes of {128 bytes, 32 rows} of a side.
-bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows);
+// Result rows [rows, columns] (sides = 1) or [rows, sides, columns] of bf16 or fp32, for stores of boxes of {row_bytes, 32 rows} of a side in the
+// swizzle of row_bytes: 128 or 64.
+bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows, uint32_t row_bytes);
 
 // ---- gated_gemm.cu: dense bf16 products of the gated feed-forward block over many rows (two-SM kernel).
 // out[m, n] = sum over k of A[m, k] B[n, k]; an operand marked `by_k` lies in memory as [k, m] or [k, n].

@@ -644,7 +644,7 @@ cudaError_t launch(Args args, cudaStream_t stream) {
   args.pair_store = g.n % 2 == 0 && reinterpret_cast<uintptr_t>(g.out) % 4 == 0;
   if (!args.tma_store) {
     maps[3] = maps[0];
-  } else if (!make_store_map(&maps[3], g.out, !g.out_bf16, static_cast<uint64_t>(g.n), 1, static_cast<uint64_t>(g.rows))) {
+  } else if (!make_store_map(&maps[3], g.out, !g.out_bf16, static_cast<uint64_t>(g.n), 1, static_cast<uint64_t>(g.rows), 128)) {
     return cudaErrorInvalidValue;
   }
   args.n_tiles = (g.n + kTileN - 1) / kTileN;

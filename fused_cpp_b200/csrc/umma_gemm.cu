@@ -765,7 +765,7 @@ bool make_adapter_map(CUtensorMap* map, const void* base, uint64_t columns, uint
                 CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows) {
+bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, uint64_t sides, uint64_t rows, uint32_t row_bytes) {
   EncodeTiledFn encode = encode_tiled_fn();
   if (encode == nullptr) return false;
   const uint64_t elem_bytes = f32 ? 4 : 2;
@@ -773,12 +773,13 @@ bool make_store_map(CUtensorMap* map, void* base, bool f32, uint64_t columns, ui
   const cuuint64_t strides3[2] = {columns * elem_bytes, sides * columns * elem_bytes};
   const cuuint64_t dims2[2] = {columns, rows};
   const cuuint64_t strides2[1] = {columns * elem_bytes};
-  const cuuint32_t inner = static_cast<cuuint32_t>(kBlockKBytes / elem_bytes);
+  const cuuint32_t inner = static_cast<cuuint32_t>(row_bytes / elem_bytes);
   const cuuint32_t box3[3] = {inner, 1, 32};
   const cuuint32_t box2[2] = {inner, 32};
   const cuuint32_t elem_strides[3] = {1, 1, 1};
   return encode(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sides > 1 ? 3 : 2, base, sides > 1 ? dims3 : dims2,
-                sides > 1 ? strides3 : strides2, sides > 1 ? box3 : box2, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                sides > 1 ? strides3 : strides2, sides > 1 ? box3 : box2, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                 CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
