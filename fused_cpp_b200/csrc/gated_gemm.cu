@@ -563,13 +563,13 @@ cudaError_t launch_tiles(Args& args, const Operands* operands, int count, const 
 
 template <Epilogue kEpilogue, bool kAByK, bool kBByK>
 cudaError_t launch_form(Args& args, const Operands* operands, int count, cudaStream_t stream, bool chained) {
-  // Tiles of 256 columns, or of 128 where those end sooner: they take 0.55 of the time each (one pair brings 48 KB instead of 64 KB a K
-  // block, for half the products), and few or unlucky numbers of the wide ones leave pairs without work.  512 rows of 7168 x 2048
-  // (32 and 56 wide tiles): forward 58.0 -> 45.0 us; 1111 rows of 2880 x 1416: backward 66.8 -> 58.8; 2048 rows of 7168 x 2048 (128 and 224) stay
-  // wide: 131.9 us, 141.2 in narrow tiles.
+  // Tiles of 256 columns, or of 128 where those end sooner: they take 0.56 to 0.64 of the time each (one pair brings 48 KB instead of 64 KB a K block, for half the
+  // products), and few or unlucky numbers of the wide ones leave pairs without work.  Narrow / wide: forward 512 rows of 7168 x 2048 45.6 / 58.9 us, 2048 rows of it 145 / 134;
+  // backward 330 rows of 832 x 1744 23.1 / 35.5, 6772 rows of 2512 x 1648 295 / 263.  Over 44 drawn shapes the backward pass takes 0.985 of the time with a rule at 0.64 of what it
+  // takes with one at 0.55, the forward pass 0.996.
   const Plan wide = plan_form<kEpilogue, 256>(args, operands, count), narrow = plan_form<kEpilogue, 128>(args, operands, count);
   if (wide.blocks < 0 || narrow.blocks < 0) return cudaErrorInvalidValue;
-  if (narrow.blocks * 11 < wide.blocks * 20) return launch_tiles<kEpilogue, kAByK, kBByK, 128>(args, operands, count, narrow.schedule, stream, chained);
+  if (narrow.blocks * 16 < wide.blocks * 25) return launch_tiles<kEpilogue, kAByK, kBByK, 128>(args, operands, count, narrow.schedule, stream, chained);
   return launch_tiles<kEpilogue, kAByK, kBByK, 256>(args, operands, count, wide.schedule, stream, chained);
 }
 
