@@ -7,11 +7,10 @@
 // fixed order.  Fragments come straight from global memory with 16-byte loads: the order of the K elements inside a group of 32 may be any as long
 // as both operands use the same, so that lane (g, q) takes elements 8q .. 8q + 7 of its row for two MMAs.  A unit is up to 32 rows of one adapter.
 //
-// Few rows (latency counts): one launch for rows and coefficients, units are made of 32 neighbouring rows by one match instruction (over 128 rows, in shared
+// One launch makes rows and coefficients of few rows (latency counts): units are made of 32 neighbouring rows by one match instruction (over 128 rows, in shared
 // memory, the list alone took 2.3 of 9.2 us of 201 rows of 1536 values, and the three of them that follow a loop of single loads are one now that
-// all loads of a warp's K range are in flight together).  Many rows (traffic counts): a unit is made of 128 rows' list, so that an adapter is read once
-// for them, in a launch of its own behind the one that quantises: with both kinds of CTA in one launch at two to an SM, 8192 rows of 16384 values took 180 us
-// instead of 150.
+// all loads of a warp's K range are in flight together).  For many rows (traffic counts), and where adapters are large (lora_units_pay), the launch here makes rows and lists
+// alone, and lora_units.cu the coefficients behind it.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
